@@ -46,7 +46,7 @@
 extern "C" {
 #endif
 
-#define TV_ABI_VERSION 4
+#define TV_ABI_VERSION 5
 
 enum tv_error {
     TV_OK = 0,
@@ -66,9 +66,11 @@ enum tv_status_bits {
     TV_STATUS_BAD_DEPTH = 16,   /* an accepted path node off its canonical depth */
     TV_STATUS_BAD_BIAS = 32,    /* a qq_bias entry other than 0 / -inf packed into visibility
                                    bits (finite values need tv_tree_attention_fp32) */
-    TV_STATUS_STALE_PLAN = 64   /* an attention plan that no longer matches the live metadata:
+    TV_STATUS_STALE_PLAN = 64,  /* an attention plan that no longer matches the live metadata:
                                    a request's prefix length or node count changed after the
                                    plan was made (tv_tree_attention_plan reads host copies) */
+    TV_STATUS_NO_PAGES = 128    /* a request that got no pages: the free list is short, or its
+                                   pages would not fit its table row */
 };
 
 /* ABI version of the loaded library (TV_ABI_VERSION at build time). */
@@ -194,6 +196,109 @@ typedef struct tv_rope_scatter_args {
 int64_t tv_sizeof_rope_scatter_args(void);
 
 int tv_rope_scatter(const tv_rope_scatter_args* args, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* per-head Q/K norm + RoPE + K/V scatter                                      */
+/* ------------------------------------------------------------------------- */
+/*
+ * The per-head RMS norms of queries and keys that precede the rotation in models/qwen3.py:193-265,
+ * with the rotation and the scatter of tv_rope_scatter in the same pass.  For every row i:
+ *     y = x * rsqrt(mean_d(x^2) + eps) * weight            x = q[i, h] or k[i, h]
+ *     z = [y1*cos - y2*sin | y2*cos + y1*sin]              HF order, halves y1, y2
+ *     out[i, h] = z(q);  k_pool[slot_i, h] = z(k);  v_pool[slot_i, h] = v[i, h]
+ * in fp32 throughout, rounded once when stored (tv_rope_scatter rounds every product, as the eager
+ * operations do).  dtype is TV_BF16, TV_F16 or TV_F32; q_weight and k_weight hold head_dim dense
+ * elements of weight_dtype (dtype or TV_F32).
+ * pool_e4m3: the pools hold one-byte e4m3 codes (element strides are bytes) and k_scale / v_scale
+ * [pages, page_size, kv_heads] the fp32 scale of each row of one head:
+ *     scale = max(amax|x| / 448, 2^-100),  code = round_to_nearest_even(x * (1 / scale))
+ * A row that holds an infinity or a NaN gets a NaN scale and zero codes.
+ * A slot of -1 marks a padding row, which writes nothing; any other position or slot out of range
+ * sets TV_STATUS_BAD_POSITION / TV_STATUS_BAD_SLOT and its row writes nothing.  Node slots must be
+ * unique.
+ */
+typedef struct tv_qk_norm_args {
+    tv_rope_scatter_args rope;
+    const void* q_weight;
+    const void* k_weight;
+    int32_t weight_dtype;
+    float eps;
+    int32_t pool_e4m3;
+    float* k_scale;          int64_t k_scale_stride[3];  /* [pages, page_size, kv_heads] */
+    float* v_scale;          int64_t v_scale_stride[3];
+} tv_qk_norm_args;
+
+int64_t tv_sizeof_qk_norm_args(void);
+
+int tv_qk_norm_rope_scatter(const tv_qk_norm_args* args, void* stream);
+
+/*
+ * tv_store_kvcache into an 8-bit cache: rows key[i] / value[i] of kv_heads heads, each head's row
+ * quantised as above, to slot slots[i]; a slot of -1 skips the row, any other slot out of range sets
+ * TV_STATUS_BAD_SLOT and skips it.
+ */
+typedef struct tv_store_e4m3_args {
+    const void* key;         int64_t key_stride[3];      /* [rows, kv_heads, D] */
+    const void* value;       int64_t value_stride[3];
+    void* k_cache;           int64_t k_cache_stride[4];  /* [pages, page_size, kv_heads, D] */
+    void* v_cache;           int64_t v_cache_stride[4];
+    float* k_scale;          int64_t k_scale_stride[3];  /* [pages, page_size, kv_heads] */
+    float* v_scale;          int64_t v_scale_stride[3];
+    int64_t pool_pages, page_size;
+    const void* slots;       int64_t slots_stride;       int32_t slots_is_int64;
+    int64_t rows;
+    int32_t kv_heads, head_dim, dtype;
+    int32_t* status;         /* optional */
+} tv_store_e4m3_args;
+
+int64_t tv_sizeof_store_e4m3_args(void);
+
+int tv_store_kvcache_e4m3(const tv_store_e4m3_args* args, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* block tables and slot maps from request lengths                             */
+/* ------------------------------------------------------------------------- */
+/*
+ * The page tables of a batch after an admission or a growth step, on the device (the reference
+ * appends pages per request on the host, engine/block_manager.py).  Request r of lengths[r] tokens
+ * needs n = ceil(lengths[r] / block_size) pages and holds h = held_counts[r] of them in
+ * held_tables[r * held_stride ...] (held_counts null: none).  It takes max(0, n - h) pages from
+ * free_pages, in request order:
+ *     tables[r, j] = held page j (j < h), the next pages of the list (h <= j < n), -1 after them
+ *     counts[r]    = max(n, h);  *taken = pages taken, always the first ones of the list
+ * A request whose pages would pass the table's width, and every request that grows from the first
+ * on that the list is short for, keeps what it holds and sets TV_STATUS_NO_PAGES.  *free_count (null:
+ * free_capacity) is the list's live length.  A negative length, a held count outside [0, held_width]
+ * or a free count outside [0, free_capacity] is clamped and sets TV_STATUS_BAD_REQUEST.
+ * tables [num_requests, width] and counts must not overlap any input.
+ */
+int tv_build_block_tables(const int32_t* lengths, const int32_t* held_tables, int64_t held_stride,
+                          int32_t held_width, const int32_t* held_counts, const int32_t* free_pages,
+                          const int32_t* free_count, int32_t free_capacity, int32_t num_requests,
+                          int32_t block_size, int32_t width, int32_t* tables, int32_t* counts,
+                          int32_t* taken, int32_t* status, void* stream);
+
+/*
+ * The maps of a packed batch of query_lens[r] rows behind cache_lens[r] cached tokens (the host
+ * loops of engine/model_runner.py:172-188 and packed_metadata.py:151-195).  Row i of request r,
+ * l rows after its first:
+ *     cu_seqlens = exclusive prefix sums of query_lens, num_requests + 1 entries
+ *     query_to_request[i] = r,  query_local_row[i] = l
+ *     positions[i] = cache_lens[r] + (depths ? depths[i] : l)
+ *     slots[i]     = page(p) * block_size + p % block_size
+ * with p = cache_lens[r] + l through block_tables[r], or p = i through arena_pages (draft trees,
+ * packed into scratch pages).  Rows from cu_seqlens[num_requests] to total_rows are padding:
+ * request -1, local row 0, position 0, slot -1.  A page outside [0, num_blocks) or past the table
+ * or arena gives slot -1 and sets TV_STATUS_BAD_SLOT; a negative cache length or position gives
+ * slot -1 and TV_STATUS_BAD_POSITION; a negative query length counts as 0 and sets
+ * TV_STATUS_BAD_REQUEST, as more rows than total_rows do (the first total_rows are mapped).
+ */
+int tv_packed_slot_maps(const int32_t* cache_lens, const int32_t* query_lens, const int32_t* block_tables,
+                        int64_t table_stride, int32_t table_width, const int32_t* arena_pages,
+                        int32_t num_arena_pages, const int32_t* depths, int32_t num_requests,
+                        int64_t total_rows, int32_t block_size, int64_t num_blocks, int32_t* cu_seqlens,
+                        int32_t* query_to_request, int32_t* query_local_row, int64_t* positions,
+                        int64_t* slots, int32_t* status, void* stream);
 
 /* ------------------------------------------------------------------------- */
 /* greedy acceptance  (speculative/jetspec/serving_ops.py:55-90)              */

@@ -8,6 +8,10 @@ Drop-in operators (same names, arguments and errors as the reference):
   accept_batch            speculative/jetspec/serving_ops.py:55-90
   rope_scatter(_prevalidated)  speculative/jetspec/tree_fusion.py:167-199
   offset_causal_mask      speculative/jetspec/prefill.py:14-26 (a chunk is a chain tree)
+Operators around them that the reference leaves to eager tensors or the host:
+  build_block_tables, packed_slot_maps     page tables and slot maps from request lengths
+  qk_norm_rope_scatter(_prevalidated)      per-head Q/K norm with the rotation and scatter
+  store_kvcache_e4m3                       the append to an 8-bit cache
 Each device operator is a hand-written gfx950 HIP kernel in libtreeverify.so.
 """
 from .packed_metadata import PackedTreeMetadata
@@ -23,6 +27,9 @@ from .tree_prefix import (
 )
 from .attention import store_kvcache
 from .tree_fusion import rope_scatter, rope_scatter_prevalidated
+from .qk_norm import qk_norm_rope_scatter, qk_norm_rope_scatter_prevalidated
+from .cache_e4m3 import store_kvcache_e4m3
+from .block_tables import build_block_tables, packed_slot_maps
 from .prefill import chain_tree_masks, offset_causal_mask
 from .state import commit_slots, copy_accepted_kv, _slots_for_blocks
 from .serving_ops import (accept_batch, accept_batch_device, accept_walk, build_child_maps, greedy_argmax,
@@ -45,6 +52,11 @@ __all__ = [
     "store_kvcache",
     "rope_scatter",
     "rope_scatter_prevalidated",
+    "qk_norm_rope_scatter",
+    "qk_norm_rope_scatter_prevalidated",
+    "store_kvcache_e4m3",
+    "build_block_tables",
+    "packed_slot_maps",
     "offset_causal_mask",
     "chain_tree_masks",
     "copy_accepted_kv",

@@ -56,6 +56,15 @@ def read_and_clear_status(device: torch.device | str | int = "cuda") -> int:
     return value
 
 
+def call(device: torch.device, entry, *args) -> int:
+    """A C entry's return code, called with `device` current: a launch goes to the current device's
+    streams only, and the caller's current device need not be the tensors' one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return entry(*args)
+    with torch.cuda.device(device):
+        return entry(*args)
+
+
 @lru_cache(maxsize=None)
 def compute_units(index: int) -> int:
     return int(torch.cuda.get_device_properties(index).multi_processor_count)

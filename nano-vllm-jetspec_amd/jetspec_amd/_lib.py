@@ -12,7 +12,7 @@ from pathlib import Path
 import threading
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libtreeverify.so"
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 TV_OK = 0
 TV_ERR_INVALID = -1
@@ -31,6 +31,7 @@ TV_STATUS_BAD_POSITION = 8
 TV_STATUS_BAD_DEPTH = 16
 TV_STATUS_BAD_BIAS = 32
 TV_STATUS_STALE_PLAN = 64
+TV_STATUS_NO_PAGES = 128
 
 TV_MAX_HOST_EOS = 8
 
@@ -69,6 +70,12 @@ EXPORTED_SYMBOLS = (
     "tv_tree_attention_fp32_chunk_keys",
     "tv_tree_attention_fp32_keys",
     "tv_tree_attention_fp32_keys_workspace_bytes",
+    "tv_sizeof_qk_norm_args",
+    "tv_qk_norm_rope_scatter",
+    "tv_sizeof_store_e4m3_args",
+    "tv_store_kvcache_e4m3",
+    "tv_build_block_tables",
+    "tv_packed_slot_maps",
 )
 
 
@@ -186,6 +193,32 @@ class RopeScatterArgs(ctypes.Structure):
     ]
 
 
+class QkNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rope", RopeScatterArgs),
+        ("q_weight", c_void_p), ("k_weight", c_void_p),
+        ("weight_dtype", c_int32), ("eps", c_float), ("pool_e4m3", c_int32),
+        ("k_scale", c_void_p), ("k_scale_stride", c_int64 * 3),
+        ("v_scale", c_void_p), ("v_scale_stride", c_int64 * 3),
+    ]
+
+
+class StoreE4m3Args(ctypes.Structure):
+    _fields_ = [
+        ("key", c_void_p), ("key_stride", c_int64 * 3),
+        ("value", c_void_p), ("value_stride", c_int64 * 3),
+        ("k_cache", c_void_p), ("k_cache_stride", c_int64 * 4),
+        ("v_cache", c_void_p), ("v_cache_stride", c_int64 * 4),
+        ("k_scale", c_void_p), ("k_scale_stride", c_int64 * 3),
+        ("v_scale", c_void_p), ("v_scale_stride", c_int64 * 3),
+        ("pool_pages", c_int64), ("page_size", c_int64),
+        ("slots", c_void_p), ("slots_stride", c_int64), ("slots_is_int64", c_int32),
+        ("rows", c_int64),
+        ("kv_heads", c_int32), ("head_dim", c_int32), ("dtype", c_int32),
+        ("status", c_void_p),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -275,6 +308,20 @@ def _declare(lib: ctypes.CDLL) -> None:
                                                            c_int32, c_int32, c_int64, POINTER(PlanInfo)]
     lib.tv_stream_capture_info.restype = c_int32
     lib.tv_stream_capture_info.argtypes = [c_void_p, POINTER(c_int32), POINTER(c_uint64)]
+    lib.tv_sizeof_qk_norm_args.restype = c_int64
+    lib.tv_sizeof_qk_norm_args.argtypes = []
+    lib.tv_qk_norm_rope_scatter.restype = c_int32
+    lib.tv_qk_norm_rope_scatter.argtypes = [POINTER(QkNormArgs), c_void_p]
+    lib.tv_sizeof_store_e4m3_args.restype = c_int64
+    lib.tv_sizeof_store_e4m3_args.argtypes = []
+    lib.tv_store_kvcache_e4m3.restype = c_int32
+    lib.tv_store_kvcache_e4m3.argtypes = [POINTER(StoreE4m3Args), c_void_p]
+    lib.tv_build_block_tables.restype = c_int32
+    lib.tv_build_block_tables.argtypes = [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
+                                          *[c_int32] * 4, *[c_void_p] * 5]
+    lib.tv_packed_slot_maps.restype = c_int32
+    lib.tv_packed_slot_maps.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p,
+                                        c_int32, c_int64, c_int32, c_int64, *[c_void_p] * 7]
     lib.tv_tree_accept.restype = c_int32
     lib.tv_tree_accept.argtypes = [c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_int32, c_void_p,
                                    c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
@@ -304,6 +351,10 @@ def library() -> ctypes.CDLL:
             raise RuntimeError("tv_tree_attention_args layout differs between library and binding")
         if lib.tv_sizeof_rope_scatter_args() != ctypes.sizeof(RopeScatterArgs):
             raise RuntimeError("tv_rope_scatter_args layout differs between library and binding")
+        if lib.tv_sizeof_qk_norm_args() != ctypes.sizeof(QkNormArgs):
+            raise RuntimeError("tv_qk_norm_args layout differs between library and binding")
+        if lib.tv_sizeof_store_e4m3_args() != ctypes.sizeof(StoreE4m3Args):
+            raise RuntimeError("tv_store_e4m3_args layout differs between library and binding")
         _lib = lib
         return lib
 
