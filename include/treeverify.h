@@ -695,6 +695,62 @@ int tv_tree_attention_fp32_chunk_keys(const int32_t* prefix_lens_host, const int
 int64_t tv_sizeof_tree_attention_fp32_args(void);
 
 /*
+ * Tree attention over an e4m3 cache (tv_store_kvcache_e4m3, tv_qk_norm_rope_scatter): the operator of
+ * tv_tree_attention with K row k of KV head h read as k_scale[k, h] * K8[k, h, :], V likewise, and
+ * the metadata's qq_bias added to the scores of tree keys (finite values included; products with
+ * log2(e) that pass float32's range stay at its ends).  Row i of request r sees the prefix positions
+ * below prefix_lens[r] and the nodes j <= i whose bias is not -inf; a row that sees nothing is zero.
+ *
+ * Queries bf16 or f16, head_dim 64, 128 or 256, any query group, page size and tree size.  Products
+ * at operand precision with fp32 sums; for bf16 output each probability times its key's scale
+ * is rounded to bf16 once, for fp32 and f16 output it is kept to 2^-17.  Code 0x7F / 0xFF is NaN: in
+ * K it makes the key's score NaN, in a prefix row of V the output's dimension, in a tree row of V
+ * the whole row for those that see it.  Masked keys never contribute, whatever their codes and scales.
+ *
+ * Every length, page and slot is read from device memory, so the launch is capturable as it is and
+ * replays follow the live values.  A request whose rows, bias or prefix lie outside total_queries,
+ * qq_bias_elems or its block table sets TV_STATUS_BAD_REQUEST and its rows are not written; a page or
+ * slot outside the pool sets TV_STATUS_BAD_PAGE and that key is skipped.
+ * The workspace (tv_tree_attention_e4m3_workspace_bytes; a negative value is an error code) is scratch
+ * of this call alone.
+ */
+typedef struct tv_tree_attention_e4m3_args {
+    const void* q;                       /* [Q, Hq, D], head dim contiguous */
+    int64_t q_stride_row, q_stride_head;
+    int32_t in_dtype;                    /* TV_BF16 or TV_F16 */
+    const void* k_pool;                  /* e4m3 codes [N, B, Hkv, D], strides in bytes */
+    const void* v_pool;
+    int64_t k_stride[4];
+    int64_t v_stride[4];
+    const float* k_scale;                /* [N, B, Hkv] */
+    const float* v_scale;
+    int64_t k_scale_stride[3];
+    int64_t v_scale_stride[3];
+    int64_t num_blocks;
+    void* out;                           /* [Q, Hq, D], head dim contiguous */
+    int64_t out_stride_row, out_stride_head;
+    int32_t out_dtype;                   /* in_dtype or TV_F32 */
+    const int32_t* cu_seqlens_q;         /* [R+1] */
+    const int32_t* prefix_lens;          /* [R] */
+    const int32_t* node_counts;          /* [R] */
+    const int32_t* block_tables;         /* [R, block_table_stride], block_table_width pages a row */
+    int64_t block_table_stride;
+    int32_t block_table_width;
+    const int64_t* tree_slots;           /* [Q] */
+    const float* qq_bias;
+    const int64_t* qq_bias_offsets;      /* [R+1] */
+    int64_t qq_bias_elems;
+    int32_t num_requests, total_queries, num_q_heads, num_kv_heads, head_dim, block_size;
+    float scale;
+    int32_t compute_units;               /* of the device: sizes the launch */
+    int32_t* status;                     /* optional */
+} tv_tree_attention_e4m3_args;
+
+int64_t tv_sizeof_tree_attention_e4m3_args(void);
+int64_t tv_tree_attention_e4m3_workspace_bytes(const tv_tree_attention_e4m3_args* args);
+int tv_tree_attention_e4m3(const tv_tree_attention_e4m3_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Allocation-free variant of tv_tree_attention.  No counterpart in the reference: it is
  * for callers that cannot allocate device memory (code under graph capture, tight serving
  * loops, harnesses that forbid allocation).  Same arguments, except that `workspace` and

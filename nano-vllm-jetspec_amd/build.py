@@ -33,6 +33,8 @@ ATTENTION_GROUP_SOURCES = (tuple(f"tv_attention_g{g}.hip" for g in GROUPS) +
                            tuple(f"tv_attention_d256_g{g}.hip" for g in GROUPS_D256))
 SOURCES = ("tv_common.cpp", "tv_plan.cpp", "tv_kvcache.hip", "tv_attention.hip", *ATTENTION_GROUP_SOURCES,
            "tv_attention_fp32.hip", "tv_attention_rows.hip",
+           "tv_attention_e4m3.hip", "tv_attention_e4m3_d64.hip", "tv_attention_e4m3_d128.hip",
+           "tv_attention_e4m3_d256.hip",
            "tv_rope.hip", "tv_qk_norm.hip", "tv_slots.hip", "tv_accept.hip", "tv_metadata.hip", "tv_plan_device.hip")
 
 # Packed-FP32 VALU instructions are kept out of the device code (they are not

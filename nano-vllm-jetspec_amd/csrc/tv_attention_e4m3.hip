@@ -1,0 +1,228 @@
+// Tree attention over an e4m3 cache: entry checks, launch shape and the merge of row blocks that
+// several workgroups share (the kernel and its mathematics are in tv_attention_e4m3.h).
+#include "tv_attention_e4m3.h"
+
+namespace tv {
+namespace {
+
+constexpr int kMergeThreads = 256;
+
+// Joins the pieces of one row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m).
+// Workgroup (x, y) looks at the boundary between the shares x and x + 1; the one at a block's first
+// boundary joins every y-th group of its rows.  Most find that their boundary ends a block or lies
+// in one that began earlier, and leave.
+template <int D, int ROWS, class T>
+__global__ void __launch_bounds__(kMergeThreads)
+e4m3_merge_kernel(const E4m3Params p) {
+    constexpr int SK = e4_step_keys(D), CH = D / 4, RPP = kMergeThreads / CH;
+    __shared__ int64_t scan[4];
+    const int64_t W = p.workgroups;
+    const int w = blockIdx.x + 1;
+    int64_t total = 0;
+    E4Place at;
+    const bool any = e4_find<ROWS, SK, kMergeThreads>(p, scan, total, at, [&](int64_t all) -> int64_t {
+        const int64_t s = e4_first_step(all, W, w);
+        return s < all ? s : -1;
+    });
+    if (!any || at.step == 0) return;
+    if (e4_first_step(total, W, w - 1) > at.begin) return;
+    const E4Request req = e4_request<ROWS, SK>(p, at.r, false);
+    const int64_t end = at.begin + at.steps;
+    const int rows = req.nodes * p.groups - at.b * ROWS < ROWS ? req.nodes * p.groups - at.b * ROWS : ROWS;
+    int pieces = 1;
+    while (e4_first_step(total, W, w - 1 + pieces) < end) ++pieces;   // total >= end ends it
+    const int ch = threadIdx.x % CH;
+    for (int row = blockIdx.y * RPP + threadIdx.x / CH; row < rows; row += gridDim.y * RPP) {
+        // The first piece is its workgroup's second one unless the block begins the share's run.
+        auto piece = [&](int i) -> int64_t {
+            const int64_t u = w - 1 + i;
+            return (2 * u + (e4_first_step(total, W, u) <= at.begin ? 1 : 0)) * ROWS + row;
+        };
+        float best = -INFINITY;
+        for (int i = 0; i < pieces; ++i) best = fmaxf(best, p.ws_ml[piece(i)].x);
+        float sum = 0.0f;
+        e4_f32x4 v = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int i = 0; i < pieces; ++i) {
+            const int64_t of = piece(i);
+            const float2 ml = p.ws_ml[of];
+            const float f = e4_weight(ml, best);
+            sum += f * ml.y;
+            v += f * *reinterpret_cast<const e4_f32x4*>(p.ws_o + of * D + 4 * ch);
+        }
+        const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int of = at.b * ROWS + row, node = of / p.groups;
+        e4_store4<T>(p, req.first_row + node, at.h * p.groups + of - node * p.groups, 4 * ch, v * scale);
+    }
+}
+
+template <int D, int ROWS>
+void launch_merge(const E4m3Params& p, bool bf16, hipStream_t s) {
+    constexpr int per_pass = kMergeThreads / (D / 4), passes = ROWS / per_pass;
+    const dim3 grid(p.workgroups - 1, passes < 8 ? passes : 8);
+    if (bf16) hipLaunchKernelGGL((e4m3_merge_kernel<D, ROWS, __bf16>), grid, dim3(kMergeThreads), 0, s, p);
+    else hipLaunchKernelGGL((e4m3_merge_kernel<D, ROWS, _Float16>), grid, dim3(kMergeThreads), 0, s, p);
+}
+
+template <int D>
+void launch_merge_d(const E4m3Params& p, int rows, bool bf16, hipStream_t s) {
+    if (rows == 32) launch_merge<D, 32>(p, bf16, s);
+    else if (rows == 64) launch_merge<D, 64>(p, bf16, s);
+    else if (rows == 128) launch_merge<D, 128>(p, bf16, s);
+    else launch_merge<D, 256>(p, bf16, s);
+}
+
+struct Launch {
+    E4m3Shape shape;
+    int32_t workgroups;
+    int64_t bytes;     // of the workspace
+};
+
+// The launch of a batch of this shape: row blocks by the rows an average request has, and as many
+// workgroups as the chip holds, or the steps a batch of this shape can have where that is fewer.
+Launch launch_of(const tv_tree_attention_e4m3_args* a) {
+    const int64_t groups = a->num_q_heads / a->num_kv_heads, rows = a->total_queries * groups;
+    const int64_t average = (rows + a->num_requests - 1) / a->num_requests;
+    Launch n;
+    n.shape = a->head_dim == 64 ? e4m3_shape_d64(average) : a->head_dim == 128 ? e4m3_shape_d128(average)
+                                                                               : e4m3_shape_d256(average);
+    const int64_t keys = e4_step_keys(a->head_dim);
+    const int64_t reach = static_cast<int64_t>(a->block_table_width) * a->block_size;
+    const int64_t blocks = (rows / n.shape.rows + a->num_requests) * a->num_kv_heads;
+    const int64_t most = blocks * ((reach + keys - 1) / keys + (a->total_queries + keys - 1) / keys);
+    const int64_t full = static_cast<int64_t>(a->compute_units) * n.shape.per_cu;
+    n.workgroups = static_cast<int32_t>(((most < full ? most : full) + 7) / 8 * 8);
+    n.bytes = 2ll * n.workgroups * n.shape.rows * (a->head_dim * 4 + 8);
+    return n;
+}
+
+int check(const tv_tree_attention_e4m3_args* a) {
+    const char* what = "tree_attention_e4m3";
+    if (!a) return fail(TV_ERR_INVALID, "%s: null args", what);
+    if (a->num_requests < 0 || a->total_queries < 0) return fail(TV_ERR_INVALID, "%s: negative batch size", what);
+    if (a->num_kv_heads < 1 || a->num_q_heads < 1 || a->num_q_heads % a->num_kv_heads) {
+        return fail(TV_ERR_INVALID, "%s: %d query heads over %d KV heads", what, a->num_q_heads, a->num_kv_heads);
+    }
+    if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) {
+        return fail(TV_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128 and 256 are built)", what, a->head_dim);
+    }
+    if (a->in_dtype != TV_BF16 && a->in_dtype != TV_F16) return fail(TV_ERR_UNSUPPORTED, "%s: queries must be bf16 or f16", what);
+    if (a->out_dtype != a->in_dtype && a->out_dtype != TV_F32) {
+        return fail(TV_ERR_UNSUPPORTED, "%s: output must be fp32 or of the queries' type", what);
+    }
+    if (!(a->scale == a->scale) || a->scale > 3.0e38f || a->scale < -3.0e38f) {
+        return fail(TV_ERR_INVALID, "%s: scale must be finite", what);
+    }
+    if (a->num_blocks < 1 || a->block_size < 1 || a->block_table_width < 0 || a->block_table_stride < 0 ||
+        a->qq_bias_elems < 0 || a->compute_units < 1) {
+        return fail(TV_ERR_INVALID, "%s: invalid pool, table or bias size", what);
+    }
+    if (a->num_blocks > 0x7fffffff / a->block_size) return fail(TV_ERR_UNSUPPORTED, "%s: pools of 2^31 slots or more", what);
+    if (static_cast<int64_t>(a->total_queries) * a->num_q_heads > 0x7fffffff - 512) {
+        return fail(TV_ERR_UNSUPPORTED, "%s: 2^31 query rows and heads or more", what);
+    }
+    return TV_OK;
+}
+
+}  // namespace
+}  // namespace tv
+
+using namespace tv;
+
+extern "C" int64_t tv_sizeof_tree_attention_e4m3_args(void) {
+    return static_cast<int64_t>(sizeof(tv_tree_attention_e4m3_args));
+}
+
+extern "C" int64_t tv_tree_attention_e4m3_workspace_bytes(const tv_tree_attention_e4m3_args* a) {
+    clear_error();
+    const int code = check(a);
+    if (code != TV_OK) return code;
+    return a->num_requests == 0 || a->total_queries == 0 ? 0 : launch_of(a).bytes;
+}
+
+extern "C" int tv_tree_attention_e4m3(const tv_tree_attention_e4m3_args* a, void* workspace, int64_t workspace_bytes,
+                                      void* stream) {
+    clear_error();
+    const int code = check(a);
+    if (code != TV_OK) return code;
+    const char* what = "tree_attention_e4m3";
+    if (a->num_requests == 0 || a->total_queries == 0) return TV_OK;
+    if (!a->q || !a->k_pool || !a->v_pool || !a->k_scale || !a->v_scale || !a->out || !a->cu_seqlens_q || !a->prefix_lens ||
+        !a->node_counts || !a->block_tables || !a->tree_slots || !a->qq_bias || !a->qq_bias_offsets) {
+        return fail(TV_ERR_INVALID, "%s: null pointer", what);
+    }
+    bool ok = aligned(a->q, 16) && a->q_stride_row % 8 == 0 && a->q_stride_head % 8 == 0 && aligned(a->k_pool, 16) &&
+              aligned(a->v_pool, 16) && a->k_stride[3] == 1 && a->v_stride[3] == 1;
+    for (int i = 0; i < 3; ++i) ok = ok && a->k_stride[i] % 16 == 0 && a->v_stride[i] % 16 == 0;
+    const int64_t piece = 16 / (a->out_dtype == TV_F32 ? 4 : 2);
+    ok = ok && aligned(a->out, 16) && a->out_stride_row % piece == 0 && a->out_stride_head % piece == 0;
+    if (!ok) return fail(TV_ERR_UNSUPPORTED, "%s: query, pool and output rows must start at 16 bytes, head dim contiguous", what);
+    const Launch n = launch_of(a);
+    if (!workspace || !aligned(workspace, 16)) return fail(TV_ERR_INVALID, "%s: null or unaligned workspace", what);
+    if (workspace_bytes < n.bytes) {
+        return fail(TV_ERR_CAPACITY, "%s: workspace of %lld bytes, %lld needed", what, static_cast<long long>(workspace_bytes),
+                    static_cast<long long>(n.bytes));
+    }
+    E4m3Params p = {};
+    p.q = a->q;
+    p.q_s0 = a->q_stride_row;
+    p.q_s1 = a->q_stride_head;
+    p.k = static_cast<const uint8_t*>(a->k_pool);
+    p.v = static_cast<const uint8_t*>(a->v_pool);
+    p.k_s0 = a->k_stride[0];
+    p.k_s1 = a->k_stride[1];
+    p.k_s2 = a->k_stride[2];
+    p.v_s0 = a->v_stride[0];
+    p.v_s1 = a->v_stride[1];
+    p.v_s2 = a->v_stride[2];
+    p.ks = a->k_scale;
+    p.vs = a->v_scale;
+    p.kc_s0 = a->k_scale_stride[0];
+    p.kc_s1 = a->k_scale_stride[1];
+    p.kc_s2 = a->k_scale_stride[2];
+    p.vc_s0 = a->v_scale_stride[0];
+    p.vc_s1 = a->v_scale_stride[1];
+    p.vc_s2 = a->v_scale_stride[2];
+    p.num_blocks = static_cast<int32_t>(a->num_blocks);
+    p.block_size = a->block_size;
+    uint32_t shift = 0;
+    while ((1ull << shift) < static_cast<uint64_t>(a->block_size)) ++shift;
+    p.div_shift = shift;
+    p.div_mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - a->block_size)) / a->block_size + 1);
+    p.out = a->out;
+    p.o_s0 = a->out_stride_row;
+    p.o_s1 = a->out_stride_head;
+    p.out_f32 = a->out_dtype == TV_F32;
+    p.cu = a->cu_seqlens_q;
+    p.plen = a->prefix_lens;
+    p.cnt = a->node_counts;
+    p.tables = a->block_tables;
+    p.t_s0 = a->block_table_stride;
+    const int64_t reach = static_cast<int64_t>(a->block_table_width) * a->block_size;
+    p.max_prefix = reach < 0x7fffff00 ? reach : 0x7fffff00;
+    p.tree_slots = a->tree_slots;
+    p.bias = a->qq_bias;
+    p.bias_off = a->qq_bias_offsets;
+    p.bias_elems = a->qq_bias_elems;
+    p.num_requests = a->num_requests;
+    p.total_queries = a->total_queries;
+    p.num_kv_heads = a->num_kv_heads;
+    p.groups = a->num_q_heads / a->num_kv_heads;
+    p.c = a->scale * 1.44269504088896340736f;
+    p.workgroups = n.workgroups;
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_ml = reinterpret_cast<float2*>(p.ws_o + 2ll * n.workgroups * n.shape.rows * a->head_dim);
+    p.status = a->status;
+    // fp32 results want the probabilities beyond bf16's 8 bits; so do f16 ones, whose step is finer.
+    const bool bf16 = a->in_dtype == TV_BF16, two = p.out_f32 || !bf16;
+    const hipStream_t s = as_stream(stream);
+    if (a->head_dim == 64) launch_e4m3_d64(p, n.shape, bf16, two, s);
+    else if (a->head_dim == 128) launch_e4m3_d128(p, n.shape, bf16, two, s);
+    else launch_e4m3_d256(p, n.shape, bf16, two, s);
+    const int launched = check_launch(what);
+    if (launched != TV_OK) return launched;
+    if (a->head_dim == 64) launch_merge_d<64>(p, n.shape.rows, bf16, s);
+    else if (a->head_dim == 128) launch_merge_d<128>(p, n.shape.rows, bf16, s);
+    else launch_merge_d<256>(p, n.shape.rows, bf16, s);
+    return check_launch("tree_attention_e4m3 merge");
+}

@@ -1,0 +1,22 @@
+// Tree attention over an e4m3 cache at head size 256.
+#include "tv_attention_e4m3.h"
+
+namespace tv {
+
+// A wave's 32 rows take 128 accumulator and 64 query registers, so one wave a SIMD; steps are half
+// as long, so the staged keys take the same LDS.
+E4m3Shape e4m3_shape_d256(int64_t average_rows) {
+    if (average_rows <= 32) return {32, 128, 2};
+    if (average_rows <= 64) return {64, 128, 2};
+    return {128, 256, 1};
+}
+
+void launch_e4m3_d256(const E4m3Params& p, const E4m3Shape& shape, bool bf16, bool two, hipStream_t s) {
+    switch (shape.rows) {
+        case 32: return e4_launch<256, 1, 2, 1>(p, bf16, two, s);
+        case 64: return e4_launch<256, 2, 1, 1>(p, bf16, two, s);
+        default: return e4_launch<256, 4, 1, 1>(p, bf16, two, s);
+    }
+}
+
+}  // namespace tv

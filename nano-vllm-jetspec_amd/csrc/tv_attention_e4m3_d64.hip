@@ -1,0 +1,24 @@
+// Tree attention over an e4m3 cache at head size 64.
+#include "tv_attention_e4m3.h"
+
+namespace tv {
+
+// Few rows put the four waves side by side on the keys, many rows on the rows; above 128 rows eight
+// waves share each key that is moved and converted, with two buffers in place of a second workgroup.
+E4m3Shape e4m3_shape_d64(int64_t average_rows) {
+    if (average_rows <= 32) return {32, 256, 2};
+    if (average_rows <= 64) return {64, 256, 2};
+    if (average_rows <= 128) return {128, 256, 2};
+    return {256, 512, 1};
+}
+
+void launch_e4m3_d64(const E4m3Params& p, const E4m3Shape& shape, bool bf16, bool two, hipStream_t s) {
+    switch (shape.rows) {
+        case 32: return e4_launch<64, 1, 4, 1>(p, bf16, two, s);
+        case 64: return e4_launch<64, 2, 2, 1>(p, bf16, two, s);
+        case 128: return e4_launch<64, 4, 1, 1>(p, bf16, two, s);
+        default: return e4_launch<64, 8, 1, 2>(p, bf16, two, s);
+    }
+}
+
+}  // namespace tv

@@ -11,7 +11,7 @@ Drop-in operators (same names, arguments and errors as the reference):
 Operators around them that the reference leaves to eager tensors or the host:
   build_block_tables, packed_slot_maps     page tables and slot maps from request lengths
   qk_norm_rope_scatter(_prevalidated)      per-head Q/K norm with the rotation and scatter
-  store_kvcache_e4m3                       the append to an 8-bit cache
+  store_kvcache_e4m3, packed_tree_attention_e4m3   an 8-bit cache: its append and its attention
 Each device operator is a hand-written gfx950 HIP kernel in libtreeverify.so.
 """
 from .packed_metadata import PackedTreeMetadata
@@ -28,7 +28,7 @@ from .tree_prefix import (
 from .attention import store_kvcache
 from .tree_fusion import rope_scatter, rope_scatter_prevalidated
 from .qk_norm import qk_norm_rope_scatter, qk_norm_rope_scatter_prevalidated
-from .cache_e4m3 import store_kvcache_e4m3
+from .cache_e4m3 import packed_tree_attention_e4m3, store_kvcache_e4m3
 from .block_tables import build_block_tables, packed_slot_maps
 from .prefill import chain_tree_masks, offset_causal_mask
 from .state import commit_slots, copy_accepted_kv, _slots_for_blocks
@@ -55,6 +55,7 @@ __all__ = [
     "qk_norm_rope_scatter",
     "qk_norm_rope_scatter_prevalidated",
     "store_kvcache_e4m3",
+    "packed_tree_attention_e4m3",
     "build_block_tables",
     "packed_slot_maps",
     "offset_causal_mask",

@@ -76,6 +76,9 @@ EXPORTED_SYMBOLS = (
     "tv_store_kvcache_e4m3",
     "tv_build_block_tables",
     "tv_packed_slot_maps",
+    "tv_sizeof_tree_attention_e4m3_args",
+    "tv_tree_attention_e4m3_workspace_bytes",
+    "tv_tree_attention_e4m3",
 )
 
 
@@ -219,6 +222,22 @@ class StoreE4m3Args(ctypes.Structure):
     ]
 
 
+class TreeAttentionE4m3Args(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_row", c_int64), ("q_stride_head", c_int64), ("in_dtype", c_int32),
+        ("k_pool", c_void_p), ("v_pool", c_void_p), ("k_stride", c_int64 * 4), ("v_stride", c_int64 * 4),
+        ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_scale_stride", c_int64 * 3), ("v_scale_stride", c_int64 * 3),
+        ("num_blocks", c_int64),
+        ("out", c_void_p), ("out_stride_row", c_int64), ("out_stride_head", c_int64), ("out_dtype", c_int32),
+        ("cu_seqlens_q", c_void_p), ("prefix_lens", c_void_p), ("node_counts", c_void_p),
+        ("block_tables", c_void_p), ("block_table_stride", c_int64), ("block_table_width", c_int32),
+        ("tree_slots", c_void_p), ("qq_bias", c_void_p), ("qq_bias_offsets", c_void_p), ("qq_bias_elems", c_int64),
+        ("num_requests", c_int32), ("total_queries", c_int32), ("num_q_heads", c_int32), ("num_kv_heads", c_int32),
+        ("head_dim", c_int32), ("block_size", c_int32),
+        ("scale", c_float), ("compute_units", c_int32), ("status", c_void_p),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -316,6 +335,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.tv_sizeof_store_e4m3_args.argtypes = []
     lib.tv_store_kvcache_e4m3.restype = c_int32
     lib.tv_store_kvcache_e4m3.argtypes = [POINTER(StoreE4m3Args), c_void_p]
+    lib.tv_sizeof_tree_attention_e4m3_args.restype = c_int64
+    lib.tv_sizeof_tree_attention_e4m3_args.argtypes = []
+    lib.tv_tree_attention_e4m3_workspace_bytes.restype = c_int64
+    lib.tv_tree_attention_e4m3_workspace_bytes.argtypes = [POINTER(TreeAttentionE4m3Args)]
+    lib.tv_tree_attention_e4m3.restype = c_int32
+    lib.tv_tree_attention_e4m3.argtypes = [POINTER(TreeAttentionE4m3Args), c_void_p, c_int64, c_void_p]
     lib.tv_build_block_tables.restype = c_int32
     lib.tv_build_block_tables.argtypes = [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
                                           *[c_int32] * 4, *[c_void_p] * 5]
@@ -355,6 +380,8 @@ def library() -> ctypes.CDLL:
             raise RuntimeError("tv_qk_norm_args layout differs between library and binding")
         if lib.tv_sizeof_store_e4m3_args() != ctypes.sizeof(StoreE4m3Args):
             raise RuntimeError("tv_store_e4m3_args layout differs between library and binding")
+        if lib.tv_sizeof_tree_attention_e4m3_args() != ctypes.sizeof(TreeAttentionE4m3Args):
+            raise RuntimeError("tv_tree_attention_e4m3_args layout differs between library and binding")
         _lib = lib
         return lib
 

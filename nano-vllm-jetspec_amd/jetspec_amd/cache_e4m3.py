@@ -55,3 +55,88 @@ def store_kvcache_e4m3(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Te
     a.status = _device.status_word(device).data_ptr()
     code = _device.call(device, _lib.library().tv_store_kvcache_e4m3, ctypes.byref(a), _device.stream_handle(device))
     _lib.check(code, "store_kvcache_e4m3")
+
+
+_METADATA_VECTORS = (("cu_seqlens_q", torch.int32), ("prefix_lens", torch.int32), ("node_counts", torch.int32),
+                     ("tree_slots", torch.int64), ("qq_bias", torch.float32), ("qq_bias_offsets", torch.int64))
+
+
+def _check_metadata(metadata, device: torch.device) -> None:
+    """The kernel reads these buffers raw: dtypes, density and sizes have to hold."""
+    requests, rows = metadata.num_requests, metadata.total_queries
+    sizes = (requests + 1, requests, requests, rows, None, requests + 1)
+    for (name, dtype), size in zip(_METADATA_VECTORS, sizes):
+        t = getattr(metadata, name)
+        if t.dtype != dtype or t.ndim != 1 or not t.is_contiguous() or (size is not None and t.numel() != size):
+            raise ValueError(f"metadata.{name} must be a contiguous {dtype} vector of the batch's size")
+        if t.device != device:
+            raise ValueError("packed attention requires CUDA queries, KV and metadata on one device")
+    tables = metadata.block_tables
+    if tables.dtype != torch.int32 or tables.ndim != 2 or tables.shape[0] != requests or tables.stride(1) != 1:
+        raise ValueError("metadata.block_tables must be int32 [requests, pages] with unit column stride")
+    if tables.device != device:
+        raise ValueError("packed attention requires CUDA queries, KV and metadata on one device")
+
+
+def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+                               v_scale: torch.Tensor, metadata, scale: float, num_queries_per_kv: int, *,
+                               output_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``packed_tree_attention`` over an e4m3 cache: one ragged launch with independent visibility.
+
+    q is [rows, heads, dim] in BF16 or FP16, dim 64, 128 or 256; the pools are e4m3 with their scales
+    and ``metadata`` is any ``PackedTreeMetadata`` (a tree of one node is a decode token, a chain tree
+    a prefill chunk).  Any query group, page size and tree size; finite ``qq_bias`` values are added
+    to the scores.  The result is new, in q's dtype or FP32; a row that sees no key is zero.  BF16
+    results round each probability times its key's scale to BF16 once, FP32 and FP16 ones keep it
+    to 2^-17.
+
+    Every length, page and slot is read on the device, so a captured call follows the staged
+    metadata, and no state is kept between calls.  Requests that reach outside the batch, the bias
+    or their table row record TV_STATUS_BAD_REQUEST (their rows are not written); pages and slots
+    outside the pool record TV_STATUS_BAD_PAGE and are skipped.
+    """
+    if q.ndim != 3 or q.shape[0] != metadata.total_queries:
+        raise ValueError("packed queries do not match the metadata")
+    if k_pool.ndim != 4 or k_pool.shape != v_pool.shape or k_pool.shape[1] != metadata.block_size:
+        raise ValueError("packed K/V page geometry does not match metadata")
+    if k_pool.dtype != E4M3 or v_pool.dtype != E4M3:
+        raise ValueError("packed_tree_attention_e4m3 takes float8_e4m3fn pools")
+    check_scales(k_pool, k_scale, "k_scale")
+    check_scales(v_pool, v_scale, "v_scale")
+    rows, heads, dim = q.shape
+    kv_heads = k_pool.shape[2]
+    if q.stride(-1) != 1 or k_pool.shape[3] != dim or dim not in (64, 128, 256):
+        raise ValueError("unsupported packed query/KV head geometry (head sizes 64, 128 and 256)")
+    if (isinstance(num_queries_per_kv, bool) or not isinstance(num_queries_per_kv, int) or num_queries_per_kv <= 0
+            or heads != kv_heads * num_queries_per_kv):
+        raise ValueError("invalid packed GQA head grouping")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("packed queries must be BF16 or FP16")
+    dtype = q.dtype if output_dtype is None else output_dtype
+    if dtype not in (q.dtype, torch.float32):
+        raise ValueError("output dtype must match the queries or be FP32")
+    device = _device.require_gpu(q, k_pool, v_pool, k_scale, v_scale, what="packed_tree_attention_e4m3")
+    _check_metadata(metadata, device)
+    out = torch.empty((rows, heads, dim), dtype=dtype, device=device)
+    if rows == 0:
+        return out
+    if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    m, tables = metadata, metadata.block_tables
+    args = _lib.TreeAttentionE4m3Args(
+        q.data_ptr(), q.stride(0), q.stride(1), _device.dtype_code(q.dtype), k_pool.data_ptr(), v_pool.data_ptr(),
+        k_pool.stride(), v_pool.stride(), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(), v_scale.stride(),
+        k_pool.shape[0], out.data_ptr(), out.stride(0), out.stride(1), _device.dtype_code(dtype),
+        m.cu_seqlens_q.data_ptr(), m.prefix_lens.data_ptr(), m.node_counts.data_ptr(), tables.data_ptr(),
+        tables.stride(0), tables.shape[1], m.tree_slots.data_ptr(), m.qq_bias.data_ptr(), m.qq_bias_offsets.data_ptr(),
+        m.qq_bias.numel(), m.num_requests, rows, heads, kv_heads, dim, m.block_size, scale,
+        _device.compute_units(device.index), _device.status_word(device).data_ptr())
+    lib = _lib.library()
+    size = lib.tv_tree_attention_e4m3_workspace_bytes(args)
+    _lib.check(min(size, 0), "packed_tree_attention_e4m3")
+    # Scratch of this call (or of the graph being captured): no two launches share one.
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    code = _device.call(device, lib.tv_tree_attention_e4m3, args, workspace.data_ptr(), size,
+                        _device.stream_handle(device))
+    _lib.check(code, "packed_tree_attention_e4m3")
+    return out
