@@ -702,10 +702,11 @@ int64_t tv_sizeof_tree_attention_fp32_args(void);
  * below prefix_lens[r] and the nodes j <= i whose bias is not -inf; a row that sees nothing is zero.
  *
  * Queries bf16 or f16, head_dim 64, 128 or 256, any query group, page size and tree size.  Products
- * at operand precision with fp32 sums; for bf16 output each probability times its key's scale
- * is rounded to bf16 once, for fp32 and f16 output it is kept to 2^-17.  Code 0x7F / 0xFF is NaN: in
- * K it makes the key's score NaN, in a prefix row of V the output's dimension, in a tree row of V
- * the whole row for those that see it.  Masked keys never contribute, whatever their codes and scales.
+ * at operand precision with fp32 sums; each probability times its key's scale is rounded to bf16
+ * once for bf16 output, kept to 2^-17 for f16 and to 2^-26 for fp32 output.  Code 0x7F / 0xFF is NaN: in
+ * K it makes the key's score NaN, in a prefix row of V the output's dimension; in a tree row of V it or
+ * a scale that is not finite makes the whole row NaN for those that see the node.  Masked keys never
+ * contribute, whatever their codes and scales.
  *
  * Every length, page and slot is read from device memory, so the launch is capturable as it is and
  * replays follow the live values.  A request whose rows, bias or prefix lie outside total_queries,

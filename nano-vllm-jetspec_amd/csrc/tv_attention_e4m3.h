@@ -8,7 +8,7 @@
 // over the request's prefix keys (through its block table) and the tree nodes its bias shows it.
 // An e4m3 code is a bf16 and an f16 value exactly, so both products run on the matrix cores at
 // operand precision with fp32 sums: 32x32x16 MFMAs, K . Q^T in the queries' type and V^T . P^T in
-// bf16, where p * vs is rounded once (or, TWO, kept to 2^-17 in two terms).  The scales never touch
+// bf16, where p * vs is rounded once or kept in TERMS bf16 terms (2: to 2^-17, 3: to 2^-26).  The scales never touch
 // the codes: ks multiplies a score, vs a probability, one multiplication each.
 //
 // Work.  A step is SK keys of one row block (ROWS score rows of one request and KV head), prefix
@@ -43,14 +43,17 @@ struct E4m3Params {
     int64_t q_s0, q_s1;
     const uint8_t* k;
     const uint8_t* v;
-    int64_t k_s0, k_s1, k_s2;
-    int64_t v_s0, v_s1, v_s2;
+    int64_t k_s0, v_s0, kc_s0, vc_s0;   // page strides of the codes and the scales
+    int32_t k_s1, k_s2, v_s1, v_s2;     // slot and head strides
+    int32_t kc_s1, kc_s2, vc_s1, vc_s2;
     const float* ks;
     const float* vs;
-    int64_t kc_s0, kc_s1, kc_s2;
-    int64_t vc_s0, vc_s1, vc_s2;
     int32_t num_blocks, block_size;
-    uint32_t div_mul, div_shift;   // pos / block_size by multiplication (E4m3Params::page_of)
+    // A whole prefix step lies in one page, K and V (and their scales) have the same strides, and a page's
+    // offsets are below 2^31; strides in bytes.
+    int32_t page_steps;
+    uint32_t f_s0, f_s1, f_c0, f_c1;
+    uint32_t div_mul, div_shift;   // pos / block_size by multiplication (e4_page_of)
     void* out;
     int64_t o_s0, o_s1;
     int32_t out_f32;
@@ -70,13 +73,6 @@ struct E4m3Params {
     float2* ws_ml;
     int32_t workgroups;            // of the attention launch
     int32_t* status;
-
-    // Quotient by the block size, exact below 2^31: multiplication by a rounded-up reciprocal
-    // (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
-    __device__ __forceinline__ int32_t page_of(int32_t pos) const {
-        const uint32_t n = static_cast<uint32_t>(pos);
-        return static_cast<int32_t>((__umulhi(div_mul, n) + n) >> div_shift);
-    }
 };
 
 // How a launch of average `rows` score rows per request and KV head is shaped.
@@ -89,10 +85,11 @@ struct E4m3Shape {
 E4m3Shape e4m3_shape_d64(int64_t average_rows);
 E4m3Shape e4m3_shape_d128(int64_t average_rows);
 E4m3Shape e4m3_shape_d256(int64_t average_rows);
-// Enqueue the attention (and nothing else); `two`: probabilities in two bf16 terms.
-void launch_e4m3_d64(const E4m3Params& p, const E4m3Shape& shape, bool bf16, bool two, hipStream_t s);
-void launch_e4m3_d128(const E4m3Params& p, const E4m3Shape& shape, bool bf16, bool two, hipStream_t s);
-void launch_e4m3_d256(const E4m3Params& p, const E4m3Shape& shape, bool bf16, bool two, hipStream_t s);
+// Enqueue the attention (and nothing else).  A probability is rounded to one bf16 term for bf16
+// output, whose own step is as coarse, and kept in two for f16 output and three for fp32.
+void launch_e4m3_d64(const E4m3Params& p, const E4m3Shape& shape, bool bf16, hipStream_t s);
+void launch_e4m3_d128(const E4m3Params& p, const E4m3Shape& shape, bool bf16, hipStream_t s);
+void launch_e4m3_d256(const E4m3Params& p, const E4m3Shape& shape, bool bf16, hipStream_t s);
 
 namespace {
 
@@ -102,6 +99,13 @@ typedef float e4_f32x16 __attribute__((ext_vector_type(16)));
 typedef float e4_f32x4 __attribute__((ext_vector_type(4)));
 typedef short e4_i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) e4_i16x4 e4_lds_i16x4;
+
+// Quotient by the block size, exact below 2^31: multiplication by a rounded-up reciprocal
+// (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+__device__ __forceinline__ int32_t e4_page_of(uint32_t mul, uint32_t shift, int32_t pos) {
+    const uint32_t n = static_cast<uint32_t>(pos);
+    return static_cast<int32_t>((__umulhi(mul, n) + n) >> shift);
+}
 
 constexpr int kE4Tile = 32;                        // keys of an MFMA tile
 // Keys of a step: 32 KiB of codes at head size 128 are in flight per workgroup, and K and V take
@@ -144,8 +148,8 @@ __device__ __forceinline__ E4Request e4_request(const E4m3Params& p, int r, bool
 // Tree nodes that some row of block b may see (nodes up to the block's last one).
 template <int ROWS>
 __device__ __forceinline__ int32_t e4_tree_keys(const E4m3Params& p, const E4Request& q, int b) {
-    const int32_t last = (b * ROWS + ROWS - 1) / p.groups;
-    return last + 1 < q.nodes ? last + 1 : q.nodes;
+    if (b + 1 == q.blocks) return q.nodes;
+    return (b * ROWS + ROWS - 1) / p.groups + 1;   // at most nodes: the block ends before the last row
 }
 
 template <int ROWS, int SK>
@@ -163,9 +167,9 @@ __device__ __forceinline__ int64_t e4_head_steps(const E4m3Params& p, const E4Re
 // A place in the order of all steps.
 struct E4Place {
     int32_t r, h, b;
-    int64_t begin;   // first step of the block, counted over the whole launch
     int32_t step;    // step within the block
     int32_t steps;   // of the block
+    int64_t begin;   // first step of the block, counted over the whole launch
 };
 
 // Counts every step of the launch into `total`, then finds step `pick(total)`.  All threads of the
@@ -308,29 +312,19 @@ __device__ __forceinline__ void e4_store4(const E4m3Params& p, int64_t row, int 
     }
 }
 
-// What a step needs, the same in every lane.
-struct E4Step {
-    int32_t r, h, b;
-    int32_t key0, count;      // first key of the step among the prefix keys or the nodes, live keys
-    int32_t tree;
-    int32_t prefix, nodes, first_row;
-    int64_t bias;
-    int32_t first, last;      // of this workgroup's run through the block
-    int32_t whole;            // the run is the whole block
-    int32_t second;           // which of the workgroup's two workspace pieces the run writes
-};
-
-template <int D, int WM, int WK, int NBUF, class T, bool TWO>
+template <int D, int WM, int WK, int NBUF, class T, int TERMS>
 __global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
 e4m3_attention_kernel(const E4m3Params p) {
     constexpr int THREADS = 64 * WM * WK, ROWS = 32 * WM, SK = e4_step_keys(D);
     constexpr int LPR = D / 16;                    // lanes that move one key's row
     constexpr int KPP = THREADS / LPR;             // keys a pass of the workgroup moves
     constexpr int PASSES = SK / KPP;
-    constexpr int TILES = SK / kE4Tile / WK;       // tiles a wave takes of a step
     constexpr int KB = SK * D * 2;                 // bytes of a step's K (or V) in LDS
+    constexpr int TILES = SK / kE4Tile / WK;       // tiles a wave takes of a step
     constexpr int NK = D / 16, NB = D / 32;        // MFMAs of a tile's scores; output blocks
+    static_assert(PASSES <= LPR, "a lane of its row for each pass's scales");
     static_assert(SK % KPP == 0 && SK % (kE4Tile * WK) == 0, "a step is whole passes and tiles");
+    static_assert(KPP % 16 == 0 || (KPP == 8 && D != 64), "the swizzle's period");
     static_assert(WK == 1 || WK * 32 * D * 4 <= NBUF * 2 * KB, "the waves' results share the staging memory");
     typedef typename E4Type<T>::vec V8;
 
@@ -349,7 +343,7 @@ e4m3_attention_kernel(const E4m3Params p) {
     // holds what they have in common: the scales of a key's heads, the keys of a head's blocks.
     if (tid < NBUF) lds_bad[tid] = 0;   // the search's barriers follow
     const int W = p.workgroups;
-    int64_t total = 0, s0 = 0, s1 = 0;
+    int64_t total = 0, s0 = 0, s1 = 0;   // all steps; this share's
     int share = 0;
     E4Place at;
     const bool any = e4_find<ROWS, SK, THREADS>(p, lds_scan, total, at, [&](int64_t all) -> int64_t {
@@ -359,110 +353,143 @@ e4m3_attention_kernel(const E4m3Params p) {
         return s0 < s1 ? s0 : -1;
     });
     if (!any) return;
-    s0 = e4_uniform(s0);
-    s1 = e4_uniform(s1);
-    int64_t todo = s1 - s0;
+    share = __builtin_amdgcn_readfirstlane(share);
+    int todo = __builtin_amdgcn_readfirstlane(static_cast<int>(s1 - s0));   // steps not yet run
 
-    // --- the order of steps -------------------------------------------------------------------
+    // Parameters that the whole prefix steps do not need are read where they are used: held over the loop,
+    // with the others, they would not fit the scalar registers.
+    typedef const __attribute__((address_space(4))) E4m3Params* Params;
+    auto cold = [&]() {
+        Params a = (Params)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(a));
+        return a;
+    };
+
+    // --- a run: steps [run0, run1) of one row block ---------------------------------------------
     E4Request req = e4_request<ROWS, SK>(p, at.r, false);
-    int n_tree = e4_tree_keys<ROWS>(p, req, at.b);
-    int run_first = 1;
-    auto describe = [&](E4Step& s) {
-        s.r = at.r;
-        s.h = at.h;
-        s.b = at.b;
-        s.tree = at.step >= req.prefix_steps;
-        s.key0 = (s.tree ? at.step - req.prefix_steps : at.step) * SK;
-        const int rest = (s.tree ? n_tree : req.prefix) - s.key0;
-        s.count = rest < SK ? rest : SK;
-        s.prefix = req.prefix;
-        s.nodes = req.nodes;
-        s.first_row = req.first_row;
-        s.bias = req.bias;
-        s.first = run_first;
-        s.last = at.step + 1 == at.steps || todo == 1;
-        s.whole = at.begin >= s0 && at.begin + at.steps <= s1;
-        s.second = at.begin >= s0;
-        run_first = s.last;
-    };
-    auto advance = [&]() {
-        --todo;
-        if (++at.step < at.steps || todo <= 0) return;
-        at.begin += at.steps;
-        at.step = 0;
-        if (++at.b == req.blocks) {
-            at.b = 0;
-            if (++at.h == p.num_kv_heads) {
-                at.h = 0;
-                do {
-                    ++at.r;
-                    req = e4_request<ROWS, SK>(p, at.r, false);
-                } while (req.blocks == 0);   // todo > 0: a later request has steps
-            }
-        }
-        at.steps = e4_block_steps<ROWS, SK>(p, req, at.b);
-        n_tree = e4_tree_keys<ROWS>(p, req, at.b);
-    };
+    int n_tree = 0;                        // nodes that the block may see
+    int run0 = at.step, run1 = 0;
+    const int32_t* table = nullptr;        // of the request
+    const int64_t* slots = nullptr;
+    const char *k_head = nullptr, *v_head = nullptr, *ks_head = nullptr, *vs_head = nullptr;   // of the KV head
+    const uint32_t s0_ = p.f_s0, s1_ = p.f_s1, c0_ = p.f_c0, c1_ = p.f_c1;
+
+    auto is_tree = [&](int i) { return i >= req.prefix_steps; };
+    auto first_key = [&](int i) { return (is_tree(i) ? i - req.prefix_steps : i) * SK; };
+    auto keys_left = [&](int i) { return (is_tree(i) ? n_tree : req.prefix) - first_key(i); };
+    auto in_page = [&](int i) { return p.page_steps && !is_tree(i) && keys_left(i) >= SK; };
 
     // --- moving a step's keys -----------------------------------------------------------------
     const int my_key = tid / LPR, my_chunk = tid % LPR;
-    int32_t entry[PASSES];
+    int32_t entry[PASSES], entry_high[PASSES];   // page numbers, or tree slots in two halves
     u32x4 kreg[PASSES], vreg[PASSES];
-    float ksr[PASSES], vsr[PASSES];
+    float ksr = 0.0f, vsr = 0.0f;   // scales of the key of pass my_chunk
     uint32_t good = 0, wrong = 0;   // passes whose key is live and found / live and not found
-    const int64_t pool_slots = static_cast<int64_t>(p.num_blocks) * p.block_size;
 
-    auto fetch_entries = [&](const E4Step& s) {
+    auto here = [](int x) {   // the same value, which the compiler cannot compute with ahead of its use
+        asm volatile("" : "+v"(x));
+        return x;
+    };
+    // LDS offsets. Keys 16 apart share a swizzle, so what differs between passes, tiles and the halves of
+    // a product is a constant; the chunks of a row are an exclusive or away from the first.
+    const int k_put = my_key * 2 * D + 16 * e4_k_chunk<D>(my_key, 2 * my_chunk);
+    const int v_put = my_key * 2 * D + 16 * e4_v_chunk<D>(my_key, 2 * my_chunk);
+    const int k_get = c * 2 * D + 16 * e4_k_chunk<D>(c, half);
+    const int v_key = 4 * half + ((lane & 15) >> 2), v_dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int v_get = v_key * 2 * D + 16 * e4_v_chunk<D>(v_key, v_dim >> 3) + 2 * (v_dim & 7);
+
+    // Loads the page numbers (tree slots: both halves) of a step; nothing looks at them before fetch_keys().
+    auto fetch_entries = [&](int i) {
+        const int key0 = first_key(i), last = keys_left(i) - 1;
+        if (in_page(i)) {
+            // One page number, the same in every lane: a vector load, which the waits on LDS do not wait for.
+            entry[0] = table[e4_page_of(p.div_mul, p.div_shift, key0) + here(0)];
+            return;
+        }
+        const Params a = cold();
+        const int my_key = here(tid) / LPR;
+        const bool tree = is_tree(i);
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int kk = i * KPP + my_key;
-            entry[i] = -1;
-            if (kk < s.count) {
-                if (s.tree) {
-                    const int64_t slot = p.tree_slots[s.first_row + s.key0 + kk];
-                    entry[i] = slot >= 0 && slot < pool_slots ? static_cast<int32_t>(slot) : -1;
-                } else {
-                    entry[i] = p.tables[s.r * p.t_s0 + p.page_of(s.key0 + kk)];
+        for (int n = 0; n < PASSES; ++n) {
+            const int kk = n * KPP + my_key, of = key0 + (kk < last ? kk : last);
+            const int32_t* from = tree ? reinterpret_cast<const int32_t*>(slots + of)
+                                       : table + e4_page_of(a->div_mul, a->div_shift, of);
+            entry[n] = from[0];
+            entry_high[n] = from[tree ? 1 : 0];
+        }
+    };
+    constexpr uint32_t kAll = (1u << PASSES) - 1;
+    const uint32_t code_of = my_key * s1_ + 16 * my_chunk, scale_of = (my_chunk * KPP + my_key) * c1_;
+    auto fetch_keys = [&](int i) {
+        const int key0 = first_key(i), left = keys_left(i);
+        good = wrong = 0;
+        // Every lane loads on every path, one whose key is past the end or not found from the pool's first
+        // row, which stage() drops: a load in a branch would be waited for where the branch ends.
+        int64_t k_of[PASSES], v_of[PASSES], ks_of = 0, vs_of = 0;
+        if (in_page(i)) {
+            const int32_t page = __builtin_amdgcn_readfirstlane(entry[0]);
+            const uint32_t offset = key0 - e4_page_of(p.div_mul, p.div_shift, key0) * p.block_size;
+            const bool found = page >= 0 && page < p.num_blocks;
+            (found ? good : wrong) = kAll;
+            const uint64_t from = found ? page : 0;
+            const uint64_t code = from * s0_ + offset * s1_;
+#pragma unroll
+            for (int n = 0; n < PASSES; ++n) k_of[n] = v_of[n] = code + n * KPP * s1_ + code_of;
+            ks_of = vs_of = from * c0_ + offset * c1_ + (my_chunk < PASSES ? scale_of : 0);
+        } else {
+            const Params a = cold();
+            const int my_key = here(tid) / LPR, my_chunk = here(tid) % LPR;
+            const bool tree = is_tree(i);
+#pragma unroll
+            for (int n = 0; n < PASSES; ++n) {
+                const int kk = n * KPP + my_key;
+                const int32_t pos = tree ? entry[n] : key0 + kk;   // a slot or a position
+                const int32_t quotient = e4_page_of(a->div_mul, a->div_shift, pos < 0 ? 0 : pos);
+                const int32_t page = !tree ? entry[n] : entry[n] < 0 || entry_high[n] != 0 ? -1 : quotient;
+                const bool live = kk < left, found = live && page >= 0 && page < a->num_blocks;
+                if (found) good |= 1u << n;
+                if (live && !found) wrong |= 1u << n;
+                const int64_t from = found ? page : 0, offset = found ? pos - quotient * a->block_size : 0;
+                k_of[n] = from * a->k_s0 + offset * a->k_s1 + 16 * my_chunk;
+                v_of[n] = from * a->v_s0 + offset * a->v_s1 + 16 * my_chunk;
+                if (my_chunk == n) {
+                    ks_of = 4 * (from * a->kc_s0 + offset * a->kc_s1);
+                    vs_of = 4 * (from * a->vc_s0 + offset * a->vc_s1);
                 }
             }
         }
-    };
-    auto fetch_keys = [&](const E4Step& s) {
-        good = wrong = 0;
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int kk = i * KPP + my_key;
-            const int32_t pos = s.tree ? entry[i] : s.key0 + kk;   // a slot or a position
-            const int32_t quotient = p.page_of(pos < 0 ? 0 : pos);
-            const int32_t page = s.tree ? (entry[i] < 0 ? -1 : quotient) : entry[i];
-            const int32_t offset = pos - quotient * p.block_size;
-            const bool live = kk < s.count, found = live && page >= 0 && page < p.num_blocks;
-            kreg[i] = u32x4{0, 0, 0, 0};
-            vreg[i] = u32x4{0, 0, 0, 0};
-            ksr[i] = vsr[i] = 0.0f;
-            if (found) {
-                good |= 1u << i;
-                kreg[i] = *reinterpret_cast<const u32x4*>(p.k + page * p.k_s0 + offset * p.k_s1 + s.h * p.k_s2 + 16 * my_chunk);
-                vreg[i] = *reinterpret_cast<const u32x4*>(p.v + page * p.v_s0 + offset * p.v_s1 + s.h * p.v_s2 + 16 * my_chunk);
-                ksr[i] = p.ks[page * p.kc_s0 + offset * p.kc_s1 + s.h * p.kc_s2];
-                vsr[i] = p.vs[page * p.vc_s0 + offset * p.vc_s1 + s.h * p.vc_s2];
-            } else if (live) {
-                wrong |= 1u << i;
-            }
+        for (int n = 0; n < PASSES; ++n) {
+            kreg[n] = *reinterpret_cast<const u32x4*>(k_head + k_of[n]);
+            vreg[n] = *reinterpret_cast<const u32x4*>(v_head + v_of[n]);
         }
+        ksr = *reinterpret_cast<const float*>(ks_head + ks_of);
+        vsr = *reinterpret_cast<const float*>(vs_head + vs_of);
     };
     // Codes to LDS as bf16/f16 values, with the step's scales; `mark` tags the buffer if a key's
     // page was not found.
-    auto stage = [&](const E4Step& s, int buf, int mark) {
+    auto stage = [&](int step, int buf, int mark) {
+        const float scale = p.c;
+        const bool tree = is_tree(step);
         char* kb = lds + buf * 2 * KB;
         char* vb = kb + KB;
+        if (__any(good != kAll)) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const uint32_t keep = (good >> i) & 1 ? 0xffffffffu : 0u;
+                kreg[i] &= keep;
+                vreg[i] &= keep;
+            }
+            if (!((good >> my_chunk) & 1)) ksr = vsr = 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int kk = i * KPP + my_key;
-            float vscale = vsr[i];
-            if (s.tree) {
-                // A product with a zero probability has to be zero: NaN codes of a node's V row turn
-                // into a NaN scale, which only rows that see the node multiply by.
+            float kscale = ksr * scale, vscale = vsr;
+            if (tree) {
+                // Rows that do not see a node have to get zero from its V row, and zero times NaN is not.
+                // So NaN codes become zeros, and they or a scale that is not finite make the node's score
+                // NaN instead, which hidden scores never show.
                 uint32_t nan = 0;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
@@ -471,7 +498,10 @@ e4m3_attention_kernel(const E4m3Params p) {
                     nan |= high;
                 }
                 const uint64_t lanes = __ballot(nan != 0);
-                if ((lanes >> (lane & ~(LPR - 1))) & ((1ull << LPR) - 1)) vscale = NAN;
+                if (((lanes >> (lane & ~(LPR - 1))) & ((1ull << LPR) - 1)) || !(fabsf(vscale) < INFINITY)) {
+                    kscale = NAN;
+                    vscale = 0.0f;
+                }
             }
             u32x4 a, b;
 #pragma unroll
@@ -481,9 +511,11 @@ e4m3_attention_kernel(const E4m3Params p) {
                 b[2 * w] = E4Type<T>::template two<false>(kreg[i][w + 2]);
                 b[2 * w + 1] = E4Type<T>::template two<true>(kreg[i][w + 2]);
             }
-            char* row = kb + kk * (2 * D);
-            *reinterpret_cast<u32x4*>(row + 16 * e4_k_chunk<D>(kk, 2 * my_chunk)) = a;
-            *reinterpret_cast<u32x4*>(row + 16 * e4_k_chunk<D>(kk, 2 * my_chunk + 1)) = b;
+            constexpr bool kAlternate = KPP % 16 != 0;   // every second pass is 8 keys off the swizzle's period
+            const int at = i * KPP * 2 * D;
+            const int kx = kAlternate && (i & 1) ? k_put ^ (8 * 16) : k_put;
+            *reinterpret_cast<u32x4*>(kb + at + kx) = a;
+            *reinterpret_cast<u32x4*>(kb + at + (kx ^ 16)) = b;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 a[2 * w] = E4Type<__bf16>::two<false>(vreg[i][w]);
@@ -491,11 +523,10 @@ e4m3_attention_kernel(const E4m3Params p) {
                 b[2 * w] = E4Type<__bf16>::two<false>(vreg[i][w + 2]);
                 b[2 * w + 1] = E4Type<__bf16>::two<true>(vreg[i][w + 2]);
             }
-            row = vb + kk * (2 * D);
-            *reinterpret_cast<u32x4*>(row + 16 * e4_v_chunk<D>(kk, 2 * my_chunk)) = a;
-            *reinterpret_cast<u32x4*>(row + 16 * e4_v_chunk<D>(kk, 2 * my_chunk + 1)) = b;
-            if (my_chunk == 0) {
-                lds_ks[buf][kk] = ksr[i] * p.c;
+            *reinterpret_cast<u32x4*>(vb + at + v_put) = a;
+            *reinterpret_cast<u32x4*>(vb + at + (v_put ^ 16)) = b;
+            if (my_chunk == i) {
+                lds_ks[buf][kk] = kscale;
                 lds_vs[buf][kk] = vscale;
                 lds_kb[buf][kk] = (good >> i) & 1 ? 0.0f : -INFINITY;
             }
@@ -512,21 +543,36 @@ e4m3_attention_kernel(const E4m3Params p) {
     float m = -INFINITY, l = 0.0f;
     int node = -1, qhead = 0;      // of this lane's row; node -1: no row
     bool wave_rows = false;        // any row of this wave
+    int nodes = 0, first_row = 0;  // of the request
+    const float* bias = nullptr;   // of this lane's node
 
-    auto start_block = [&](const E4Step& s) {
-        const int row = s.b * ROWS + 32 * wm + c;
-        wave_rows = s.b * ROWS + 32 * wm < s.nodes * p.groups;
-        const int n = row / p.groups;
-        node = n < s.nodes ? n : -1;
-        qhead = s.h * p.groups + row - n * p.groups;
+    // The block that `at` names, whose run begins at at.step.
+    auto start_block = [&]() {
+        const Params a = cold();
+        nodes = req.nodes;
+        first_row = req.first_row;
+        n_tree = e4_tree_keys<ROWS>(p, req, at.b);
+        run0 = at.step;
+        run1 = at.steps - run0 < todo ? at.steps : run0 + todo;
+        table = a->tables + at.r * a->t_s0;
+        slots = a->tree_slots + req.first_row;
+        k_head = reinterpret_cast<const char*>(a->k) + at.h * static_cast<int64_t>(a->k_s2);
+        v_head = reinterpret_cast<const char*>(a->v) + at.h * static_cast<int64_t>(a->v_s2);
+        ks_head = reinterpret_cast<const char*>(a->ks + at.h * static_cast<int64_t>(a->kc_s2));
+        vs_head = reinterpret_cast<const char*>(a->vs + at.h * static_cast<int64_t>(a->vc_s2));
+        const int groups = a->groups;
+        const int row = at.b * ROWS + 32 * wm + c;
+        wave_rows = at.b * ROWS + 32 * wm < nodes * groups;
+        const int n = row / groups;
+        node = n < nodes ? n : -1;
+        qhead = at.h * groups + row - n * groups;
+        bias = a->bias + req.bias + static_cast<int64_t>(node < 0 ? 0 : node) * nodes;
+        const T* src = static_cast<const T*>(a->q) + static_cast<int64_t>(first_row + (node < 0 ? 0 : node)) * a->q_s0 +
+                       qhead * a->q_s1 + 8 * half;
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
             u32x4 x = {0, 0, 0, 0};
-            if (node >= 0) {
-                const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(s.first_row + node) * p.q_s0 +
-                               qhead * p.q_s1 + 16 * i + 8 * half;
-                x = *reinterpret_cast<const u32x4*>(src);
-            }
+            if (node >= 0) x = *reinterpret_cast<const u32x4*>(src + 16 * i);
             qb[i] = __builtin_bit_cast(V8, x);
         }
 #pragma unroll
@@ -535,103 +581,172 @@ e4m3_attention_kernel(const E4m3Params p) {
         l = 0.0f;
     };
 
-    auto tile = [&](const E4Step& s, int buf, int t, bool masked) {
-        const char* kb = lds + buf * 2 * KB + t * kE4Tile * 2 * D;
-        const char* vb = kb + KB;
+    // K . Q^T of a tile (LDS at `kb`): element i is key 8*(i/4) + 4*half + i%4 of the tile.
+    auto products = [&](const char* kb) {
         e4_f32x16 x = {};
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(kb + c * 2 * D + 16 * e4_k_chunk<D>(c, 2 * i + half));
+            const u32x4 a = *reinterpret_cast<const u32x4*>(kb + (k_get ^ (32 * i)));
             x = E4Type<T>::run(__builtin_bit_cast(V8, a), qb[i], x);
         }
+        return x;
+    };
+    // Products to scores, with the biases; those that the row does not see become -inf, whatever they are.
+    auto mask = [&](int step, int buf, int t, e4_f32x16& x, const e4_f32x16& ks) {
+        const int key0 = t * kE4Tile + 4 * (here(lane) >> 5);
+        const int last = node < n_tree ? node : n_tree - 1;   // the last node seen
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const e4_f32x4 ks = *reinterpret_cast<const e4_f32x4*>(&lds_ks[buf][t * kE4Tile + 8 * g + 4 * half]);
+        for (int h = 0; h < 2; ++h) {
+            float b[8];
+            if (is_tree(step)) {
+                const int of0 = first_key(step) + key0 + 16 * h;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * g + e] *= ks[e];
+                for (int i = 0; i < 8; ++i) {
+                    const int of = of0 + 8 * (i >> 2) + (i & 3);
+                    b[i] = bias[of <= last ? of : 0];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int of = of0 + 8 * (i >> 2) + (i & 3);
+                    // In score units; a finite bias stays finite.
+                    float b2 = b[i] * 1.44269504088896340736f;
+                    if (fabsf(b2) == INFINITY && fabsf(b[i]) != INFINITY) b2 = copysignf(FLT_MAX, b2);
+                    b[i] = of <= last ? b2 : -INFINITY;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const e4_f32x4 kb = *reinterpret_cast<const e4_f32x4*>(&lds_kb[buf][key0 + 16 * h + 8 * g]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 8 * h + 4 * g + e;
+                    const float add = kb[e] == 0.0f ? b[4 * g + e] : kb[e];
+                    x[i] = add == -INFINITY ? -INFINITY : fmaf(x[i], ks[i], add);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);   // eight biases in registers at a time
         }
-        if (masked) {
-            const float* bias = p.bias + s.bias + static_cast<int64_t>(node < 0 ? 0 : node) * s.nodes;
+    };
+    // The wave's tiles of a step, in two phases each: the exponentials of a tile, while the next tile's K
+    // operands arrive, and the matrix products of both, while this tile's V operands do.
+    auto tiles_of = [&](int step, int buf, bool masked) {
+        const char* kb = lds + buf * 2 * KB + wk * kE4Tile * 2 * D;
+        const char* vb = kb + KB;
+        const float* ksb = &lds_ks[buf][wk * kE4Tile + 4 * half];
+        const float* vsb = &lds_vs[buf][wk * kE4Tile + 4 * half];
+        const int tiles = (keys_left(step) + kE4Tile - 1) / kE4Tile;   // at most TILES * WK count
+        e4_f32x16 x = products(kb);
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
+            const int t = n * WK + wk;
+            if (t >= tiles) break;
+            const int key = n * WK * kE4Tile;   // of the tile, from the wave's first
+            e4_f32x16 ks;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const e4_f32x4 four = *reinterpret_cast<const e4_f32x4*>(ksb + key + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ks[4 * g + e] = four[e];
+            }
+            if (masked) {
+                mask(step, buf, t, x, ks);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ks[i] = 1.0f;
+            }
+            // Probabilities against the row's reference, which is near the largest score seen: it is
+            // raised only when a tile's would pass 2^8, until when they cost no precision.
+            float negative = m == -INFINITY ? 0.0f : -m;
+            e4_f32x16 pr;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int kk = t * kE4Tile + 8 * (i >> 2) + 4 * half + (i & 3);
-                float add = lds_kb[buf][kk];
-                if (s.tree) {
-                    const int of = s.key0 + kk;
-                    const bool seen = kk < s.count && of <= node;
-                    const float b = bias[seen ? of : 0];
-                    // In score units; a finite bias stays finite.
-                    float b2 = b * 1.44269504088896340736f;
-                    if (fabsf(b2) == INFINITY && fabsf(b) != INFINITY) b2 = copysignf(FLT_MAX, b2);
-                    add = seen && add == 0.0f ? b2 : -INFINITY;
+                pr[i] = __builtin_amdgcn_exp2f(fmaf(x[i], ks[i], negative));
+                sum[i & 3] += pr[i];
+            }
+            float tile_sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const bool over = !(tile_sum <= 256.0f) || m == -INFINITY;
+            if (__any(over)) {   // other rows of the wave keep their reference: no row depends on another
+                float top = x[0] * ks[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i] * ks[i]);
+                const float raised = e4_pair_max(over ? 1.0f : 0.0f) != 0.0f ? fmaxf(m, e4_pair_max(top)) : m;
+                const float factor = raised == m ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
+                m = raised;
+                l *= factor;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) acc[i] *= factor;
+                negative = m == -INFINITY ? 0.0f : -m;
+                tile_sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    pr[i] = __builtin_amdgcn_exp2f(fmaf(x[i], ks[i], negative));
+                    tile_sum += pr[i];
                 }
-                x[i] = add == -INFINITY ? -INFINITY : x[i] + add;
             }
-        }
-        float top = x[0];
+            l += tile_sum;
+            e4_bf16x8 pb[TERMS][2];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
-        top = e4_pair_max(top);
-        // The reference maximum is raised only when a tile passes it by 2^8: until then the
-        // probabilities stay below 2^8, which costs no precision.
-        if (__any(top > m + 8.0f)) {
-            const float raised = fmaxf(m, top);
-            const float factor = raised == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
-            m = raised;
-            l *= factor;
+            for (int g = 0; g < 4; ++g) {
+                const e4_f32x4 vs = *reinterpret_cast<const e4_f32x4*>(vsb + key + 8 * g);
 #pragma unroll
-            for (int i = 0; i < NB; ++i) acc[i] *= factor;
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        e4_bf16x8 pb[2], pl[2];
-        float sum = 0.0f;
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 4 * g + e;
+                    float pv = pr[i] * vs[e];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const e4_f32x4 vs = *reinterpret_cast<const e4_f32x4*>(&lds_vs[buf][t * kE4Tile + 8 * g + 4 * half]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = 4 * g + e;
-                const float pr = __builtin_amdgcn_exp2f(x[i] - ref);
-                sum += pr;
-                float pv = pr * vs[e];
-                if (masked && x[i] == -INFINITY) pv = 0.0f;   // whatever the key's scale is
-                const __bf16 hi = static_cast<__bf16>(pv);
-                pb[i >> 3][i & 7] = hi;
-                if constexpr (TWO) pl[i >> 3][i & 7] = static_cast<__bf16>(pv - static_cast<float>(hi));
+                    for (int q = 0; q < TERMS; ++q) {
+                        pb[q][i >> 3][i & 7] = static_cast<__bf16>(pv);
+                        if (q + 1 < TERMS) pv -= static_cast<float>(pb[q][i >> 3][i & 7]);
+                    }
+                }
             }
-        }
-        l += sum;
+            __builtin_amdgcn_sched_barrier(0);
+            e4_i16x4 va[NB][2];
+            auto read_values = [&](int kk) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
+                for (int db = 0; db < NB; ++db) {
+                    const char* lo = vb + (key + 16 * kk) * 2 * D + (v_get ^ (64 * db));
+                    va[db][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((e4_lds_i16x4*)lo);
+                    va[db][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((e4_lds_i16x4*)(lo + 8 * 2 * D));
+                }
+            };
+            read_values(0);
+            if (n + 1 < TILES) x = products(kb + (key + WK * kE4Tile) * 2 * D);
 #pragma unroll
-            for (int db = 0; db < NB; ++db) {
-                const int s16 = lane & 15, group = lane >> 4;
-                const int key = 16 * kk + 4 * half + (s16 >> 2);
-                const int dim = 32 * db + 16 * (group & 1) + 4 * (s16 & 3);
-                const char* lo = vb + key * 2 * D + 16 * e4_v_chunk<D>(key, dim >> 3) + 2 * (dim & 7);
-                const char* hi = vb + (key + 8) * 2 * D + 16 * e4_v_chunk<D>(key + 8, dim >> 3) + 2 * (dim & 7);
-                const e4_i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((e4_lds_i16x4*)lo);
-                const e4_i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((e4_lds_i16x4*)hi);
-                const e4_bf16x8 v8 = __builtin_bit_cast(e4_bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-                acc[db] = E4Type<__bf16>::run(v8, pb[kk], acc[db]);
-                if constexpr (TWO) acc[db] = E4Type<__bf16>::run(v8, pl[kk], acc[db]);
+            for (int kk = 0; kk < 2; ++kk) {
+                if (kk) read_values(kk);
+#pragma unroll
+                for (int db = 0; db < NB; ++db) {
+                    const e4_bf16x8 v8 = __builtin_bit_cast(
+                        e4_bf16x8, __builtin_shufflevector(va[db][0], va[db][1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int q = 0; q < TERMS; ++q) acc[db] = E4Type<__bf16>::run(v8, pb[q][kk], acc[db]);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    // A finished run: the row's output, or its unnormalised sum with (m, l) for the merge.
-    auto put = [&](const E4Step& s, int row_in_block, int row_node, int head, int dim, e4_f32x4 v, float row_l) {
-        if (s.whole) {
+    // A finished run: the row's output, or its unnormalised sum with (m, l) for the merge, in the share's
+    // second piece if the run begins its block.
+    bool whole = false;
+    int64_t piece = 0;
+    auto put = [&](int row_in_block, int row_node, int head, int dim, e4_f32x4 v, float row_l) {
+        if (whole) {
             const float scale = row_l == 0.0f ? 0.0f : 1.0f / row_l;   // a row that sees nothing is zero
-            e4_store4<T>(p, s.first_row + row_node, head, dim, v * scale);
+            e4_store4<T>(p, first_row + row_node, head, dim, v * scale);
         } else {
-            const int64_t piece = 2 * static_cast<int64_t>(share) + s.second;
             *reinterpret_cast<e4_f32x4*>(p.ws_o + (piece * ROWS + row_in_block) * D + dim) = v;
         }
     };
-    auto finish = [&](const E4Step& s) {
+    auto finish = [&]() {
+        // The lane's place, opaque: addresses made of it here would otherwise be kept over the whole share.
+        const int c = here(lane) & 31, half = here(lane) >> 5, tid = here(threadIdx.x);
         l = e4_pair_sum(l);
-        const int64_t piece = 2 * static_cast<int64_t>(share) + s.second;
+        whole = run0 == 0 && run1 == at.steps;
+        piece = 2 * static_cast<int64_t>(share) + (run0 == 0 ? 1 : 0);
         if constexpr (WK == 1) {
             if (node >= 0) {
 #pragma unroll
@@ -639,10 +754,10 @@ e4m3_attention_kernel(const E4m3Params p) {
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         const e4_f32x4 v = {acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
-                        put(s, 32 * wm + c, node, qhead, 32 * db + 8 * g + 4 * half, v, l);
+                        put(32 * wm + c, node, qhead, 32 * db + 8 * g + 4 * half, v, l);
                     }
                 }
-                if (!s.whole && half == 0) p.ws_ml[piece * ROWS + 32 * wm + c] = make_float2(m, l);
+                if (!whole && half == 0) p.ws_ml[piece * ROWS + 32 * wm + c] = make_float2(m, l);
             }
         } else {
             // The waves of one row group join their keys through LDS, one row group at a time.
@@ -665,9 +780,9 @@ e4m3_attention_kernel(const E4m3Params p) {
                 __syncthreads();
                 for (int e = tid; e < 32 * CH; e += THREADS) {
                     const int row = e / CH, ch = e % CH;
-                    const int in_block = 32 * g0 + row, of = s.b * ROWS + in_block;
+                    const int in_block = 32 * g0 + row, of = at.b * ROWS + in_block;
                     const int n = of / p.groups;
-                    if (n >= s.nodes) continue;
+                    if (n >= nodes) continue;
                     float best = -INFINITY;
 #pragma unroll
                     for (int w = 0; w < WK; ++w) best = fmaxf(best, lds_ml[w * WM + g0][row].x);
@@ -680,65 +795,80 @@ e4m3_attention_kernel(const E4m3Params p) {
                         sum += f * ml.y;
                         v += f * all[(w * 32 + row) * CH + (ch ^ (row & (CH - 1 < 31 ? CH - 1 : 31)))];
                     }
-                    put(s, in_block, n, s.h * p.groups + of - n * p.groups, 4 * ch, v, sum);
-                    if (!s.whole && ch == 0) p.ws_ml[piece * ROWS + in_block] = make_float2(best, sum);
+                    put(in_block, n, at.h * p.groups + of - n * p.groups, 4 * ch, v, sum);
+                    if (!whole && ch == 0) p.ws_ml[piece * ROWS + in_block] = make_float2(best, sum);
                 }
                 __syncthreads();
             }
         }
     };
 
-    // --- the run ------------------------------------------------------------------------------
-    E4Step now, next, after;
+    // --- the share, run by run ----------------------------------------------------------------
     int count = 1;   // steps begun, the mark of a buffer with a missing page
-    describe(now);
-    fetch_entries(now);
-    fetch_keys(now);
-    advance();
-    bool more = todo > 0;
-    if (more) {
-        describe(next);
-        fetch_entries(next);
-        advance();
-    }
-    for (int buf = 0;; buf = NBUF == 2 ? buf ^ 1 : 0, ++count) {
-        if (NBUF == 1) __syncthreads();   // the last step's reads of the buffer are done
-        stage(now, buf, count);
-        if (more) {
-            fetch_keys(next);
-            if (todo > 0) {
-                describe(after);
-                fetch_entries(after);
+    auto compute = [&](int i, int buf) {
+        if (wave_rows) tiles_of(i, buf, is_tree(i) || keys_left(i) < SK || lds_bad[buf] == count);
+    };
+    for (;;) {
+        start_block();
+        fetch_entries(run0);
+        fetch_keys(run0);
+        if (run0 + 1 < run1) fetch_entries(run0 + 1);
+        if constexpr (NBUF == 1) {
+            for (int i = run0; i < run1; ++i, ++count) {
+                __syncthreads();   // the last step's reads of the buffer are done
+                stage(i, 0, count);
+                if (i + 1 < run1) fetch_keys(i + 1);
+                if (i + 2 < run1) fetch_entries(i + 2);
+                __syncthreads();
+                compute(i, 0);
+            }
+        } else {
+            // Two buffers: a step is staged while the one before it is computed, by half of the waves (one
+            // a SIMD) before their tiles and by the others after, so that each SIMD has one wave on its
+            // matrix unit while the other converts.
+            static_assert(WK == 1, "finish() would join over buffers in use");
+            const bool late = wave >= WM / 2;
+            auto prepare = [&](int i, int buf, int mark) {
+                if (i >= run1) return;
+                stage(i, buf, mark);
+                if (i + 1 < run1) fetch_keys(i + 1);
+                if (i + 2 < run1) fetch_entries(i + 2);
+            };
+            prepare(run0, 0, count);
+            __syncthreads();
+            int buf = 0;
+            for (int i = run0; i < run1; ++i, ++count, buf ^= 1) {
+                if (!late) prepare(i + 1, buf ^ 1, count + 1);
+                compute(i, buf);
+                if (late) prepare(i + 1, buf ^ 1, count + 1);
+                __syncthreads();
             }
         }
-        if (now.first) start_block(now);
-        __syncthreads();
-        if (wave_rows) {
-            const bool masked = now.tree || now.count < SK || lds_bad[buf] == count;
-            if (masked) {
-                for (int t = wk; t * kE4Tile < now.count; t += WK) tile(now, buf, t, true);
-            } else {
-#pragma unroll 1
-                for (int t = 0; t < TILES; ++t) tile(now, buf, t * WK + wk, false);
+        finish();
+        todo -= run1 - run0;
+        if (todo <= 0) break;
+        at.step = 0;
+        if (++at.b == req.blocks) {
+            at.b = 0;
+            if (++at.h == p.num_kv_heads) {
+                at.h = 0;
+                do {
+                    ++at.r;
+                    req = e4_request<ROWS, SK>(p, at.r, false);
+                } while (req.blocks == 0);   // todo > 0: a later request has steps
             }
         }
-        if (now.last) finish(now);
-        if (!more) break;
-        more = todo > 0;
-        now = next;
-        if (more) {
-            next = after;
-            advance();
-        }
+        at.steps = e4_block_steps<ROWS, SK>(p, req, at.b);
     }
 }
 
 template <int D, int WM, int WK, int NBUF>
-void e4_launch(const E4m3Params& p, bool bf16, bool two, hipStream_t s) {
+void e4_launch(const E4m3Params& p, bool bf16, hipStream_t s) {
     const dim3 grid(p.workgroups), block(64 * WM * WK);
-    if (bf16 && !two) hipLaunchKernelGGL((e4m3_attention_kernel<D, WM, WK, NBUF, __bf16, false>), grid, block, 0, s, p);
-    else if (bf16) hipLaunchKernelGGL((e4m3_attention_kernel<D, WM, WK, NBUF, __bf16, true>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((e4m3_attention_kernel<D, WM, WK, NBUF, _Float16, true>), grid, block, 0, s, p);
+    if (bf16 && !p.out_f32) hipLaunchKernelGGL((e4m3_attention_kernel<D, WM, WK, NBUF, __bf16, 1>), grid, block, 0, s, p);
+    else if (bf16) hipLaunchKernelGGL((e4m3_attention_kernel<D, WM, WK, NBUF, __bf16, 3>), grid, block, 0, s, p);
+    else if (!p.out_f32) hipLaunchKernelGGL((e4m3_attention_kernel<D, WM, WK, NBUF, _Float16, 2>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((e4m3_attention_kernel<D, WM, WK, NBUF, _Float16, 3>), grid, block, 0, s, p);
 }
 
 }  // namespace

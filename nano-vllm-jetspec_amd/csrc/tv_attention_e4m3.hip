@@ -29,15 +29,14 @@ e4m3_merge_kernel(const E4m3Params p) {
     const E4Request req = e4_request<ROWS, SK>(p, at.r, false);
     const int64_t end = at.begin + at.steps;
     const int rows = req.nodes * p.groups - at.b * ROWS < ROWS ? req.nodes * p.groups - at.b * ROWS : ROWS;
-    int pieces = 1;
-    while (e4_first_step(total, W, w - 1 + pieces) < end) ++pieces;   // total >= end ends it
+    // Pieces are those of the shares w - 1 to the one that reaches the end; the first share's is its
+    // second piece if its run begins the block, the others begin with their piece.
+    const int64_t n = total < W ? total : W;
+    const int pieces = static_cast<int>((end * n + total - 1) / total) - (w - 1);
+    const int64_t piece0 = 2 * (w - 1) + (e4_first_step(total, W, w - 1) <= at.begin ? 1 : 0);
     const int ch = threadIdx.x % CH;
     for (int row = blockIdx.y * RPP + threadIdx.x / CH; row < rows; row += gridDim.y * RPP) {
-        // The first piece is its workgroup's second one unless the block begins the share's run.
-        auto piece = [&](int i) -> int64_t {
-            const int64_t u = w - 1 + i;
-            return (2 * u + (e4_first_step(total, W, u) <= at.begin ? 1 : 0)) * ROWS + row;
-        };
+        auto piece = [&](int i) -> int64_t { return (i == 0 ? piece0 : 2ll * (w - 1 + i)) * ROWS + row; };
         float best = -INFINITY;
         for (int i = 0; i < pieces; ++i) best = fmaxf(best, p.ws_ml[piece(i)].x);
         float sum = 0.0f;
@@ -157,6 +156,12 @@ extern "C" int tv_tree_attention_e4m3(const tv_tree_attention_e4m3_args* a, void
     const int64_t piece = 16 / (a->out_dtype == TV_F32 ? 4 : 2);
     ok = ok && aligned(a->out, 16) && a->out_stride_row % piece == 0 && a->out_stride_head % piece == 0;
     if (!ok) return fail(TV_ERR_UNSUPPORTED, "%s: query, pool and output rows must start at 16 bytes, head dim contiguous", what);
+    const int64_t* strides[] = {a->k_stride, a->v_stride, a->k_scale_stride, a->v_scale_stride};
+    for (const int64_t* stride : strides) {
+        if (stride[0] < 0 || stride[1] < 0 || stride[2] < 0 || stride[1] > 0x7fffffff || stride[2] > 0x7fffffff) {
+            return fail(TV_ERR_UNSUPPORTED, "%s: slot and head strides must be below 2^31, none negative", what);
+        }
+    }
     const Launch n = launch_of(a);
     if (!workspace || !aligned(workspace, 16)) return fail(TV_ERR_INVALID, "%s: null or unaligned workspace", what);
     if (workspace_bytes < n.bytes) {
@@ -170,21 +175,35 @@ extern "C" int tv_tree_attention_e4m3(const tv_tree_attention_e4m3_args* a, void
     p.k = static_cast<const uint8_t*>(a->k_pool);
     p.v = static_cast<const uint8_t*>(a->v_pool);
     p.k_s0 = a->k_stride[0];
-    p.k_s1 = a->k_stride[1];
-    p.k_s2 = a->k_stride[2];
     p.v_s0 = a->v_stride[0];
-    p.v_s1 = a->v_stride[1];
-    p.v_s2 = a->v_stride[2];
+    p.kc_s0 = a->k_scale_stride[0];
+    p.vc_s0 = a->v_scale_stride[0];
+    p.k_s1 = static_cast<int32_t>(a->k_stride[1]);
+    p.k_s2 = static_cast<int32_t>(a->k_stride[2]);
+    p.v_s1 = static_cast<int32_t>(a->v_stride[1]);
+    p.v_s2 = static_cast<int32_t>(a->v_stride[2]);
+    p.kc_s1 = static_cast<int32_t>(a->k_scale_stride[1]);
+    p.kc_s2 = static_cast<int32_t>(a->k_scale_stride[2]);
+    p.vc_s1 = static_cast<int32_t>(a->v_scale_stride[1]);
+    p.vc_s2 = static_cast<int32_t>(a->v_scale_stride[2]);
     p.ks = a->k_scale;
     p.vs = a->v_scale;
-    p.kc_s0 = a->k_scale_stride[0];
-    p.kc_s1 = a->k_scale_stride[1];
-    p.kc_s2 = a->k_scale_stride[2];
-    p.vc_s0 = a->v_scale_stride[0];
-    p.vc_s1 = a->v_scale_stride[1];
-    p.vc_s2 = a->v_scale_stride[2];
     p.num_blocks = static_cast<int32_t>(a->num_blocks);
     p.block_size = a->block_size;
+    const int64_t keys = e4_step_keys(a->head_dim);
+    bool same = a->block_size % keys == 0;
+    for (int i = 0; i < 3; ++i) {
+        same = same && a->k_stride[i] == a->v_stride[i] && a->k_scale_stride[i] == a->v_scale_stride[i];
+    }
+    const int64_t reach_of[] = {a->block_size * a->k_stride[1], 4 * a->block_size * a->k_scale_stride[1]};
+    p.page_steps = same && a->k_stride[0] <= 0xffffffffll && a->k_scale_stride[0] <= 0x3fffffffll &&
+                   reach_of[0] <= 0x7fffffff && reach_of[1] <= 0x7fffffff;
+    if (p.page_steps) {
+        p.f_s0 = static_cast<uint32_t>(a->k_stride[0]);
+        p.f_s1 = static_cast<uint32_t>(a->k_stride[1]);
+        p.f_c0 = static_cast<uint32_t>(4 * a->k_scale_stride[0]);
+        p.f_c1 = static_cast<uint32_t>(4 * a->k_scale_stride[1]);
+    }
     uint32_t shift = 0;
     while ((1ull << shift) < static_cast<uint64_t>(a->block_size)) ++shift;
     p.div_shift = shift;
@@ -213,12 +232,11 @@ extern "C" int tv_tree_attention_e4m3(const tv_tree_attention_e4m3_args* a, void
     p.ws_o = static_cast<float*>(workspace);
     p.ws_ml = reinterpret_cast<float2*>(p.ws_o + 2ll * n.workgroups * n.shape.rows * a->head_dim);
     p.status = a->status;
-    // fp32 results want the probabilities beyond bf16's 8 bits; so do f16 ones, whose step is finer.
-    const bool bf16 = a->in_dtype == TV_BF16, two = p.out_f32 || !bf16;
+    const bool bf16 = a->in_dtype == TV_BF16;
     const hipStream_t s = as_stream(stream);
-    if (a->head_dim == 64) launch_e4m3_d64(p, n.shape, bf16, two, s);
-    else if (a->head_dim == 128) launch_e4m3_d128(p, n.shape, bf16, two, s);
-    else launch_e4m3_d256(p, n.shape, bf16, two, s);
+    if (a->head_dim == 64) launch_e4m3_d64(p, n.shape, bf16, s);
+    else if (a->head_dim == 128) launch_e4m3_d128(p, n.shape, bf16, s);
+    else launch_e4m3_d256(p, n.shape, bf16, s);
     const int launched = check_launch(what);
     if (launched != TV_OK) return launched;
     if (a->head_dim == 64) launch_merge_d<64>(p, n.shape.rows, bf16, s);

@@ -12,12 +12,12 @@ E4m3Shape e4m3_shape_d128(int64_t average_rows) {
     return {256, 512, 1};
 }
 
-void launch_e4m3_d128(const E4m3Params& p, const E4m3Shape& shape, bool bf16, bool two, hipStream_t s) {
+void launch_e4m3_d128(const E4m3Params& p, const E4m3Shape& shape, bool bf16, hipStream_t s) {
     switch (shape.rows) {
-        case 32: return e4_launch<128, 1, 4, 1>(p, bf16, two, s);
-        case 64: return e4_launch<128, 2, 2, 1>(p, bf16, two, s);
-        case 128: return e4_launch<128, 4, 1, 1>(p, bf16, two, s);
-        default: return e4_launch<128, 8, 1, 2>(p, bf16, two, s);
+        case 32: return e4_launch<128, 1, 4, 1>(p, bf16, s);
+        case 64: return e4_launch<128, 2, 2, 1>(p, bf16, s);
+        case 128: return e4_launch<128, 4, 1, 1>(p, bf16, s);
+        default: return e4_launch<128, 8, 1, 2>(p, bf16, s);
     }
 }
 

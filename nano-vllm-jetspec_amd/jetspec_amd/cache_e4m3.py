@@ -87,8 +87,8 @@ def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     and ``metadata`` is any ``PackedTreeMetadata`` (a tree of one node is a decode token, a chain tree
     a prefill chunk).  Any query group, page size and tree size; finite ``qq_bias`` values are added
     to the scores.  The result is new, in q's dtype or FP32; a row that sees no key is zero.  BF16
-    results round each probability times its key's scale to BF16 once, FP32 and FP16 ones keep it
-    to 2^-17.
+    results round each probability times its key's scale to BF16 once, FP16 ones keep it to 2^-17
+    and FP32 ones to 2^-26.
 
     Every length, page and slot is read on the device, so a captured call follows the staged
     metadata, and no state is kept between calls.  Requests that reach outside the batch, the bias

@@ -1,7 +1,8 @@
 """The e4m3 tree attention on the GPU against 64 bits.
 
 Tolerance, derived.  With normalised weights w_k and values u_k = vs_k V8_k, let S = sum_k w_k |u_k| per
-output.  A probability times its scale is rounded to bf16 (2^-8 of it) or kept in two terms (2^-17).
+output.  A probability times its scale is rounded to bf16 (2^-8 of it) or kept in two terms (2^-17,
+f16 output) or three (2^-26, fp32 output).
 Scores are sums of D exact products in fp32, scaled by two roundings: at most (D + 4) 2^-24 of
 sum_d |q_d k_d| scale, and a bias adds its own rounding of the score; a probability is off by that
 and by 2^-21 of its exponential, in the numerator and in the sum.  The sums over n keys and the joins
@@ -72,7 +73,7 @@ class Batch:
     def check(self, out, requests=None):
         """Compares the rows of `requests` (all) with the formula in 64 bits."""
         got = self.run(out) if not isinstance(out, torch.Tensor) else out
-        two = got.dtype != BF16
+        rounded = {BF16: 2.0 ** -8, F16: 2.0 ** -17, F32: 2.0 ** -26}[got.dtype]
         m = self.meta
         half_step = torch.finfo(got.dtype).eps / 2
         for r in range(len(self.prefixes)) if requests is None else requests:
@@ -94,7 +95,7 @@ class Batch:
                 w = torch.where(seen.any(-1, keepdim=True), w, 0)
                 expect, spread = torch.mm(w, v), torch.mm(w, v.abs())
                 slack = ((q.shape[1] + 4) * 2.0 ** -24 * torch.where(seen, size, 0).amax(-1, keepdim=True) + 2.0 ** -21)
-                relative = (2.0 ** -17 if two else 2.0 ** -8) + 2 * slack + 2 * (keys.numel() + 600) * 2.0 ** -24
+                relative = rounded + 2 * slack + 2 * (keys.numel() + 600) * 2.0 ** -24
                 allowed = relative * spread * (1 + 2.0 ** -6)
                 allowed = allowed + half_step * (expect.abs() + allowed) + (2.0 ** -25 if got.dtype == F16 else 0)
                 off = (got[rows, mine].double().reshape(expect.shape) - expect).abs() - allowed
@@ -252,8 +253,8 @@ def test_biases_of_the_lowest_value():
         v = batch.rows(batch.v, batch.vs, keys, h)
         for i in range(6):
             mine = v[torch.as_tensor(seen[i], device=DEV)]
-            # Equal weights: the two-term probabilities and the quotient, and a sum of 6.
-            allowed = (2.0 ** -17 + 10 * 2.0 ** -24) * mine.abs().mean(0)
+            # Equal weights: the three-term probabilities and the quotient, and a sum of 6.
+            allowed = (2.0 ** -26 + 10 * 2.0 ** -24) * mine.abs().mean(0)
             assert bool(((got[i, 4 * h].double() - mine.mean(0)).abs() <= allowed).all())
 
 
