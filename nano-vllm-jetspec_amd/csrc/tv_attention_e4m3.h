@@ -38,6 +38,16 @@
 
 namespace tv {
 
+// A row block whose pieces the merge joins, written by the workgroup whose share its first step ends.
+struct E4m3Job {
+    int32_t pieces;        // 0: none
+    int32_t rows;          // live rows of the block
+    int32_t first_row;     // packed row of the request's first node
+    int32_t head0;         // first query head of the KV head
+    int32_t row0;          // the block's first row, counted as node * group + head over the request
+    int32_t unused[3];
+};
+
 struct E4m3Params {
     const void* q;
     int64_t q_s0, q_s1;
@@ -71,6 +81,7 @@ struct E4m3Params {
     float c;                       // scale * log2(e)
     float* ws_o;
     float2* ws_ml;
+    struct E4m3Job* jobs;          // one a workgroup of the attention launch
     int32_t workgroups;            // of the attention launch
     int32_t* status;
 };
@@ -169,80 +180,115 @@ struct E4Place {
     int32_t r, h, b;
     int32_t step;    // step within the block
     int32_t steps;   // of the block
-    int64_t begin;   // first step of the block, counted over the whole launch
 };
 
-// Counts every step of the launch into `total`, then finds step `pick(total)`.  All threads of the
-// workgroup call it; `scratch` is LDS of its own.
-template <int ROWS, int SK, int THREADS, class PICK>
-__device__ __forceinline__ bool e4_find(const E4m3Params& p, int64_t* scratch, int64_t& total, E4Place& place, PICK pick) {
-    constexpr int WAVES = THREADS / 64;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (p.num_requests + THREADS - 1) / THREADS;
-    const int r0 = tid * per, r1 = r0 + per < p.num_requests ? r0 + per : p.num_requests;
-    int64_t mine = 0;
-    for (int r = r0; r < r1; ++r) {
-        const E4Request q = e4_request<ROWS, SK>(p, r, blockIdx.x == 0 && blockIdx.y == 0);
-        mine += e4_head_steps<ROWS, SK>(p, q) * p.num_kv_heads;
-    }
-    int64_t end = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(end, o);
-        if (lane >= o) end += y;
-    }
-    if (lane == 63) scratch[wave] = end;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) end += scratch[w];
-        total += scratch[w];
-    }
-    __syncthreads();
-    const int64_t target = pick(total);
-    if (target < 0 || target >= total) return false;   // the same in every thread
-    const int64_t begin = end - mine;
-    if (begin <= target && target < end) {
-        // This thread's requests hold it.
-        int64_t at = begin;
-        for (int r = r0; r < r1; ++r) {
-            const E4Request q = e4_request<ROWS, SK>(p, r, false);
-            const int64_t head = e4_head_steps<ROWS, SK>(p, q);
-            if (target >= at + head * p.num_kv_heads) {
-                at += head * p.num_kv_heads;
-                continue;
-            }
-            const int32_t h = static_cast<int32_t>((target - at) / head);
-            at += h * head;
-            int b = 0, steps = e4_block_steps<ROWS, SK>(p, q, 0);
-            while (target >= at + steps) {
-                at += steps;
-                steps = e4_block_steps<ROWS, SK>(p, q, ++b);
-            }
-            scratch[0] = (static_cast<int64_t>(r) << 32) | static_cast<uint32_t>(h);
-            scratch[1] = (static_cast<int64_t>(b) << 32) | static_cast<uint32_t>(steps);
-            scratch[2] = at;
-            break;
-        }
-    }
-    __syncthreads();
-    const int64_t a = scratch[0], c = scratch[1], at = scratch[2];
-    __syncthreads();
-    place.r = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(a >> 32));
-    place.h = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(a));
-    place.b = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(c >> 32));
-    place.steps = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(c));
-    place.begin = e4_uniform(at);
-    place.step = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(target - place.begin));
-    return true;
+// Unsigned quotient; 64-bit division only where it has to be.
+__device__ __forceinline__ int64_t e4_divide(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
 }
 
-// Steps [first, last) of workgroup w: an equal share of all.  With fewer steps than workgroups the
-// first `total` take one each.
-__device__ __forceinline__ int64_t e4_first_step(int64_t total, int64_t workgroups, int64_t w) {
-    const int64_t n = total < workgroups ? total : workgroups;
-    return w >= n ? total : total * w / n;
+// First step of workgroup w: equal shares of all.  With fewer steps than workgroups the first `total` take
+// one each.
+__device__ __forceinline__ int64_t e4_first_step(int64_t total, int32_t workgroups, int32_t w) {
+    if (total <= workgroups) return w < total ? w : total;
+    const int64_t each = e4_divide(total, workgroups);
+    const uint32_t rest = static_cast<uint32_t>(total - each * workgroups);   // below the workgroups: 32-bit products
+    return each * w + rest * static_cast<uint32_t>(w) / static_cast<uint32_t>(workgroups);
+}
+
+// Counts every step of the launch into `total`, then finds step `pick(total)`; false if that is no step.
+// All threads of the workgroup call it; `scratch` is LDS of its own.
+template <int ROWS, int SK, int THREADS, class PICK>
+__device__ __forceinline__ bool e4_find(const E4m3Params& p, int64_t* scratch, int64_t& total, E4Place& place, E4Request& request,
+                                        PICK pick) {
+    constexpr int WAVES = THREADS / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const bool report = blockIdx.x == 0;
+    int64_t at, target;    // first step of request r, the step to find
+    int r;
+    if (p.num_requests <= 64) {
+        // A lane per request, in every wave by itself.
+        E4Request q = {};
+        int64_t mine = 0;
+        if (lane < p.num_requests) {
+            q = e4_request<ROWS, SK>(p, lane, report && wave == 0);
+            mine = e4_head_steps<ROWS, SK>(p, q) * p.num_kv_heads;
+        }
+        int64_t end = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t y = __shfl_up(end, o);
+            if (lane >= o) end += y;
+        }
+        total = e4_uniform(__shfl(end, 63));
+        target = e4_uniform(pick(total));
+        if (target < 0 || target >= total) return false;
+        r = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<long long>(__ballot(end > target))) - 1);
+        at = e4_uniform(__shfl(end - mine, r));
+        request.prefix = __builtin_amdgcn_readlane(q.prefix, r);
+        request.nodes = __builtin_amdgcn_readlane(q.nodes, r);
+        request.first_row = __builtin_amdgcn_readlane(q.first_row, r);
+        request.bias = e4_uniform(__shfl(q.bias, r));
+        request.prefix_steps = __builtin_amdgcn_readlane(q.prefix_steps, r);
+        request.blocks = __builtin_amdgcn_readlane(q.blocks, r);
+    } else {
+        const int per = (p.num_requests + THREADS - 1) / THREADS;
+        const int r0 = tid * per, r1 = r0 + per < p.num_requests ? r0 + per : p.num_requests;
+        int64_t mine = 0;
+        for (int i = r0; i < r1; ++i) {
+            const E4Request q = e4_request<ROWS, SK>(p, i, report);
+            mine += e4_head_steps<ROWS, SK>(p, q) * p.num_kv_heads;
+        }
+        int64_t end = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t y = __shfl_up(end, o);
+            if (lane >= o) end += y;
+        }
+        if (lane == 63) scratch[wave] = end;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            if (w < wave) end += scratch[w];
+            total += scratch[w];
+        }
+        __syncthreads();
+        total = e4_uniform(total);
+        target = e4_uniform(pick(total));
+        if (target < 0 || target >= total) return false;   // the same in every thread
+        if (end - mine <= target && target < end) {        // this thread's requests hold it
+            int64_t first = end - mine;
+            for (int i = r0; i < r1; ++i) {
+                const E4Request q = e4_request<ROWS, SK>(p, i, false);
+                const int64_t next = first + e4_head_steps<ROWS, SK>(p, q) * p.num_kv_heads;
+                if (target < next) {
+                    scratch[0] = i;
+                    scratch[1] = first;
+                    break;
+                }
+                first = next;
+            }
+        }
+        __syncthreads();
+        r = __builtin_amdgcn_readfirstlane(static_cast<int>(scratch[0]));
+        at = e4_uniform(scratch[1]);
+        __syncthreads();
+        request = e4_request<ROWS, SK>(p, r, false);
+    }
+    place.r = r;
+    const int64_t head = e4_head_steps<ROWS, SK>(p, request);
+    place.h = static_cast<int32_t>(e4_divide(target - at, head));
+    at += place.h * head;
+    place.b = 0;
+    place.steps = e4_block_steps<ROWS, SK>(p, request, 0);
+    while (target >= at + place.steps) {
+        at += place.steps;
+        place.steps = e4_block_steps<ROWS, SK>(p, request, ++place.b);
+    }
+    place.step = static_cast<int32_t>(target - at);
+    return true;
 }
 
 template <class T>
@@ -346,12 +392,14 @@ e4m3_attention_kernel(const E4m3Params p) {
     int64_t total = 0, s0 = 0, s1 = 0;   // all steps; this share's
     int share = 0;
     E4Place at;
-    const bool any = e4_find<ROWS, SK, THREADS>(p, lds_scan, total, at, [&](int64_t all) -> int64_t {
+    E4Request req;
+    const bool any = e4_find<ROWS, SK, THREADS>(p, lds_scan, total, at, req, [&](int64_t all) -> int64_t {
         share = all < W ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x % 8 * (W / 8) + blockIdx.x / 8);
         s0 = e4_first_step(all, W, share);
         s1 = e4_first_step(all, W, share + 1);
         return s0 < s1 ? s0 : -1;
     });
+    if (tid == 0) p.jobs[share].pieces = 0;
     if (!any) return;
     share = __builtin_amdgcn_readfirstlane(share);
     int todo = __builtin_amdgcn_readfirstlane(static_cast<int>(s1 - s0));   // steps not yet run
@@ -366,7 +414,6 @@ e4m3_attention_kernel(const E4m3Params p) {
     };
 
     // --- a run: steps [run0, run1) of one row block ---------------------------------------------
-    E4Request req = e4_request<ROWS, SK>(p, at.r, false);
     int n_tree = 0;                        // nodes that the block may see
     int run0 = at.step, run1 = 0;
     const int32_t* table = nullptr;        // of the request
@@ -702,7 +749,6 @@ e4m3_attention_kernel(const E4m3Params p) {
                     }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
             e4_i16x4 va[NB][2];
             auto read_values = [&](int kk) {
 #pragma unroll
@@ -725,7 +771,6 @@ e4m3_attention_kernel(const E4m3Params p) {
                     for (int q = 0; q < TERMS; ++q) acc[db] = E4Type<__bf16>::run(v8, pb[q][kk], acc[db]);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
@@ -747,6 +792,19 @@ e4m3_attention_kernel(const E4m3Params p) {
         l = e4_pair_sum(l);
         whole = run0 == 0 && run1 == at.steps;
         piece = 2 * static_cast<int64_t>(share) + (run0 == 0 ? 1 : 0);
+        if (run0 == 0 && !whole && tid == 0) {
+            // The share ends inside the block: the pieces go on to the share that holds the block's last
+            // step, the first u with first_step(u) >= end (each share of `total` steps is total / n long).
+            const int64_t n = total < W ? total : W, end = s1 + (at.steps - run1);
+            E4m3Job job = {};
+            job.pieces = static_cast<int32_t>(e4_divide(end * n + total - 1, total)) - share;
+            const int32_t row0 = at.b * ROWS, live = nodes * p.groups - row0;
+            job.rows = live < ROWS ? live : ROWS;
+            job.first_row = first_row;
+            job.head0 = at.h * p.groups;
+            job.row0 = row0;
+            p.jobs[share] = job;
+        }
         if constexpr (WK == 1) {
             if (node >= 0) {
 #pragma unroll

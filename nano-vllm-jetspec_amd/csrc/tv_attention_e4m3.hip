@@ -8,57 +8,55 @@ namespace {
 constexpr int kMergeThreads = 256;
 
 // Joins the pieces of one row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m).
-// Workgroup (x, y) looks at the boundary between the shares x and x + 1; the one at a block's first
-// boundary joins every y-th group of its rows.  Most find that their boundary ends a block or lies
-// in one that began earlier, and leave.
+// Workgroup (x, y) takes the job that workgroup x of the attention left, if any, and of its rows every y-th
+// group.  Each thread keeps four pieces of a row in flight; what bounds it is their latency.
 template <int D, int ROWS, class T>
 __global__ void __launch_bounds__(kMergeThreads)
 e4m3_merge_kernel(const E4m3Params p) {
-    constexpr int SK = e4_step_keys(D), CH = D / 4, RPP = kMergeThreads / CH;
-    __shared__ int64_t scan[4];
-    const int64_t W = p.workgroups;
-    const int w = blockIdx.x + 1;
-    int64_t total = 0;
-    E4Place at;
-    const bool any = e4_find<ROWS, SK, kMergeThreads>(p, scan, total, at, [&](int64_t all) -> int64_t {
-        const int64_t s = e4_first_step(all, W, w);
-        return s < all ? s : -1;
-    });
-    if (!any || at.step == 0) return;
-    if (e4_first_step(total, W, w - 1) > at.begin) return;
-    const E4Request req = e4_request<ROWS, SK>(p, at.r, false);
-    const int64_t end = at.begin + at.steps;
-    const int rows = req.nodes * p.groups - at.b * ROWS < ROWS ? req.nodes * p.groups - at.b * ROWS : ROWS;
-    // Pieces are those of the shares w - 1 to the one that reaches the end; the first share's is its
-    // second piece if its run begins the block, the others begin with their piece.
-    const int64_t n = total < W ? total : W;
-    const int pieces = static_cast<int>((end * n + total - 1) / total) - (w - 1);
-    const int64_t piece0 = 2 * (w - 1) + (e4_first_step(total, W, w - 1) <= at.begin ? 1 : 0);
+    constexpr int CH = D / 4, RPP = kMergeThreads / CH;
+    const int share = blockIdx.x;
+    const E4m3Job job = p.jobs[share];
+    if (job.pieces == 0) return;
     const int ch = threadIdx.x % CH;
-    for (int row = blockIdx.y * RPP + threadIdx.x / CH; row < rows; row += gridDim.y * RPP) {
-        auto piece = [&](int i) -> int64_t { return (i == 0 ? piece0 : 2ll * (w - 1 + i)) * ROWS + row; };
-        float best = -INFINITY;
-        for (int i = 0; i < pieces; ++i) best = fmaxf(best, p.ws_ml[piece(i)].x);
-        float sum = 0.0f;
+    for (int row = blockIdx.y * RPP + threadIdx.x / CH; row < job.rows; row += gridDim.y * RPP) {
+        // The first piece is its share's second, the following shares begin with theirs.
+        auto piece = [&](int i) -> int64_t { return static_cast<int64_t>(2 * (share + i) + (i == 0 ? 1 : 0)) * ROWS + row; };
+        float best = -INFINITY, sum = 0.0f;
         e4_f32x4 v = {0, 0, 0, 0};
-#pragma unroll 4
-        for (int i = 0; i < pieces; ++i) {
-            const int64_t of = piece(i);
-            const float2 ml = p.ws_ml[of];
-            const float f = e4_weight(ml, best);
-            sum += f * ml.y;
-            v += f * *reinterpret_cast<const e4_f32x4*>(p.ws_o + of * D + 4 * ch);
+        for (int i0 = 0; i0 < job.pieces; i0 += 4) {
+            float2 ml[4];
+            e4_f32x4 o[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int64_t of = piece(i0 + n < job.pieces ? i0 + n : i0);
+                ml[n] = p.ws_ml[of];
+                o[n] = *reinterpret_cast<const e4_f32x4*>(p.ws_o + of * D + 4 * ch);
+            }
+            float top = best;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) top = fmaxf(top, ml[n].x);
+            const float keep = best == top ? 1.0f : __builtin_amdgcn_exp2f(best - top);   // -inf twice: 1
+            sum *= keep;
+            v *= keep;
+            best = top;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                if (i0 + n >= job.pieces) break;
+                const float f = e4_weight(ml[n], best);
+                sum += f * ml[n].y;
+                v += f * o[n];
+            }
         }
         const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int of = at.b * ROWS + row, node = of / p.groups;
-        e4_store4<T>(p, req.first_row + node, at.h * p.groups + of - node * p.groups, 4 * ch, v * scale);
+        const int of = job.row0 + row, node = of / p.groups;
+        e4_store4<T>(p, job.first_row + node, job.head0 + of - node * p.groups, 4 * ch, v * scale);
     }
 }
 
 template <int D, int ROWS>
 void launch_merge(const E4m3Params& p, bool bf16, hipStream_t s) {
     constexpr int per_pass = kMergeThreads / (D / 4), passes = ROWS / per_pass;
-    const dim3 grid(p.workgroups - 1, passes < 8 ? passes : 8);
+    const dim3 grid(p.workgroups, passes < 16 ? passes : 16);
     if (bf16) hipLaunchKernelGGL((e4m3_merge_kernel<D, ROWS, __bf16>), grid, dim3(kMergeThreads), 0, s, p);
     else hipLaunchKernelGGL((e4m3_merge_kernel<D, ROWS, _Float16>), grid, dim3(kMergeThreads), 0, s, p);
 }
@@ -91,7 +89,7 @@ Launch launch_of(const tv_tree_attention_e4m3_args* a) {
     const int64_t most = blocks * ((reach + keys - 1) / keys + (a->total_queries + keys - 1) / keys);
     const int64_t full = static_cast<int64_t>(a->compute_units) * n.shape.per_cu;
     n.workgroups = static_cast<int32_t>(((most < full ? most : full) + 7) / 8 * 8);
-    n.bytes = 2ll * n.workgroups * n.shape.rows * (a->head_dim * 4 + 8);
+    n.bytes = 2ll * n.workgroups * n.shape.rows * (a->head_dim * 4 + 8) + n.workgroups * static_cast<int64_t>(sizeof(E4m3Job));
     return n;
 }
 
@@ -231,6 +229,7 @@ extern "C" int tv_tree_attention_e4m3(const tv_tree_attention_e4m3_args* a, void
     p.workgroups = n.workgroups;
     p.ws_o = static_cast<float*>(workspace);
     p.ws_ml = reinterpret_cast<float2*>(p.ws_o + 2ll * n.workgroups * n.shape.rows * a->head_dim);
+    p.jobs = reinterpret_cast<E4m3Job*>(p.ws_ml + 2ll * n.workgroups * n.shape.rows);
     p.status = a->status;
     const bool bf16 = a->in_dtype == TV_BF16;
     const hipStream_t s = as_stream(stream);
