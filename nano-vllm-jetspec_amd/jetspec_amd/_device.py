@@ -56,13 +56,37 @@ def read_and_clear_status(device: torch.device | str | int = "cuda") -> int:
     return value
 
 
-def call(device: torch.device, entry, *args) -> int:
-    """A C entry's return code, called with `device` current: a launch goes to the current device's
-    streams only, and the caller's current device need not be the tensors' one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return entry(*args)
-    with torch.cuda.device(device):
-        return entry(*args)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_status_pointers: dict[int, int] = {}
+
+
+def one_gpu(what: str, *tensors: torch.Tensor) -> int:
+    """Index of the GPU that all tensors are on; ``require_gpu``'s errors otherwise."""
+    index = tensors[0].get_device()
+    if index < 0:
+        raise ValueError(f"{what} requires GPU tensors (got {tensors[0].device}); there is no CPU path")
+    for tensor in tensors:
+        if tensor.get_device() != index:
+            raise ValueError(f"{what} requires all tensors on one device")
+    return index
+
+
+def status_pointer(index: int) -> int:
+    """Address of a device's status word."""
+    pointer = _status_pointers.get(index)
+    if pointer is None:
+        pointer = _status_pointers[index] = status_word(torch.device("cuda", index)).data_ptr()
+    return pointer
+
+
+def launch(index: int, entry, *args) -> int:
+    """A C entry's return code, called on torch's current stream of a device with that device current: a
+    launch goes to the current device's streams only, and the caller's need not be the tensors' one."""
+    stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+    if index == torch.cuda.current_device():
+        return entry(*args, stream)
+    with torch.cuda.device(index):
+        return entry(*args, stream)
 
 
 @lru_cache(maxsize=None)

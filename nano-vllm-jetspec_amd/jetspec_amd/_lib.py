@@ -7,6 +7,7 @@ device entry point raises ``RuntimeError`` naming the problem.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_uint64, c_void_p
 from pathlib import Path
 import threading
@@ -238,6 +239,36 @@ class TreeAttentionE4m3Args(ctypes.Structure):
     ]
 
 
+def _fields_format(structure, base: int = 0) -> list[tuple[int, str, int]]:
+    """(offset, struct code, size) of every scalar of a structure, nested ones and arrays laid out flat."""
+    codes = {c_void_p: "P", c_int64: "q", c_int32: "i", c_float: "f"}
+    found = []
+    for name, kind in structure._fields_:
+        at = base + getattr(structure, name).offset
+        if issubclass(kind, ctypes.Structure):
+            found += _fields_format(kind, at)
+        elif issubclass(kind, ctypes.Array):
+            size = ctypes.sizeof(kind._type_)
+            found += [(at + i * size, codes[kind._type_], size) for i in range(kind._length_)]
+        else:
+            found.append((at, codes[kind], ctypes.sizeof(kind)))
+    return found
+
+
+def packer(structure):
+    """``pack(*values)`` of a structure's scalars in order, as the bytes an entry takes: filling a ctypes
+    structure field by field costs more than a small kernel."""
+    text, at = "=", 0
+    for offset, code, size in _fields_format(structure):
+        text += "x" * (offset - at) + {"P": "Q"}.get(code, code)
+        at = offset + size
+    return struct.Struct(text + "x" * (ctypes.sizeof(structure) - at)).pack
+
+
+pack_qk_norm = packer(QkNormArgs)
+pack_store_e4m3 = packer(StoreE4m3Args)
+pack_tree_attention_e4m3 = packer(TreeAttentionE4m3Args)
+
 _lock = threading.Lock()
 _lib = None
 
@@ -330,17 +361,17 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.tv_sizeof_qk_norm_args.restype = c_int64
     lib.tv_sizeof_qk_norm_args.argtypes = []
     lib.tv_qk_norm_rope_scatter.restype = c_int32
-    lib.tv_qk_norm_rope_scatter.argtypes = [POINTER(QkNormArgs), c_void_p]
+    lib.tv_qk_norm_rope_scatter.argtypes = [c_void_p, c_void_p]
     lib.tv_sizeof_store_e4m3_args.restype = c_int64
     lib.tv_sizeof_store_e4m3_args.argtypes = []
     lib.tv_store_kvcache_e4m3.restype = c_int32
-    lib.tv_store_kvcache_e4m3.argtypes = [POINTER(StoreE4m3Args), c_void_p]
+    lib.tv_store_kvcache_e4m3.argtypes = [c_void_p, c_void_p]
     lib.tv_sizeof_tree_attention_e4m3_args.restype = c_int64
     lib.tv_sizeof_tree_attention_e4m3_args.argtypes = []
     lib.tv_tree_attention_e4m3_workspace_bytes.restype = c_int64
-    lib.tv_tree_attention_e4m3_workspace_bytes.argtypes = [POINTER(TreeAttentionE4m3Args)]
+    lib.tv_tree_attention_e4m3_workspace_bytes.argtypes = [c_void_p]   # packed bytes or a structure by reference
     lib.tv_tree_attention_e4m3.restype = c_int32
-    lib.tv_tree_attention_e4m3.argtypes = [POINTER(TreeAttentionE4m3Args), c_void_p, c_int64, c_void_p]
+    lib.tv_tree_attention_e4m3.argtypes = [c_void_p, c_void_p, c_int64, c_void_p]
     lib.tv_build_block_tables.restype = c_int32
     lib.tv_build_block_tables.argtypes = [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
                                           *[c_int32] * 4, *[c_void_p] * 5]

@@ -23,12 +23,16 @@ def _vector(tensor: torch.Tensor, what: str) -> torch.Tensor:
     """An integer vector as the kernels read it: dense int32."""
     if tensor.ndim != 1 or tensor.dtype not in _INDEX_DTYPES:
         raise ValueError(f"{what} must be an int32 or int64 vector")
+    if tensor.dtype is torch.int32 and tensor.is_contiguous():
+        return tensor
     return tensor.to(torch.int32).contiguous()
 
 
 def _table(tensor: torch.Tensor, requests: int, what: str) -> torch.Tensor:
     if tensor.ndim != 2 or tensor.shape[0] != requests or tensor.dtype not in _INDEX_DTYPES:
         raise ValueError(f"{what} must be an int32 or int64 [requests, pages] table")
+    if tensor.dtype is torch.int32 and tensor.is_contiguous():
+        return tensor
     tensor = tensor.to(torch.int32)
     return tensor if tensor.stride(1) == 1 and tensor.stride(0) >= tensor.shape[1] else tensor.contiguous()
 
@@ -69,18 +73,19 @@ def build_block_tables(lengths: torch.Tensor, free_pages: torch.Tensor, block_si
         if free_count.numel() != 1:
             raise ValueError("free_count is one integer")
         tensors.append(free_count)
-    device = _device.require_gpu(*tensors, what="build_block_tables")
+    index = _device.one_gpu("build_block_tables", *tensors)
+    device = lengths.device
     tables = torch.empty((requests, width), dtype=torch.int32, device=device)
     counts = torch.empty(requests, dtype=torch.int32, device=device)
     taken = torch.empty(1, dtype=torch.int32, device=device)
-    code = _device.call(
-        device, _lib.library().tv_build_block_tables, lengths.data_ptr(),
-        None if held_tables is None else held_tables.data_ptr(), 0 if held_tables is None else held_tables.stride(0),
-        0 if held_tables is None else held_tables.shape[1], None if held_counts is None else held_counts.data_ptr(),
-        free_pages.data_ptr(), None if free_count is None else free_count.data_ptr(), free_pages.numel(), requests,
-        block_size, width, tables.data_ptr(), counts.data_ptr(), taken.data_ptr(),
-        _device.status_word(device).data_ptr(), _device.stream_handle(device))
-    _lib.check(code, "build_block_tables")
+    held = (None, 0, 0, None) if held_tables is None else (held_tables.data_ptr(), held_tables.stride(0),
+                                                           held_tables.shape[1], held_counts.data_ptr())
+    code = _device.launch(
+        index, _lib.library().tv_build_block_tables, lengths.data_ptr(), *held, free_pages.data_ptr(),
+        None if free_count is None else free_count.data_ptr(), free_pages.numel(), requests, block_size, width,
+        tables.data_ptr(), counts.data_ptr(), taken.data_ptr(), _device.status_pointer(index))
+    if code:
+        _lib.check(code, "build_block_tables")
     return tables, counts, taken
 
 
@@ -124,21 +129,22 @@ def packed_slot_maps(cache_lens: torch.Tensor, query_lens: torch.Tensor, total_r
         if depths.numel() != total_rows:
             raise ValueError("depths needs one entry per packed row")
         tensors.append(depths)
-    device = _device.require_gpu(*tensors, what="packed_slot_maps")
+    index = _device.one_gpu("packed_slot_maps", *tensors)
+    device = cache_lens.device
     cu = torch.empty(requests + 1, dtype=torch.int32, device=device)
     request = torch.empty(total_rows, dtype=torch.int32, device=device)
     local = torch.empty(total_rows, dtype=torch.int32, device=device)
     positions = torch.empty(total_rows, dtype=torch.int64, device=device)
     slots = torch.empty(total_rows, dtype=torch.int64, device=device)
-    paged = block_tables is not None
     # An empty table or arena has no address, and every row of it is out of range.
-    pages = block_tables if paged else arena_pages
-    where = pages.data_ptr() or cu.data_ptr()
-    code = _device.call(
-        device, _lib.library().tv_packed_slot_maps, cache_lens.data_ptr(), query_lens.data_ptr(),
-        where if paged else None, pages.stride(0) if paged else 0, pages.shape[1] if paged else 0,
-        None if paged else where, 0 if paged else pages.numel(), None if depths is None else depths.data_ptr(), requests,
-        total_rows, block_size, num_blocks, cu.data_ptr(), request.data_ptr(), local.data_ptr(), positions.data_ptr(),
-        slots.data_ptr(), _device.status_word(device).data_ptr(), _device.stream_handle(device))
-    _lib.check(code, "packed_slot_maps")
+    if block_tables is not None:
+        pages = (block_tables.data_ptr() or cu.data_ptr(), block_tables.stride(0), block_tables.shape[1], None, 0)
+    else:
+        pages = (None, 0, 0, arena_pages.data_ptr() or cu.data_ptr(), arena_pages.numel())
+    code = _device.launch(
+        index, _lib.library().tv_packed_slot_maps, cache_lens.data_ptr(), query_lens.data_ptr(), *pages,
+        None if depths is None else depths.data_ptr(), requests, total_rows, block_size, num_blocks, cu.data_ptr(),
+        request.data_ptr(), local.data_ptr(), positions.data_ptr(), slots.data_ptr(), _device.status_pointer(index))
+    if code:
+        _lib.check(code, "packed_slot_maps")
     return cu, request, local, positions, slots

@@ -9,8 +9,6 @@ as a pool of head size 1 (``scales.unsqueeze(-1)``).
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _device, _lib
@@ -26,56 +24,39 @@ def store_kvcache_e4m3(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Te
     codes (it reads as NaN).  Slots must be unique; one outside the cache writes nothing and records
     TV_STATUS_BAD_SLOT.
     """
-    if key.ndim != 3 or value.shape != key.shape or key.dtype != value.dtype:
+    shape, pool = key.shape, k_cache.shape
+    if len(shape) != 3 or value.shape != shape or key.dtype is not value.dtype:
         raise ValueError("key and value must be [rows,heads,dim] of one shape and dtype")
-    rows, heads, dim = key.shape
+    rows, heads, dim = shape
     if heads < 1 or not 2 <= dim <= 256 or dim % 2:
         raise ValueError("store_kvcache_e4m3 takes even head sizes from 2 to 256")
-    if (k_cache.ndim != 4 or v_cache.shape != k_cache.shape or tuple(k_cache.shape[2:]) != (heads, dim)
-            or k_cache.dtype != E4M3 or v_cache.dtype != E4M3 or k_cache.shape[0] < 1 or k_cache.shape[1] < 1):
+    if (len(pool) != 4 or v_cache.shape != pool or pool[2] != heads or pool[3] != dim or k_cache.dtype is not E4M3
+            or v_cache.dtype is not E4M3 or pool[0] < 1 or pool[1] < 1):
         raise ValueError("caches must be float8_e4m3fn [pages,page_size,heads,dim]")
-    check_scales(k_cache, k_scale, "k_scale")
-    check_scales(v_cache, v_scale, "v_scale")
-    if slot_mapping.ndim != 1 or slot_mapping.numel() != rows or slot_mapping.dtype not in (torch.int32, torch.int64):
+    k_strides, v_strides = check_scales(pool, k_scale, "k_scale"), check_scales(pool, v_scale, "v_scale")
+    if slot_mapping.shape != (rows,) or slot_mapping.dtype not in (torch.int32, torch.int64):
         raise ValueError("slot_mapping must be an int32 or int64 [rows] vector")
-    device = _device.require_gpu(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, what="store_kvcache_e4m3")
+    index = _device.one_gpu("store_kvcache_e4m3", key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
     if rows == 0:
         return
-    a = _lib.StoreE4m3Args()
-    a.key, a.key_stride[:] = key.data_ptr(), key.stride()
-    a.value, a.value_stride[:] = value.data_ptr(), value.stride()
-    a.k_cache, a.k_cache_stride[:] = k_cache.data_ptr(), k_cache.stride()
-    a.v_cache, a.v_cache_stride[:] = v_cache.data_ptr(), v_cache.stride()
-    a.k_scale, a.k_scale_stride[:] = k_scale.data_ptr(), k_scale.stride()
-    a.v_scale, a.v_scale_stride[:] = v_scale.data_ptr(), v_scale.stride()
-    a.pool_pages, a.page_size = k_cache.shape[0], k_cache.shape[1]
-    a.slots, a.slots_stride = slot_mapping.data_ptr(), slot_mapping.stride(0)
-    a.slots_is_int64 = slot_mapping.dtype == torch.int64
-    a.rows, a.kv_heads, a.head_dim, a.dtype = rows, heads, dim, _device.dtype_code(key.dtype)
-    a.status = _device.status_word(device).data_ptr()
-    code = _device.call(device, _lib.library().tv_store_kvcache_e4m3, ctypes.byref(a), _device.stream_handle(device))
-    _lib.check(code, "store_kvcache_e4m3")
+    args = _lib.pack_store_e4m3(
+        key.data_ptr(), *key.stride(), value.data_ptr(), *value.stride(), k_cache.data_ptr(), *k_cache.stride(),
+        v_cache.data_ptr(), *v_cache.stride(), k_scale.data_ptr(), *k_strides, v_scale.data_ptr(), *v_strides, pool[0],
+        pool[1], slot_mapping.data_ptr(), slot_mapping.stride(0), slot_mapping.dtype is torch.int64, rows, heads, dim,
+        _device.dtype_code(key.dtype), _device.status_pointer(index))
+    code = _device.launch(index, _lib.library().tv_store_kvcache_e4m3, args)
+    if code:
+        _lib.check(code, "store_kvcache_e4m3")
 
 
-_METADATA_VECTORS = (("cu_seqlens_q", torch.int32), ("prefix_lens", torch.int32), ("node_counts", torch.int32),
-                     ("tree_slots", torch.int64), ("qq_bias", torch.float32), ("qq_bias_offsets", torch.int64))
-
-
-def _check_metadata(metadata, device: torch.device) -> None:
-    """The kernel reads these buffers raw: dtypes, density and sizes have to hold."""
-    requests, rows = metadata.num_requests, metadata.total_queries
-    sizes = (requests + 1, requests, requests, rows, None, requests + 1)
-    for (name, dtype), size in zip(_METADATA_VECTORS, sizes):
-        t = getattr(metadata, name)
-        if t.dtype != dtype or t.ndim != 1 or not t.is_contiguous() or (size is not None and t.numel() != size):
-            raise ValueError(f"metadata.{name} must be a contiguous {dtype} vector of the batch's size")
-        if t.device != device:
-            raise ValueError("packed attention requires CUDA queries, KV and metadata on one device")
-    tables = metadata.block_tables
-    if tables.dtype != torch.int32 or tables.ndim != 2 or tables.shape[0] != requests or tables.stride(1) != 1:
-        raise ValueError("metadata.block_tables must be int32 [requests, pages] with unit column stride")
-    if tables.device != device:
+def _vector(metadata, name: str, dtype: torch.dtype, size: int | None, index: int) -> int:
+    """Address of a metadata buffer, which the kernel reads raw: type, density and size have to hold."""
+    t = getattr(metadata, name)
+    if t.dtype is not dtype or t.ndim != 1 or not t.is_contiguous() or (size is not None and t.numel() != size):
+        raise ValueError(f"metadata.{name} must be a contiguous {dtype} vector of the batch's size")
+    if t.get_device() != index:
         raise ValueError("packed attention requires CUDA queries, KV and metadata on one device")
+    return t.data_ptr()
 
 
 def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
@@ -95,48 +76,59 @@ def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     or their table row record TV_STATUS_BAD_REQUEST (their rows are not written); pages and slots
     outside the pool record TV_STATUS_BAD_PAGE and are skipped.
     """
-    if q.ndim != 3 or q.shape[0] != metadata.total_queries:
+    m, shape, pool, kind = metadata, q.shape, k_pool.shape, q.dtype
+    if len(shape) != 3 or shape[0] != m.total_queries:
         raise ValueError("packed queries do not match the metadata")
-    if k_pool.ndim != 4 or k_pool.shape != v_pool.shape or k_pool.shape[1] != metadata.block_size:
+    if len(pool) != 4 or v_pool.shape != pool or pool[1] != m.block_size:
         raise ValueError("packed K/V page geometry does not match metadata")
-    if k_pool.dtype != E4M3 or v_pool.dtype != E4M3:
+    if k_pool.dtype is not E4M3 or v_pool.dtype is not E4M3:
         raise ValueError("packed_tree_attention_e4m3 takes float8_e4m3fn pools")
-    check_scales(k_pool, k_scale, "k_scale")
-    check_scales(v_pool, v_scale, "v_scale")
-    rows, heads, dim = q.shape
-    kv_heads = k_pool.shape[2]
-    if q.stride(-1) != 1 or k_pool.shape[3] != dim or dim not in (64, 128, 256):
+    k_strides, v_strides = check_scales(pool, k_scale, "k_scale"), check_scales(pool, v_scale, "v_scale")
+    rows, heads, dim = shape
+    q_strides = q.stride()
+    if q_strides[2] != 1 or pool[3] != dim or dim not in (64, 128, 256):
         raise ValueError("unsupported packed query/KV head geometry (head sizes 64, 128 and 256)")
     if (isinstance(num_queries_per_kv, bool) or not isinstance(num_queries_per_kv, int) or num_queries_per_kv <= 0
-            or heads != kv_heads * num_queries_per_kv):
+            or heads != pool[2] * num_queries_per_kv):
         raise ValueError("invalid packed GQA head grouping")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if kind is not torch.bfloat16 and kind is not torch.float16:
         raise ValueError("packed queries must be BF16 or FP16")
-    dtype = q.dtype if output_dtype is None else output_dtype
-    if dtype not in (q.dtype, torch.float32):
+    dtype = kind if output_dtype is None else output_dtype
+    if dtype is not kind and dtype is not torch.float32:
         raise ValueError("output dtype must match the queries or be FP32")
-    device = _device.require_gpu(q, k_pool, v_pool, k_scale, v_scale, what="packed_tree_attention_e4m3")
-    _check_metadata(metadata, device)
-    out = torch.empty((rows, heads, dim), dtype=dtype, device=device)
+    index = _device.one_gpu("packed_tree_attention_e4m3", q, k_pool, v_pool, k_scale, v_scale)
+    requests = m.num_requests
+    cu = _vector(m, "cu_seqlens_q", torch.int32, requests + 1, index)
+    prefixes = _vector(m, "prefix_lens", torch.int32, requests, index)
+    counts = _vector(m, "node_counts", torch.int32, requests, index)
+    slots = _vector(m, "tree_slots", torch.int64, rows, index)
+    bias = _vector(m, "qq_bias", torch.float32, None, index)
+    offsets = _vector(m, "qq_bias_offsets", torch.int64, requests + 1, index)
+    tables = m.block_tables
+    width = tables.shape
+    if tables.dtype is not torch.int32 or len(width) != 2 or width[0] != requests or tables.stride(1) != 1:
+        raise ValueError("metadata.block_tables must be int32 [requests, pages] with unit column stride")
+    if tables.get_device() != index:
+        raise ValueError("packed attention requires CUDA queries, KV and metadata on one device")
+    out = torch.empty(shape, dtype=dtype, device=q.device)
     if rows == 0:
         return out
-    if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    if q_strides[0] % 8 or q_strides[1] % 8 or q.data_ptr() % 16:
         q = q.contiguous()
-    m, tables = metadata, metadata.block_tables
-    args = _lib.TreeAttentionE4m3Args(
-        q.data_ptr(), q.stride(0), q.stride(1), _device.dtype_code(q.dtype), k_pool.data_ptr(), v_pool.data_ptr(),
-        k_pool.stride(), v_pool.stride(), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(), v_scale.stride(),
-        k_pool.shape[0], out.data_ptr(), out.stride(0), out.stride(1), _device.dtype_code(dtype),
-        m.cu_seqlens_q.data_ptr(), m.prefix_lens.data_ptr(), m.node_counts.data_ptr(), tables.data_ptr(),
-        tables.stride(0), tables.shape[1], m.tree_slots.data_ptr(), m.qq_bias.data_ptr(), m.qq_bias_offsets.data_ptr(),
-        m.qq_bias.numel(), m.num_requests, rows, heads, kv_heads, dim, m.block_size, scale,
-        _device.compute_units(device.index), _device.status_word(device).data_ptr())
+        q_strides = q.stride()
+    args = _lib.pack_tree_attention_e4m3(
+        q.data_ptr(), q_strides[0], q_strides[1], _device.dtype_code(kind), k_pool.data_ptr(), v_pool.data_ptr(),
+        *k_pool.stride(), *v_pool.stride(), k_scale.data_ptr(), v_scale.data_ptr(), *k_strides, *v_strides, pool[0],
+        out.data_ptr(), heads * dim, dim, _device.dtype_code(dtype), cu, prefixes, counts, tables.data_ptr(),
+        tables.stride(0), width[1], slots, bias, offsets, m.qq_bias.numel(), requests, rows, heads, pool[2], dim, pool[1],
+        scale, _device.compute_units(index), _device.status_pointer(index))
     lib = _lib.library()
     size = lib.tv_tree_attention_e4m3_workspace_bytes(args)
-    _lib.check(min(size, 0), "packed_tree_attention_e4m3")
+    if size < 0:
+        _lib.check(size, "packed_tree_attention_e4m3")
     # Scratch of this call (or of the graph being captured): no two launches share one.
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    code = _device.call(device, lib.tv_tree_attention_e4m3, args, workspace.data_ptr(), size,
-                        _device.stream_handle(device))
-    _lib.check(code, "packed_tree_attention_e4m3")
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    code = _device.launch(index, lib.tv_tree_attention_e4m3, args, workspace.data_ptr(), size)
+    if code:
+        _lib.check(code, "packed_tree_attention_e4m3")
     return out

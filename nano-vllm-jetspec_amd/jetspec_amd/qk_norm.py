@@ -9,8 +9,6 @@ slot and head.  Everything between the read and the write is fp32, rounded once;
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _device, _lib
@@ -21,53 +19,61 @@ _VALUE_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 E4M3 = torch.float8_e4m3fn
 
 
-def check_scales(pool: torch.Tensor, scale: torch.Tensor | None, what: str) -> None:
-    """The fp32 scales [pages, page_size, kv_heads] beside an e4m3 pool."""
-    if scale is None or scale.dtype != torch.float32 or scale.shape != pool.shape[:3]:
+def check_scales(shape, scale: torch.Tensor | None, what: str) -> tuple[int, ...]:
+    """The fp32 scales [pages, page_size, kv_heads] beside an e4m3 pool of `shape`; returns their strides."""
+    if scale is None or scale.dtype is not torch.float32 or scale.shape != shape[:3]:
         raise ValueError(f"{what} must be float32 [pages,page_size,kv_heads] beside its e4m3 pool")
-    if min(scale.stride()) <= 0:
+    strides = scale.stride()
+    if min(strides) <= 0:
         raise ValueError(f"{what} must have positive strides")
+    return strides
 
 
 def _check_shapes(q, k, v, q_weight, k_weight, positions, cache, k_pool, v_pool, node_slots, k_scale, v_scale, out,
-                  eps) -> torch.device:
-    """What the kernel's addresses rest on; no tensor value is read.  Returns the device."""
-    if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape:
+                  eps) -> tuple[int, bool, tuple, tuple]:
+    """What the kernel's addresses rest on; no tensor value is read.  Returns the GPU's index, whether the
+    pools are e4m3, and the shapes of q and the pools."""
+    shape, kv_shape, dtype = q.shape, k.shape, q.dtype
+    if len(shape) != 3 or len(kv_shape) != 3 or v.shape != kv_shape:
         raise ValueError("Q/K/V must be [rows,heads,dim] with equal K/V geometry")
-    rows, q_heads, dim = q.shape
-    if (q_heads < 1 or k.shape[0] != rows or k.shape[1] < 1 or k.shape[2] != dim or q_heads % k.shape[1]
-            or not 2 <= dim <= 256 or dim % 2):
+    rows, q_heads, dim = shape
+    kv_rows, kv_heads, kv_dim = kv_shape
+    if (q_heads < 1 or kv_rows != rows or kv_heads < 1 or kv_dim != dim or q_heads % kv_heads or not 2 <= dim <= 256
+            or dim % 2):
         raise ValueError("invalid Q/K/V GQA or even head geometry")
-    if q.dtype not in _VALUE_DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    if dtype not in _VALUE_DTYPES or k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError("Q/K/V must share one of BF16, FP16 and FP32")
-    if (tuple(positions.shape) != (rows,) or tuple(node_slots.shape) != (rows,)
-            or positions.dtype not in _INDEX_DTYPES or node_slots.dtype not in _INDEX_DTYPES):
+    if (positions.shape != (rows,) or node_slots.shape != (rows,) or positions.dtype not in _INDEX_DTYPES
+            or node_slots.dtype not in _INDEX_DTYPES):
         raise ValueError("positions and node_slots must be integer [rows] vectors")
-    if (cache.ndim not in (2, 3) or (cache.ndim == 3 and cache.shape[1] != 1) or cache.shape[-1] != dim
-            or cache.shape[0] < 1 or cache.dtype not in (torch.bfloat16, torch.float32)):
+    turns = cache.shape
+    if (len(turns) not in (2, 3) or (len(turns) == 3 and turns[1] != 1) or turns[-1] != dim or turns[0] < 1
+            or cache.dtype not in (torch.bfloat16, torch.float32)):
         raise ValueError("cos/sin cache must be BF16/FP32 [positions,dim] or [positions,1,dim]")
-    for weight in (q_weight, k_weight):
-        if (tuple(weight.shape) != (dim,) or weight.dtype != q_weight.dtype or weight.dtype not in (q.dtype, torch.float32)
-                or not weight.is_contiguous()):
-            raise ValueError("norm weights must be dense [dim] vectors in FP32 or the Q/K/V dtype")
-    if (k_pool.ndim != 4 or v_pool.shape != k_pool.shape or k_pool.shape[0] < 1 or k_pool.shape[1] < 1
-            or tuple(k_pool.shape[2:]) != (k.shape[1], dim) or k_pool.dtype not in (q.dtype, E4M3)
-            or v_pool.dtype != k_pool.dtype):
+    kind = q_weight.dtype
+    if (q_weight.shape != (dim,) or k_weight.shape != (dim,) or k_weight.dtype is not kind
+            or (kind is not dtype and kind is not torch.float32) or not q_weight.is_contiguous()
+            or not k_weight.is_contiguous()):
+        raise ValueError("norm weights must be dense [dim] vectors in FP32 or the Q/K/V dtype")
+    pool, stored = k_pool.shape, k_pool.dtype
+    e4m3 = stored is E4M3
+    if (len(pool) != 4 or v_pool.shape != pool or pool[0] < 1 or pool[1] < 1 or pool[2] != kv_heads or pool[3] != dim
+            or not (e4m3 or stored is dtype) or v_pool.dtype is not stored):
         raise ValueError("KV pools must match [pages,page_size,kv_heads,dim] in the Q/K/V dtype or float8_e4m3fn")
-    tensors = [q, k, v, q_weight, k_weight, positions, cache, k_pool, v_pool, node_slots]
-    if k_pool.dtype == E4M3:
-        check_scales(k_pool, k_scale, "k_scale")
-        check_scales(v_pool, v_scale, "v_scale")
-        tensors += [k_scale, v_scale]
-    elif k_scale is not None or v_scale is not None:
+    if not e4m3 and (k_scale is not None or v_scale is not None):
         raise ValueError("scales belong to float8_e4m3fn pools")
-    if out is not None:
-        if out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("output must match Q shape and dtype")
-        tensors.append(out)
+    if out is not None and (out.shape != shape or out.dtype is not dtype):
+        raise ValueError("output must match Q shape and dtype")
     if not 0.0 <= eps < float("inf"):
         raise ValueError("eps must be finite and not negative")
-    return _device.require_gpu(*tensors, what="qk_norm_rope_scatter")
+    tensors = [q, k, v, q_weight, k_weight, positions, cache, k_pool, v_pool, node_slots]
+    if e4m3:
+        check_scales(pool, k_scale, "k_scale")
+        check_scales(pool, v_scale, "v_scale")
+        tensors += [k_scale, v_scale]
+    if out is not None:
+        tensors.append(out)
+    return _device.one_gpu("qk_norm_rope_scatter", *tensors), e4m3, shape, pool
 
 
 def _check_layouts(q, k, v, q_weight, k_weight, positions, cache, k_pool, v_pool, node_slots, k_scale, v_scale, out):
@@ -127,36 +133,22 @@ def qk_norm_rope_scatter_prevalidated(q, k, v, q_weight, k_weight, positions, co
     refuses to write for a position or slot out of range (status bits, read with
     ``read_and_clear_status``) instead of touching memory it does not own.
     """
-    device = _check_shapes(q, k, v, q_weight, k_weight, positions, cos_sin_cache, k_pool, v_pool, node_slots, k_scale,
-                           v_scale, out, eps)
-    if q.shape[0] == 0:
+    index, e4m3, shape, pool = _check_shapes(q, k, v, q_weight, k_weight, positions, cos_sin_cache, k_pool, v_pool,
+                                             node_slots, k_scale, v_scale, out, eps)
+    if shape[0] == 0:
         return out
-    args = _lib.QkNormArgs()
-    rope = args.rope
-    rope.q, rope.k, rope.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    rope.q_stride[:], rope.k_stride[:], rope.v_stride[:] = q.stride(), k.stride(), v.stride()
-    rope.positions, rope.positions_stride = positions.data_ptr(), positions.stride(0)
-    rope.positions_is_int64 = positions.dtype == torch.int64
-    rope.cache, rope.cache_rows = cos_sin_cache.data_ptr(), cos_sin_cache.shape[0]
-    rope.cache_stride_row, rope.cache_stride_elem = cos_sin_cache.stride(0), cos_sin_cache.stride(-1)
-    rope.cache_dtype = _device.dtype_code(cos_sin_cache.dtype)
-    rope.k_pool, rope.v_pool = k_pool.data_ptr(), v_pool.data_ptr()
-    rope.k_pool_stride[:], rope.v_pool_stride[:] = k_pool.stride(), v_pool.stride()
-    rope.pool_pages, rope.page_size = k_pool.shape[0], k_pool.shape[1]
-    rope.node_slots, rope.slots_stride = node_slots.data_ptr(), node_slots.stride(0)
-    rope.slots_is_int64 = node_slots.dtype == torch.int64
-    rope.out, rope.out_stride[:] = out.data_ptr(), out.stride()
-    rope.rows, rope.q_heads, rope.kv_heads, rope.head_dim = q.shape[0], q.shape[1], k.shape[1], q.shape[2]
-    rope.dtype = _device.dtype_code(q.dtype)
-    rope.status = _device.status_word(device).data_ptr()
-    args.q_weight, args.k_weight = q_weight.data_ptr(), k_weight.data_ptr()
-    args.weight_dtype = _device.dtype_code(q_weight.dtype)
-    args.eps = eps
-    if k_pool.dtype == E4M3:
-        args.pool_e4m3 = 1
-        args.k_scale, args.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-        args.k_scale_stride[:], args.v_scale_stride[:] = k_scale.stride(), v_scale.stride()
-    code = _device.call(device, _lib.library().tv_qk_norm_rope_scatter, ctypes.byref(args),
-                        _device.stream_handle(device))
-    _lib.check(code, "qk_norm_rope_scatter")
+    turn = cos_sin_cache.stride()
+    scales = ((1, k_scale.data_ptr(), *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride()) if e4m3
+              else (0, 0, 0, 0, 0, 0, 0, 0, 0))
+    args = _lib.pack_qk_norm(
+        q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), positions.data_ptr(),
+        positions.stride(0), positions.dtype is torch.int64, cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], turn[0],
+        turn[-1], _device.dtype_code(cos_sin_cache.dtype), k_pool.data_ptr(), *k_pool.stride(), v_pool.data_ptr(),
+        *v_pool.stride(), pool[0], pool[1], node_slots.data_ptr(), node_slots.stride(0), node_slots.dtype is torch.int64,
+        out.data_ptr(), *out.stride(), shape[0], shape[1], pool[2], shape[2], _device.dtype_code(q.dtype),
+        _device.status_pointer(index), q_weight.data_ptr(), k_weight.data_ptr(), _device.dtype_code(q_weight.dtype), eps,
+        *scales)
+    code = _device.launch(index, _lib.library().tv_qk_norm_rope_scatter, args)
+    if code:
+        _lib.check(code, "qk_norm_rope_scatter")
     return out
