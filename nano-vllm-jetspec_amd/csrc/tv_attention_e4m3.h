@@ -39,13 +39,12 @@
 namespace tv {
 
 // A row block whose pieces the merge joins, written by the workgroup whose share its first step ends.
-struct E4m3Job {
-    int32_t pieces;        // 0: none
-    int32_t rows;          // live rows of the block
+struct alignas(16) E4m3Job {
+    uint16_t pieces;       // 0: none
+    uint16_t rows;         // live rows of the block
     int32_t first_row;     // packed row of the request's first node
     int32_t head0;         // first query head of the KV head
     int32_t row0;          // the block's first row, counted as node * group + head over the request
-    int32_t unused[3];
 };
 
 struct E4m3Params {
@@ -797,9 +796,9 @@ e4m3_attention_kernel(const E4m3Params p) {
             // step, the first u with first_step(u) >= end (each share of `total` steps is total / n long).
             const int64_t n = total < W ? total : W, end = s1 + (at.steps - run1);
             E4m3Job job = {};
-            job.pieces = static_cast<int32_t>(e4_divide(end * n + total - 1, total)) - share;
+            job.pieces = static_cast<uint16_t>(static_cast<int32_t>(e4_divide(end * n + total - 1, total)) - share);
             const int32_t row0 = at.b * ROWS, live = nodes * p.groups - row0;
-            job.rows = live < ROWS ? live : ROWS;
+            job.rows = static_cast<uint16_t>(live < ROWS ? live : ROWS);
             job.first_row = first_row;
             job.head0 = at.h * p.groups;
             job.row0 = row0;

@@ -6,29 +6,64 @@ namespace tv {
 namespace {
 
 constexpr int kMergeThreads = 256;
+constexpr int kMaxShares = 1024;     // workgroups of the attention
+constexpr int kMergeGroups = 1024;   // workgroups of the merge: four a compute unit
+// Up to here the merge launches a workgroup per share and eighth of its rows, most of which find
+// no job; above, the search for the work costs less.  One request of 777 keys, 64 shares: 13.1 us against
+// 14.1 with the search; one of 16384 keys, 512 shares: 33.6 us with it, 64.1 without.
+constexpr int kFewShares = 128;
+// A row of up to so many pieces is joined by one group of lanes, others by a whole workgroup.  Four requests
+// of 12288 keys and 250 rows, 17 pieces: 92 us so, 101 with a limit of 4; a limit above 64 costs a request
+// of 16384 keys and 64 rows 39.8 us in place of 33.6.
+constexpr int kFewPieces = 16;
 
-// Joins the pieces of one row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m).
-// Workgroup (x, y) takes the job that workgroup x of the attention left, if any, and of its rows every y-th
-// group.  Each thread keeps four pieces of a row in flight; what bounds it is their latency.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int32_t add_from(int32_t x) {
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, false);
+}
+
+// Sum over the lanes up to this one: inside the rows of 16, then each row's last lane to the rows behind.
+__device__ __forceinline__ int32_t running_sum(int32_t x) {
+    x = add_from<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8
+    x = add_from<0x112, 0xf>(x);
+    x = add_from<0x114, 0xf>(x);
+    x = add_from<0x118, 0xf>(x);
+    x = add_from<0x142, 0xa>(x);   // row_bcast 15 to rows 1 and 3
+    x = add_from<0x143, 0xc>(x);   // row_bcast 31 to rows 2 and 3
+    return x;
+}
+
+// Joins the pieces of the row blocks that several workgroups share: o = sum_i w_i O_i / sum_i w_i l_i,
+// w_i = 2^(m_i - max m).  Which blocks these are only the attention's workgroups know (their jobs), so each
+// workgroup here adds up all jobs' work, a row's pieces, and takes an equal part of the rows.  The pieces
+// come from memory and their latency bounds it, so a thread keeps four in flight.
 template <int D, int ROWS, class T>
 __global__ void __launch_bounds__(kMergeThreads)
 e4m3_merge_kernel(const E4m3Params p) {
-    constexpr int CH = D / 4, RPP = kMergeThreads / CH;
-    const int share = blockIdx.x;
-    const E4m3Job job = p.jobs[share];
-    if (job.pieces == 0) return;
-    const int ch = threadIdx.x % CH;
-    for (int row = blockIdx.y * RPP + threadIdx.x / CH; row < job.rows; row += gridDim.y * RPP) {
-        // The first piece is its share's second, the following shares begin with theirs.
-        auto piece = [&](int i) -> int64_t { return static_cast<int64_t>(2 * (share + i) + (i == 0 ? 1 : 0)) * ROWS + row; };
-        float best = -INFINITY, sum = 0.0f;
-        e4_f32x4 v = {0, 0, 0, 0};
-        for (int i0 = 0; i0 < job.pieces; i0 += 4) {
+    constexpr int CH = D / 4, kSlots = kMergeThreads / CH;
+    __shared__ e4_f32x4 part[2][kMergeThreads];
+    __shared__ float2 part_ml[2][kSlots];
+    __shared__ int32_t work[kMaxShares + 64];   // a wave looks at 64 shares from any of them on
+    __shared__ int32_t wave_work[kMergeThreads / 64], start[2];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int ch = tid % CH, slot = tid / CH;
+    int share = blockIdx.x, buffer = 0;
+    E4m3Job job;
+    float best, sum;
+    e4_f32x4 v;
+    // Pieces i0, i0 + step, ... of a row.
+    auto join = [&](int row, int i0, int step) {
+        best = -INFINITY;
+        sum = 0.0f;
+        v = e4_f32x4{0, 0, 0, 0};
+        for (; i0 < job.pieces; i0 += 4 * step) {
             float2 ml[4];
             e4_f32x4 o[4];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                const int64_t of = piece(i0 + n < job.pieces ? i0 + n : i0);
+                const int i = i0 + n * step < job.pieces ? i0 + n * step : i0;
+                // The first piece is its share's second, the following shares begin with theirs.
+                const int64_t of = static_cast<int64_t>(2 * (share + i) + (i == 0 ? 1 : 0)) * ROWS + row;
                 ml[n] = p.ws_ml[of];
                 o[n] = *reinterpret_cast<const e4_f32x4*>(p.ws_o + of * D + 4 * ch);
             }
@@ -41,22 +76,106 @@ e4m3_merge_kernel(const E4m3Params p) {
             best = top;
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                if (i0 + n >= job.pieces) break;
+                if (i0 + n * step >= job.pieces) break;
                 const float f = e4_weight(ml[n], best);
                 sum += f * ml[n].y;
                 v += f * o[n];
             }
         }
+    };
+    auto store = [&](int row) {
         const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int of = job.row0 + row, node = of / p.groups;
         e4_store4<T>(p, job.first_row + node, job.head0 + of - node * p.groups, 4 * ch, v * scale);
+    };
+    // Rows [row0, row1) of the job that `share` left.
+    auto join_rows = [&](int row0, int row1) {
+        if (job.pieces <= kFewPieces) {
+            for (int row = row0 + slot; row < row1; row += kSlots) {
+                join(row, 0, 1);
+                store(row);
+            }
+            return;
+        }
+        for (int row = row0; row < row1; ++row, buffer ^= 1) {
+            join(row, slot, kSlots);
+            part[buffer][tid] = v;
+            if (ch == 0) part_ml[buffer][slot] = make_float2(best, sum);
+            __syncthreads();   // the next row's parts go to the other buffer
+            if (slot != 0) continue;
+#pragma unroll
+            for (int n = 1; n < kSlots; ++n) best = fmaxf(best, part_ml[buffer][n].x);
+            sum = 0.0f;
+            v = e4_f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < kSlots; ++n) {
+                const float2 ml = part_ml[buffer][n];
+                const float f = e4_weight(ml, best);
+                sum += f * ml.y;
+                v += f * part[buffer][n * CH + ch];
+            }
+            store(row);
+        }
+    };
+    if (gridDim.y > 1) {
+        job = p.jobs[share];
+        if (job.pieces == 0) return;
+        const int rows = (job.rows + gridDim.y - 1) / gridDim.y, row0 = blockIdx.y * rows;
+        join_rows(row0, min(row0 + rows, static_cast<int>(job.rows)));
+        return;
+    }
+    const int per = (p.workgroups + kMergeThreads - 1) / kMergeThreads;
+    int32_t mine = 0;
+    for (int k = 0; k < per; ++k) {
+        const int j = tid * per + k;
+        const int32_t w = j < p.workgroups ? p.jobs[j].pieces * p.jobs[j].rows : 0;
+        work[j] = w;
+        mine += w;
+    }
+    int32_t upto = running_sum(mine);   // of the threads up to this one
+    if (lane == 63) wave_work[tid >> 6] = upto;
+    __syncthreads();
+    int32_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kMergeThreads / 64; ++w) {
+        if (w < (tid >> 6)) upto += wave_work[w];
+        total += wave_work[w];
+    }
+    const int32_t each = (total + static_cast<int32_t>(gridDim.x) - 1) / static_cast<int32_t>(gridDim.x);
+    const int32_t lo = blockIdx.x * each, hi = lo + each < total ? lo + each : total;
+    if (lo >= hi) return;
+    if (upto - mine <= lo && lo < upto) {
+        int32_t before = upto - mine;
+        int j = tid * per;
+        while (before + work[j] <= lo) before += work[j++];
+        start[0] = j;
+        start[1] = before;
+    }
+    __syncthreads();
+    share = __builtin_amdgcn_readfirstlane(start[0]);
+    for (int32_t before = __builtin_amdgcn_readfirstlane(start[1]); before < hi; before += work[share++]) {
+        // The next share that left a job: there is one, since `before` is below the total.
+        for (;;) {
+            const uint64_t any = __ballot(work[share + lane] != 0);
+            if (any) {
+                share += __ffsll(static_cast<unsigned long long>(any)) - 1;
+                break;
+            }
+            share += 64;
+        }
+        job = p.jobs[share];
+        const int32_t from = lo - before, to = hi - before;
+        join_rows(from <= 0 ? 0 : (from + job.pieces - 1) / job.pieces,
+                  to >= work[share] ? job.rows : (to + job.pieces - 1) / job.pieces);
     }
 }
 
 template <int D, int ROWS>
 void launch_merge(const E4m3Params& p, bool bf16, hipStream_t s) {
-    constexpr int per_pass = kMergeThreads / (D / 4), passes = ROWS / per_pass;
-    const dim3 grid(p.workgroups, passes < 16 ? passes : 16);
+    const int32_t heads = p.num_kv_heads * p.groups;
+    const int64_t most = static_cast<int64_t>(p.total_queries) * heads;   // a row is the least part
+    const dim3 grid = p.workgroups <= kFewShares ? dim3(p.workgroups, 8)
+                                                 : dim3(static_cast<uint32_t>(most < kMergeGroups ? most : kMergeGroups));
     if (bf16) hipLaunchKernelGGL((e4m3_merge_kernel<D, ROWS, __bf16>), grid, dim3(kMergeThreads), 0, s, p);
     else hipLaunchKernelGGL((e4m3_merge_kernel<D, ROWS, _Float16>), grid, dim3(kMergeThreads), 0, s, p);
 }
@@ -87,7 +206,8 @@ Launch launch_of(const tv_tree_attention_e4m3_args* a) {
     const int64_t reach = static_cast<int64_t>(a->block_table_width) * a->block_size;
     const int64_t blocks = (rows / n.shape.rows + a->num_requests) * a->num_kv_heads;
     const int64_t most = blocks * ((reach + keys - 1) / keys + (a->total_queries + keys - 1) / keys);
-    const int64_t full = static_cast<int64_t>(a->compute_units) * n.shape.per_cu;
+    int64_t full = static_cast<int64_t>(a->compute_units) * n.shape.per_cu;
+    full = full < kMaxShares ? full : kMaxShares;
     n.workgroups = static_cast<int32_t>(((most < full ? most : full) + 7) / 8 * 8);
     n.bytes = 2ll * n.workgroups * n.shape.rows * (a->head_dim * 4 + 8) + n.workgroups * static_cast<int64_t>(sizeof(E4m3Job));
     return n;

@@ -4,7 +4,8 @@
 namespace tv {
 
 // A wave's 32 rows take 128 accumulator and 64 query registers, so one wave a SIMD; steps are half
-// as long, so the staged keys take the same LDS.
+// as long, so the staged keys take the same LDS.  64 requests of 8192 to 32768 keys and 8 KV heads, blocks
+// of 32 / 64 / 128: 4 rows 1761 / 2187 / 2750 us, 64 rows 3559 / 2258 / 2804, 120 rows 7018 / 4457 / 2830.
 E4m3Shape e4m3_shape_d256(int64_t average_rows) {
     if (average_rows <= 32) return {32, 128, 2};
     if (average_rows <= 64) return {64, 128, 2};
