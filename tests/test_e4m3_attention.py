@@ -101,5 +101,5 @@ def test_the_workspace_covers_every_shape():
             a.num_requests, a.total_queries, a.num_q_heads, a.num_kv_heads, a.head_dim = 40, 40 * average, 2, 2, dim
             a.num_blocks, a.block_size, a.block_table_width, a.compute_units, a.scale = 1 << 20, 256, 100, 256, 1.0
             size = lib.tv_tree_attention_e4m3_workspace_bytes(ctypes.byref(a))
-            groups, rest = divmod(size, 2 * rows * (4 * dim + 8) + 32)   # and a job of 32 bytes
+            groups, rest = divmod(size, 2 * rows * (4 * dim + 8) + 16)   # and a job of 16 bytes
             assert rest == 0 and groups in (256, 512), (dim, average)
