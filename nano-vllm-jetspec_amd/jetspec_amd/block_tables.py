@@ -19,13 +19,18 @@ from . import _device, _lib
 _INDEX_DTYPES = (torch.int32, torch.int64)
 
 
+def _narrow(tensor: torch.Tensor) -> torch.Tensor:
+    """int32 values; what does not fit is the nearest that does, and too large or negative either way."""
+    return tensor if tensor.dtype is torch.int32 else tensor.clamp(-1 << 31, (1 << 31) - 1).to(torch.int32)
+
+
 def _vector(tensor: torch.Tensor, what: str) -> torch.Tensor:
     """An integer vector as the kernels read it: dense int32."""
     if tensor.ndim != 1 or tensor.dtype not in _INDEX_DTYPES:
         raise ValueError(f"{what} must be an int32 or int64 vector")
     if tensor.dtype is torch.int32 and tensor.is_contiguous():
         return tensor
-    return tensor.to(torch.int32).contiguous()
+    return _narrow(tensor).contiguous()
 
 
 def _table(tensor: torch.Tensor, requests: int, what: str) -> torch.Tensor:
@@ -33,7 +38,7 @@ def _table(tensor: torch.Tensor, requests: int, what: str) -> torch.Tensor:
         raise ValueError(f"{what} must be an int32 or int64 [requests, pages] table")
     if tensor.dtype is torch.int32 and tensor.is_contiguous():
         return tensor
-    tensor = tensor.to(torch.int32)
+    tensor = _narrow(tensor)
     return tensor if tensor.stride(1) == 1 and tensor.stride(0) >= tensor.shape[1] else tensor.contiguous()
 
 

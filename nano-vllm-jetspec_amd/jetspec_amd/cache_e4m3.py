@@ -67,7 +67,8 @@ def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     q is [rows, heads, dim] in BF16 or FP16, dim 64, 128 or 256; the pools are e4m3 with their scales
     and ``metadata`` is any ``PackedTreeMetadata`` (a tree of one node is a decode token, a chain tree
     a prefill chunk).  Any query group, page size and tree size; finite ``qq_bias`` values are added
-    to the scores.  The result is new, in q's dtype or FP32; a row that sees no key is zero.  BF16
+    to the scores.  The result is new, in q's dtype or FP32; a row that sees no key is zero, one that no
+    request counts (padding of a captured batch) is not written.  BF16
     results round each probability times its key's scale to BF16 once, FP16 ones keep it to 2^-17
     and FP32 ones to 2^-26.
 
@@ -93,6 +94,8 @@ def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
         raise ValueError("invalid packed GQA head grouping")
     if kind is not torch.bfloat16 and kind is not torch.float16:
         raise ValueError("packed queries must be BF16 or FP16")
+    if not -3e38 <= scale <= 3e38:   # fp32 in the kernel
+        raise ValueError("scale must be finite")
     dtype = kind if output_dtype is None else output_dtype
     if dtype is not kind and dtype is not torch.float32:
         raise ValueError("output dtype must match the queries or be FP32")

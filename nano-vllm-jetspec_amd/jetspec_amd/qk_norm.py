@@ -64,7 +64,7 @@ def _check_shapes(q, k, v, q_weight, k_weight, positions, cache, k_pool, v_pool,
         raise ValueError("scales belong to float8_e4m3fn pools")
     if out is not None and (out.shape != shape or out.dtype is not dtype):
         raise ValueError("output must match Q shape and dtype")
-    if not 0.0 <= eps < float("inf"):
+    if not 0.0 <= eps <= 3e38:   # fp32 in the kernel
         raise ValueError("eps must be finite and not negative")
     tensors = [q, k, v, q_weight, k_weight, positions, cache, k_pool, v_pool, node_slots]
     if e4m3:
@@ -133,6 +133,8 @@ def qk_norm_rope_scatter_prevalidated(q, k, v, q_weight, k_weight, positions, co
     refuses to write for a position or slot out of range (status bits, read with
     ``read_and_clear_status``) instead of touching memory it does not own.
     """
+    if out is None:
+        raise ValueError("qk_norm_rope_scatter_prevalidated writes to a given output")
     index, e4m3, shape, pool = _check_shapes(q, k, v, q_weight, k_weight, positions, cos_sin_cache, k_pool, v_pool,
                                              node_slots, k_scale, v_scale, out, eps)
     if shape[0] == 0:

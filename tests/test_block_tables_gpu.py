@@ -101,6 +101,17 @@ def test_bad_lengths_and_counts_are_clamped():
     assert read_and_clear_status(DEV) == _lib.TV_STATUS_BAD_REQUEST
 
 
+def test_values_past_32_bits_do_not_wrap():
+    """2^32 + 3 in an int64 input is no 3: too long, too far or no page, as the nearest 32-bit value is."""
+    far = torch.tensor([2 ** 32 + 3, 5], device=DEV)
+    _, counts, taken = build_block_tables(far, ints([3, 4]), 10, 4)
+    assert counts.tolist() == [0, 1] and taken.tolist() == [1]
+    assert read_and_clear_status(DEV) == _lib.TV_STATUS_NO_PAGES
+    slots = packed_slot_maps(ints([0, 0]), ints([1, 1]), 2, 4, 8, block_tables=far.unsqueeze(1))[4]
+    assert slots.tolist() == [-1, 20]
+    assert read_and_clear_status(DEV) == _lib.TV_STATUS_BAD_SLOT
+
+
 def test_no_requests():
     tables, counts, taken = build_block_tables(ints([]), ints([1, 2]), 16, 3)
     assert tables.shape == (0, 3) and counts.numel() == 0 and taken.tolist() == [0]

@@ -34,6 +34,8 @@ def operands(dim=64, dtype=torch.bfloat16):
     (dict(num_queries_per_kv=True), "head grouping"),
     (dict(num_queries_per_kv=4.0), "head grouping"),
     (dict(output_dtype=torch.float16), "output dtype"),
+    (dict(scale=1e39), "scale must be finite"),
+    (dict(scale=float("nan")), "scale must be finite"),
     ({}, "requires GPU tensors"),
 ])
 def test_refuses(change, message):
@@ -103,3 +105,25 @@ def test_the_workspace_covers_every_shape():
             size = lib.tv_tree_attention_e4m3_workspace_bytes(ctypes.byref(a))
             groups, rest = divmod(size, 2 * rows * (4 * dim + 8) + 16)   # and a job of 16 bytes
             assert rest == 0 and groups in (256, 512), (dim, average)
+
+
+def test_packed_arguments_are_the_structure():
+    """The bytes that an entry gets are those of the structure filled field by field."""
+    for pack, kind in ((_lib.pack_qk_norm, _lib.QkNormArgs), (_lib.pack_store_e4m3, _lib.StoreE4m3Args),
+                       (_lib.pack_tree_attention_e4m3, _lib.TreeAttentionE4m3Args)):
+        values = []
+
+        def fill(block):
+            for name, field in block._fields_:
+                if issubclass(field, ctypes.Structure):
+                    fill(getattr(block, name))
+                elif issubclass(field, ctypes.Array):
+                    for i in range(field._length_):
+                        values.append(len(values) + 1)
+                        getattr(block, name)[i] = values[-1]
+                else:
+                    values.append(len(values) + 1)
+                    setattr(block, name, values[-1])
+        block = kind()
+        fill(block)
+        assert pack(*values) == bytes(block)

@@ -153,6 +153,15 @@ def test_a_long_context_is_cut_and_joined(dim, groups, size):
     batch.check(F32)
 
 
+@pytest.mark.parametrize("dim, groups, sizes", [(128, 4, [15, 1, 16, 3]), (64, 4, [60, 64, 2, 33]), (128, 3, [80, 60, 90, 1]),
+                                                (256, 2, [9, 30, 7, 1])])
+def test_requests_in_a_few_pieces_each(dim, groups, sizes):
+    """Some rows are joined from a few pieces, others from more, by workgroups that share them out."""
+    batch = Batch([9001, 300, 6000, 4097], trees(sizes), dim=dim, kv_heads=8, groups=groups, page=128, gain=2.0)
+    first = batch.check(F32)
+    assert torch.equal(first, batch.run(F32))
+
+
 def test_many_requests():
     rng = np.random.default_rng(1)
     n = 900
@@ -279,6 +288,38 @@ def test_layouts():
     batch.k = torch.zeros(batch.k.numel() + 8, dtype=torch.uint8, device=DEV).view(E4M3)[8:].view(heads_first[0].shape)
     with pytest.raises(ValueError, match="start at 16 bytes"):
         batch.run()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_layouts_of_large_pages(dim):
+    """Pages of whole steps, read by the page where keys and values lie alike and key by key where not."""
+    batch = Batch([700, 256, 255], trees([20, 1, 9]), dim=dim, page=256)
+    expect = batch.check(BF16)
+    plain = batch.k, batch.v, batch.ks, batch.vs
+    stack = torch.zeros((2, 3, *batch.k.shape), dtype=torch.uint8, device=DEV).view(E4M3)
+    stack[0, 1], stack[1, 1] = batch.k, batch.v
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in plain]
+    wide = torch.zeros((*batch.ks.shape[:2], 5), device=DEV)[..., 1:3]
+    wide.copy_(batch.vs)
+    for batch.k, batch.v, batch.ks, batch.vs in ((stack[0, 1], stack[1, 1], *plain[2:]), heads_first,
+                                                 (heads_first[0], *plain[1:]), (*plain[:2], heads_first[2], plain[3]),
+                                                 (*plain[:3], wide)):
+        assert torch.equal(batch.run(), expect)
+    assert read_and_clear_status(DEV) == 0
+
+
+@pytest.mark.parametrize("dim, page", [(64, 128), (128, 128), (128, 256), (256, 64), (256, 256)])
+@pytest.mark.parametrize("bad", [-1, 10 ** 6, 2 ** 31 - 1])
+def test_bad_large_pages_are_skipped_and_reported(dim, page, bad):
+    batch = Batch([3 * page + 5, 90], trees([4, 4]), dim=dim, page=page)
+    clean = batch.run()
+    batch.meta.block_tables[0, 1] = bad
+    got = batch.run()
+    assert read_and_clear_status(DEV) == _lib.TV_STATUS_BAD_PAGE
+    assert torch.equal(got[4:], clean[4:])
+    batch.keys[0] = np.delete(batch.keys[0], np.arange(page, 2 * page))
+    batch.prefixes[0] -= page
+    batch.check(got)
 
 
 def test_scores_without_scale_and_with_a_negative_one():

@@ -65,6 +65,7 @@ def z(*shape, kind=torch.bfloat16):
     (True, dict(v_scale=z(2, 16, 1, kind=torch.float32).expand(2, 16, 2)), "positive strides"),
     (False, dict(eps=float("nan")), "eps must be"),
     (False, dict(eps=-1.0), "eps must be"),
+    (False, dict(eps=1e39), "eps must be"),
     (False, {}, "requires GPU tensors"),
     (True, {}, "requires GPU tensors"),
 ])
@@ -156,3 +157,8 @@ def test_entries_reject_bad_arguments_without_a_device():
                        (dict(pool_pages=0), invalid), (dict(slots_stride=0), invalid), (dict(rows=1 << 31), unsupported)):
         assert store(**over) == code, over
     assert store(rows=0) == _lib.TV_OK
+
+
+def test_the_launch_only_form_needs_an_output():
+    with pytest.raises(ValueError, match="given output"):
+        qk_norm_rope_scatter_prevalidated(**operands(), out=None)
