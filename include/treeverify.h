@@ -24,6 +24,16 @@
  *   tv_truncate_accepted  max_new_tokens / EOS cut of the accepted outputs and the
  *                         packed commit paths, replaces batch_runtime.py:636-655
  *
+ * and the operators around them that the reference leaves to the host or to eager
+ * PyTorch, or does not have:
+ *
+ *   tv_build_block_tables       page tables from request lengths and a free list
+ *   tv_packed_slot_maps         row maps, positions and slots from request lengths
+ *   tv_qk_norm_rope_scatter     per-head Q/K RMS norm + RoPE + K/V scatter, to pools
+ *                               of the operands' type or e4m3 with a scale per row
+ *   tv_store_kvcache_e4m3       K/V append to an e4m3 cache
+ *   tv_tree_attention_e4m3      packed tree attention over an e4m3 cache
+ *
  * Conventions
  *   - Every pointer argument is a device pointer unless its name ends in _host.
  *   - Strides are in ELEMENTS, never bytes.
