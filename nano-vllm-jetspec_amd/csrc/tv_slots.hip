@@ -9,7 +9,9 @@
 //
 // Both are prefix sums over the requests followed by independent rows.  The sums are a few KB that
 // stay in the L2, so every workgroup recomputes what it needs of them instead of waiting for a
-// launch that publishes them: one launch each, no workspace, no atomics.
+// launch that publishes them: one launch each, no workspace, no atomics.  Latency bounds both (three
+// dependent loads, two scans): tables of 2048 entries for 512 requests 5.7 us (6.3 MB, 1.1 TB/s), the maps of 250
+// rows 3.9 us, of 531 thousand rows 8.7 us (1.5 TB/s).
 #include <stdint.h>
 
 #include "tv_internal.h"
@@ -296,7 +298,8 @@ extern "C" int tv_build_block_tables(const int32_t* lengths, const int32_t* held
     p.counts = counts;
     p.taken = taken;
     p.status = status;
-    // A workgroup per request while the sums that each recomputes stay small beside its row.
+    // A workgroup per request while the sums that each recomputes stay small beside its row: 512 requests 5.7 us
+    // against 6.5 with 256 workgroups, 2000 requests 13.0 against 19.4.
     const int groups = num_requests < 1 ? 1 : num_requests < 1024 ? num_requests : 1024;
     hipLaunchKernelGGL(block_tables_kernel, dim3(groups), dim3(kThreads), 0, as_stream(stream), p);
     return check_launch("build_block_tables");
@@ -340,6 +343,9 @@ extern "C" int tv_packed_slot_maps(const int32_t* cache_lens, const int32_t* que
     p.positions = positions;
     p.slots = slots;
     p.status = status;
+    // A row a thread while that gives the chip no more workgroups than it holds, then four, which share a
+    // workgroup's scan: 130 thousand rows of 61 requests 4.7 us against 6.4 with four, a million of 1000 requests 14.1
+    // against 12.0.
     const int64_t one = (total_rows + kThreads - 1) / kThreads;
     if (one <= 1024) {
         hipLaunchKernelGGL(slot_maps_kernel<1>, dim3(one < 1 ? 1 : one), dim3(kThreads), 0, as_stream(stream), p);
