@@ -113,7 +113,7 @@ def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
         raise ValueError("metadata.block_tables must be int32 [requests, pages] with unit column stride")
     if tables.get_device() != index:
         raise ValueError("packed attention requires CUDA queries, KV and metadata on one device")
-    out = torch.empty(shape, dtype=dtype, device=q.device)
+    out = torch.empty(rows, heads, dim, dtype=dtype, device=q.device)
     if rows == 0:
         return out
     if q_strides[0] % 8 or q_strides[1] % 8 or q.data_ptr() % 16:
