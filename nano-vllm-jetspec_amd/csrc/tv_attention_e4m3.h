@@ -391,9 +391,9 @@ e4m3_attention_kernel(const E4m3Params p) {
     const int wm = wave % WM, wk = wave / WM;
     const int c = lane & 31, half = lane >> 5;
 
+    if (tid < NBUF) lds_bad[tid] = 0;   // ordered before the first mark by the barrier behind the search
     // Neighbouring shares go to one XCD (workgroups are dealt to the 8 in turn), whose L2 then
     // holds what they have in common: the scales of a key's heads, the keys of a head's blocks.
-    if (tid < NBUF) lds_bad[tid] = 0;   // the search's barriers follow
     const int W = p.workgroups;
     int64_t total = 0, s0 = 0, s1 = 0;   // all steps; this share's
     int share = 0;
@@ -407,6 +407,9 @@ e4m3_attention_kernel(const E4m3Params p) {
     });
     if (tid == 0) p.jobs[share].pieces = 0;
     if (!any) return;
+    // Two buffers stage the first step, and may mark it, without a barrier of their own (the search has none for up
+    // to 64 requests); with one buffer every step begins with a barrier.
+    if constexpr (NBUF == 2) __syncthreads();
     share = __builtin_amdgcn_readfirstlane(share);
     int todo = __builtin_amdgcn_readfirstlane(static_cast<int>(s1 - s0));   // steps not yet run
 
