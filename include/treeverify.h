@@ -752,7 +752,7 @@ typedef struct tv_tree_attention_e4m3_args {
     const int64_t* qq_bias_offsets;      /* [R+1] */
     int64_t qq_bias_elems;
     int32_t num_requests, total_queries, num_q_heads, num_kv_heads, head_dim, block_size;
-    float scale;
+    float scale;                         /* at most 2.3e38 in size: scale * log2(e) is fp32 */
     int32_t compute_units;               /* of the device: sizes the launch */
     int32_t* status;                     /* optional */
 } tv_tree_attention_e4m3_args;

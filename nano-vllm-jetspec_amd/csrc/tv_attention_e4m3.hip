@@ -16,6 +16,8 @@ constexpr int kFewShares = 128;
 // of 12288 keys and 250 rows, 17 pieces: 92 us so, 101 with a limit of 4; a limit above 64 costs a request
 // of 16384 keys and 64 rows 39.8 us in place of 33.6.
 constexpr int kFewPieces = 16;
+// Scores are in units of log2: scale * log2(e) is an fp32 number, which it is up to 2.358e38.
+constexpr float kMaxScale = 2.3e38f;
 
 template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ int32_t add_from(int32_t x) {
@@ -227,8 +229,8 @@ int check(const tv_tree_attention_e4m3_args* a) {
     if (a->out_dtype != a->in_dtype && a->out_dtype != TV_F32) {
         return fail(TV_ERR_UNSUPPORTED, "%s: output must be fp32 or of the queries' type", what);
     }
-    if (!(a->scale == a->scale) || a->scale > 3.0e38f || a->scale < -3.0e38f) {
-        return fail(TV_ERR_INVALID, "%s: scale must be finite", what);
+    if (!(fabsf(a->scale) <= kMaxScale)) {
+        return fail(TV_ERR_INVALID, "%s: scale must be finite, and its product with log2(e) in fp32", what);
     }
     if (a->num_blocks < 1 || a->block_size < 1 || a->block_table_width < 0 || a->block_table_stride < 0 ||
         a->qq_bias_elems < 0 || a->compute_units < 1) {

@@ -94,8 +94,8 @@ def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
         raise ValueError("invalid packed GQA head grouping")
     if kind is not torch.bfloat16 and kind is not torch.float16:
         raise ValueError("packed queries must be BF16 or FP16")
-    if not -3e38 <= scale <= 3e38:   # fp32 in the kernel
-        raise ValueError("scale must be finite")
+    if not -2.3e38 <= scale <= 2.3e38:   # scale * log2(e) is fp32 in the kernel
+        raise ValueError("scale must be finite, and its product with log2(e) in fp32")
     dtype = kind if output_dtype is None else output_dtype
     if dtype is not kind and dtype is not torch.float32:
         raise ValueError("output dtype must match the queries or be FP32")
