@@ -772,13 +772,17 @@ e4m3_attention_kernel(const E4m3Params p) {
             float negative = m == -INFINITY ? 0.0f : -m;
             e4_f32x16 pr, next = {};
             if (kEarly && n + 1 < TILES) next = products(kb + (key + WK * kE4Tile) * 2 * D);
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            // Both times in one order: a row whose neighbours raise their reference is summed a second time.
+            auto exponentials = [&]() {
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                pr[i] = __builtin_amdgcn_exp2f(fmaf(x[i], ks[i], negative));
-                sum[i & 3] += pr[i];
-            }
-            float tile_sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                for (int i = 0; i < 16; ++i) {
+                    pr[i] = __builtin_amdgcn_exp2f(fmaf(x[i], ks[i], negative));
+                    sum[i & 3] += pr[i];
+                }
+                return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            };
+            float tile_sum = exponentials();
             const bool over = !(tile_sum <= 256.0f) || m == -INFINITY;
             if (__any(over)) {   // other rows of the wave keep their reference: no row depends on another
                 float top = x[0] * ks[0];
@@ -791,12 +795,7 @@ e4m3_attention_kernel(const E4m3Params p) {
 #pragma unroll
                 for (int i = 0; i < NB; ++i) acc[i] *= factor;
                 negative = m == -INFINITY ? 0.0f : -m;
-                tile_sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    pr[i] = __builtin_amdgcn_exp2f(fmaf(x[i], ks[i], negative));
-                    tile_sum += pr[i];
-                }
+                tile_sum = exponentials();
             }
             l += tile_sum;
             e4_bf16x8 pb[TERMS][2];
