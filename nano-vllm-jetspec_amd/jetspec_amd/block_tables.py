@@ -24,13 +24,19 @@ def _narrow(tensor: torch.Tensor) -> torch.Tensor:
     return tensor if tensor.dtype is torch.int32 else tensor.clamp(-1 << 31, (1 << 31) - 1).to(torch.int32)
 
 
-def _vector(tensor: torch.Tensor, what: str) -> torch.Tensor:
+def _narrow_places(tensor: torch.Tensor) -> torch.Tensor:
+    """int32 cache lengths or depths: one too large for int32 becomes the lowest, since the nearest is a place
+    that a row could have, and would map to without a word."""
+    return tensor if tensor.dtype is torch.int32 else tensor.clamp(-1 << 31, 1 << 31).to(torch.int32)   # 2^31 wraps
+
+
+def _vector(tensor: torch.Tensor, what: str, narrow=_narrow) -> torch.Tensor:
     """An integer vector as the kernels read it: dense int32."""
     if tensor.ndim != 1 or tensor.dtype not in _INDEX_DTYPES:
         raise ValueError(f"{what} must be an int32 or int64 vector")
     if tensor.dtype is torch.int32 and tensor.is_contiguous():
         return tensor
-    return _narrow(tensor).contiguous()
+    return narrow(tensor).contiguous()
 
 
 def _table(tensor: torch.Tensor, requests: int, what: str) -> torch.Tensor:
@@ -109,16 +115,16 @@ def packed_slot_maps(cache_lens: torch.Tensor, query_lens: torch.Tensor, total_r
     request -1, position 0 and slot -1, which the appends skip.
 
     A page outside ``[0, num_blocks)`` or past the table or the arena gives slot -1 and records
-    TV_STATUS_BAD_SLOT; negative cache lengths or positions record TV_STATUS_BAD_POSITION; negative
-    query lengths (counted as 0) and batches of more than ``total_rows`` rows record
-    TV_STATUS_BAD_REQUEST.
+    TV_STATUS_BAD_SLOT; negative cache lengths or positions, and int64 cache lengths or depths past
+    int32, give slot -1 and record TV_STATUS_BAD_POSITION; negative query lengths (counted as 0) and
+    batches of more than ``total_rows`` rows record TV_STATUS_BAD_REQUEST.
     """
     total_rows, block_size, num_blocks = int(total_rows), int(block_size), int(num_blocks)
     if total_rows < 0 or block_size < 1 or num_blocks < 1:
         raise ValueError("packed_slot_maps requires a row count, a positive block size and a positive pool size")
     if (block_tables is None) == (arena_pages is None):
         raise ValueError("packed_slot_maps maps through either block_tables or arena_pages")
-    cache_lens, query_lens = _vector(cache_lens, "cache_lens"), _vector(query_lens, "query_lens")
+    cache_lens, query_lens = _vector(cache_lens, "cache_lens", _narrow_places), _vector(query_lens, "query_lens")
     requests = int(cache_lens.numel())
     if query_lens.numel() != requests:
         raise ValueError("cache_lens and query_lens disagree on the request count")
@@ -130,7 +136,7 @@ def packed_slot_maps(cache_lens: torch.Tensor, query_lens: torch.Tensor, total_r
         arena_pages = _vector(arena_pages, "arena_pages")
         tensors.append(arena_pages)
     if depths is not None:
-        depths = _vector(depths, "depths")
+        depths = _vector(depths, "depths", _narrow_places)
         if depths.numel() != total_rows:
             raise ValueError("depths needs one entry per packed row")
         tensors.append(depths)
