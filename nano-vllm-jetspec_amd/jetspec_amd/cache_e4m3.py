@@ -117,7 +117,7 @@ def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     if rows == 0:
         return out
     if q_strides[0] % 8 or q_strides[1] % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)   # dense ones too: their start may be what is off
         q_strides = q.stride()
     args = _lib.pack_tree_attention_e4m3(
         q.data_ptr(), q_strides[0], q_strides[1], _device.dtype_code(kind), k_pool.data_ptr(), v_pool.data_ptr(),
