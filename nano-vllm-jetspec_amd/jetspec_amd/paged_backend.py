@@ -422,7 +422,7 @@ def _launch(q, k_pool, v_pool, metadata, scale, out, *, chunk_keys: int = 0, exa
     if entry is not None and entry[0] is _FP32_ROUTE:
         return _launch_fp32(entry[1], q, out, scale, stream, entry[2])
     if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)   # dense ones too: their start may be what is off
     if torch.cuda.is_current_stream_capturing():
         return _launch_captured(q, k_pool, v_pool, metadata, scale, out, num_kv_heads, queries_per_kv, chunk_keys,
                                 stream, exact)
@@ -625,7 +625,7 @@ def _legacy_mfma(q, k_pool, v_pool, req, scale, num_queries_per_kv: int, block_s
     ws_bytes = workspace_bytes(info.workspace_bytes, info.num_partial_slots, int(q.shape[2]))
     workspace = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=device)
     if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)   # dense ones too: their start may be what is off
     a = _lib.TreeAttentionArgs()
     a.q = q.data_ptr()
     a.q_stride_row, a.q_stride_head = q.stride(0), q.stride(1)
