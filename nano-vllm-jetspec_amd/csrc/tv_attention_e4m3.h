@@ -29,11 +29,13 @@
 // stand: product slot t of lane half g is key 16*kk + 8*(t/4) + 4*g + t%4, which the transposing
 // reads of V deliver.
 //
-// What bounds it.  Few rows: memory; single tokens of 32 requests over 16384 keys of 8 heads of 128 read 4.3 TB/s, 5.2
-// where the slots of a head are contiguous.  Many rows: the matrix unit (36 % busy), the vector unit (39 %:
-// exponentials, scales, rounding, conversion) and LDS (37 %), which the two waves of a SIMD hardly overlap; 64
-// trees of 64 nodes and 4 query heads a KV head over 8192 to 32768 keys take 1.85 ms, 0.80 PFLOP/s.  Whole steps
-// with one of these parts left out take 7 to 12 % less.
+// What bounds it.  Few rows: memory; single tokens of 32 requests over 16384 keys of 8 heads of 128 read 4.3 TB/s,
+// 5.2 where the slots of a head are contiguous.  At head size 64 two heads share a 128-byte line and are read at
+// different times: 64 requests over 8192 to 32768 keys, 557 us against 316 with a head's slots contiguous.  Many
+// rows: the matrix unit (36 % busy), the vector unit (39 %: exponentials, scales, rounding, conversion) and LDS
+// (37 %), which the two waves of a SIMD hardly overlap; 64 trees of 64 nodes and 4 query heads a KV head over 8192
+// to 32768 keys (uniform) take 1.85 ms, 0.80 PFLOP/s.  Whole steps with one of these parts left out take 7 to 12 %
+// less.
 #pragma once
 
 #include <float.h>

@@ -5,9 +5,11 @@ namespace tv {
 
 // Few rows put the four waves side by side on the keys, many rows on the rows.  Where row blocks of 256
 // would be well filled, eight waves share each key that is moved and converted, with two buffers in place
-// of a second workgroup.  64 requests of 8192 to 32768 keys and 8 KV heads, blocks of 32 / 64 / 128 / 256:
+// of a second workgroup.  64 requests of 8192 to 32768 keys (uniform) and 8 KV heads, blocks of 32 / 64 / 128 / 256:
 // 64 rows 1340 / 773 / 880 / 1268 us, 120 rows 2439 / 1521 / 1089 / 1298, 250 rows 4949 / 3025 / 2162 / 1841;
-// of 256 to 4096 keys, 4 rows 94 / 106 / 120 / 187; 8 such requests of 160 rows 60 / 52 / 49 / 52.
+// of 256 to 4096 keys, 4 rows 94 / 106 / 120 / 187; 8 such requests of 160 rows 60 / 52 / 49 / 52.  Against the rule: 4
+// rows over the long ones 658 / 600.  It sees the batch's average rows, not its lengths, and requests of unlike
+// rows share one block size: 63 single tokens beside a chunk of 512 nodes run in blocks of 64.
 E4m3Shape e4m3_shape_d128(int64_t average_rows) {
     if (average_rows <= 32) return {32, 256, 2};
     if (average_rows <= 64) return {64, 256, 2};

@@ -4,7 +4,7 @@
 namespace tv {
 
 // A wave's 32 rows take 128 accumulator and 64 query registers, so one wave a SIMD; steps are half
-// as long, so the staged keys take the same LDS.  64 requests of 8192 to 32768 keys and 8 KV heads, blocks
+// as long, so the staged keys take the same LDS.  64 requests of 8192 to 32768 keys (uniform) and 8 KV heads, blocks
 // of 32 / 64 / 128: 4 rows 1777 / 2076 / 2750 us, 60 rows 3559 / 2107 / 2804, 120 rows 7018 / 4457 / 2830; 64
 // rows with two waves on the rows alone, two workgroups a CU: 60 rows 2339.
 E4m3Shape e4m3_shape_d256(int64_t average_rows) {

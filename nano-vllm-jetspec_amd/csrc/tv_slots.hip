@@ -344,8 +344,9 @@ extern "C" int tv_packed_slot_maps(const int32_t* cache_lens, const int32_t* que
     p.slots = slots;
     p.status = status;
     // A row a thread while that gives the chip no more workgroups than it holds, then four, which share a
-    // workgroup's scan: 130 thousand rows of 61 requests 4.7 us against 6.4 with four, a million of 1000 requests 14.1
-    // against 12.0.
+    // workgroup's scan.  One against four: 130 thousand rows of 61 requests 4.7 / 6.4 us, 508 thousand of 250 7.9 / 8.6, 531
+    // thousand of 61 8.0 / 8.7, 576 thousand of 16 7.8 / 8.0, 608 thousand of 4 7.8 / 7.5, a million of one 9.6 / 8.3, of
+    // 1000 13.6 / 11.8.  The two meet near 600 thousand rows: from the border, 262 thousand, up to there four cost up to 9 %.
     const int64_t one = (total_rows + kThreads - 1) / kThreads;
     if (one <= 1024) {
         hipLaunchKernelGGL(slot_maps_kernel<1>, dim3(one < 1 ? 1 : one), dim3(kThreads), 0, as_stream(stream), p);

@@ -5,7 +5,8 @@
 ``scale = max(amax / 448, 2^-100)``, so every value is within half an e4m3 step of the appended one
 and no calibration is needed.  Half the bytes of a bf16 cache, plus 4 per row.  Since the scales
 are indexed as the slots are, ``copy_accepted_kv`` commits both: the codes as any pool, the scales
-as a pool of head size 1 (``scales.unsqueeze(-1)``).
+as a pool of head size 1 (``scales.unsqueeze(-1)``).  The appends fill pools of any even head size up to
+256; the attention reads those of 64, 128 and 256.
 """
 from __future__ import annotations
 
@@ -70,7 +71,7 @@ def packed_tree_attention_e4m3(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     to the scores.  The result is new, in q's dtype or FP32; a row that sees no key is zero, one that no
     request counts (padding of a captured batch) is not written.  BF16
     results round each probability times its key's scale to BF16 once, FP16 ones keep it to 2^-17
-    and FP32 ones to 2^-26.
+    and FP32 ones to 2^-26: a BF16 result with less error is the FP32 one, rounded.
 
     Every length, page and slot is read on the device, so a captured call follows the staged
     metadata, and no state is kept between calls.  Requests that reach outside the batch, the bias
