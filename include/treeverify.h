@@ -33,6 +33,12 @@
  *                               of the operands' type or e4m3 with a scale per row
  *   tv_store_kvcache_e4m3       K/V append to an e4m3 cache
  *   tv_tree_attention_e4m3      packed tree attention over an e4m3 cache
+ *   tv_rotary_scatter           rotation from positions and frequencies (half or
+ *                               interleaved pairs, part of the head) + K/V scatter
+ *   tv_window_attention         packed tree attention with a sliding window and first
+ *                               tokens that stay visible
+ *   tv_token_logprobs           log probabilities of given tokens, entropy and top
+ *                               alternatives of logits rows
  *
  * Conventions
  *   - Every pointer argument is a device pointer unless its name ends in _host.
@@ -760,6 +766,113 @@ typedef struct tv_tree_attention_e4m3_args {
 int64_t tv_sizeof_tree_attention_e4m3_args(void);
 int64_t tv_tree_attention_e4m3_workspace_bytes(const tv_tree_attention_e4m3_args* args);
 int tv_tree_attention_e4m3(const tv_tree_attention_e4m3_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Packed tree attention with a sliding window: the row of node i at position P_i sees
+ * prefix key j iff P_i - j < window or j < sinks, and the tree nodes j <= i that its bias
+ * shows it (not -inf; finite values are added to the scores) at P_i - P_j < window or
+ * P_j < sinks.  positions[row] is the request's prefix length plus the node's depth, so it
+ * lies in [prefix, prefix + i]; one outside is taken as the nearer end and records
+ * TV_STATUS_BAD_POSITION.  Table entries of pages that no row sees are not read and may
+ * hold anything.  A row that sees no key is zero; rows that no request counts are left
+ * as they were.  Head sizes are multiples of 8 up to 256, any query group, page and tree
+ * size.  No counterpart in the reference.
+ *
+ * Requests that reach outside the batch, the bias or their table row record
+ * TV_STATUS_BAD_REQUEST and are left out; pages and slots outside the pool record
+ * TV_STATUS_BAD_PAGE and their keys are skipped.  An infinite or NaN value row makes NaN
+ * of a row that sees it, or keeps its infinities; rows that do not see it are unaffected.
+ * `workspace` is tv_window_attention_workspace_bytes() bytes (it may be 0), the call's own
+ * until its work is done.
+ */
+typedef struct tv_window_attention_args {
+    const void* q;                       /* [Q, Hq, D], head dim contiguous */
+    int64_t q_stride_row, q_stride_head;
+    int32_t in_dtype;                    /* TV_BF16 or TV_F16: q and the pools */
+    const void* k_pool;                  /* [N, B, Hkv, D], head dim contiguous */
+    const void* v_pool;
+    int64_t k_stride[4];
+    int64_t v_stride[4];
+    int64_t num_blocks;
+    void* out;                           /* [Q, Hq, D], head dim contiguous */
+    int64_t out_stride_row, out_stride_head;
+    int32_t out_dtype;                   /* in_dtype or TV_F32 */
+    const int32_t* cu_seqlens_q;         /* [R+1] */
+    const int32_t* prefix_lens;          /* [R] */
+    const int32_t* node_counts;          /* [R] */
+    const int32_t* block_tables;         /* [R, block_table_stride], block_table_width pages a row */
+    int64_t block_table_stride;
+    int32_t block_table_width;
+    const int64_t* tree_slots;           /* [Q] */
+    const float* qq_bias;
+    const int64_t* qq_bias_offsets;      /* [R+1] */
+    int64_t qq_bias_elems;
+    const void* positions;               /* [Q], int32 or int64 */
+    int32_t positions_is_int64;
+    int32_t window, sinks;               /* at least 1, at least 0 */
+    int32_t num_requests, total_queries, num_q_heads, num_kv_heads, head_dim, block_size;
+    float scale;                         /* at most 2.3e38 in size: scale * log2(e) is fp32 */
+    int32_t compute_units;               /* of the device: sizes the launch */
+    int32_t* status;                     /* optional */
+} tv_window_attention_args;
+
+int64_t tv_sizeof_window_attention_args(void);
+int64_t tv_window_attention_workspace_bytes(const tv_window_attention_args* args);
+int tv_window_attention(const tv_window_attention_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Rotation of Q and K from positions and frequencies, with the K/V scatter: row i's pair p
+ * of a head, (x[p], x[n + p]) or with `interleaved` (x[2p], x[2p + 1]), n = num_frequencies,
+ * is turned by positions[i] * frequencies[p] radians (the angle in 64 bits) and multiplied
+ * by gain; dimensions from 2n on are copied.  Q goes to out, K to its slot, V is copied to
+ * its slot, in fp32 rounded once.  Slot -1 skips a row; a slot or position outside (positions
+ * are in [0, 2^31)) writes nothing for the row and sets TV_STATUS_BAD_SLOT / _BAD_POSITION.
+ * `cache` and its fields of the argument block are not used.  Extends tv_rope_scatter.
+ */
+typedef struct tv_rotary_args {
+    tv_rope_scatter_args rope;           /* dtype bf16, f16 or fp32: q, k, v, out and the pools */
+    const double* frequencies;           /* [num_frequencies] */
+    int32_t num_frequencies;             /* 1 to head_dim / 2 */
+    int32_t interleaved;
+    float gain;
+} tv_rotary_args;
+
+int64_t tv_sizeof_rotary_args(void);
+int tv_rotary_scatter(const tv_rotary_args* args, void* stream);
+
+/*
+ * Per result row i, over the logits x of row rows[i] (row i itself where `rows` is NULL):
+ *   logprobs[i, j] = x[token_ids[i, j]] - log sum e^x,  0 for token -1 (none),
+ *   entropy[i]     = log sum e^x - sum e^x x / sum e^x,
+ *   top_ids[i, :]  = the `top` largest logits' indices, NaN above all, ties to the lowest
+ *                    index; top_logprobs their log probabilities.
+ * Words at -inf have probability zero.  A row with a NaN or +inf, or of only -inf, has NaN
+ * in its numbers.  A row index of -1 (padding) gives zeros and ids -1; other indices and
+ * tokens outside give NaN (ids -1) and record TV_STATUS_BAD_REQUEST.  top is at most 64 and
+ * at most vocab.  `workspace` is tv_token_logprobs_workspace_bytes() bytes (it may be 0).
+ */
+typedef struct tv_token_logprobs_args {
+    const void* logits;                  /* [num_logits, vocab], unit column stride */
+    int64_t logits_stride;
+    int64_t num_logits, vocab;
+    int32_t dtype;
+    const void* rows;                    /* [num_rows] or NULL */
+    int32_t rows_is_int64;
+    const void* token_ids;               /* [num_rows, tokens] dense */
+    int32_t tokens_is_int64;
+    int64_t num_rows;
+    int32_t tokens, top;
+    float* logprobs;                     /* [num_rows, tokens] */
+    float* entropy;                      /* [num_rows] */
+    int64_t* top_ids;                    /* [num_rows, top] */
+    float* top_logprobs;                 /* [num_rows, top] */
+    int32_t compute_units;
+    int32_t* status;
+} tv_token_logprobs_args;
+
+int64_t tv_sizeof_token_logprobs_args(void);
+int64_t tv_token_logprobs_workspace_bytes(const tv_token_logprobs_args* args);
+int tv_token_logprobs(const tv_token_logprobs_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Allocation-free variant of tv_tree_attention.  No counterpart in the reference: it is

@@ -35,7 +35,9 @@ SOURCES = ("tv_common.cpp", "tv_plan.cpp", "tv_kvcache.hip", "tv_attention.hip",
            "tv_attention_fp32.hip", "tv_attention_rows.hip",
            "tv_attention_e4m3.hip", "tv_attention_e4m3_d64.hip", "tv_attention_e4m3_d128.hip",
            "tv_attention_e4m3_d256.hip",
-           "tv_rope.hip", "tv_qk_norm.hip", "tv_slots.hip", "tv_accept.hip", "tv_metadata.hip", "tv_plan_device.hip")
+           "tv_window.hip", "tv_window_d64.hip", "tv_window_d128.hip", "tv_window_d256.hip",
+           "tv_rope.hip", "tv_qk_norm.hip", "tv_rotary.hip", "tv_slots.hip", "tv_accept.hip",
+           "tv_logprobs.hip", "tv_metadata.hip", "tv_plan_device.hip")
 
 # Packed-FP32 VALU instructions are kept out of the device code (they are not
 # needed: the hot loops are MFMA and single-precision VALU work).

@@ -1,0 +1,575 @@
+// Log probabilities of given tokens, the entropy and the top alternatives of logits rows, for gfx950.
+//
+// Row x of V logits, in one pass:
+//     Z = sum_j 2^(c x_j - R),  E = sum_j 2^(c x_j - R) (c x_j - R),  c = log2 e, R a reference near c max x,
+//     log p_t = x_t - (R + log2 Z) / c,   entropy = (log2 Z - E / Z) / c,
+// and the k largest logits by (value, lowest index).  A lane keeps its own R, Z and E; R is raised, and the
+// sums scaled, only when a logit passes it by more than 8, so terms stay below 2^12.  A word at -inf adds
+// nothing to either sum (its exponent is held at -200, whose power is zero).
+//
+// The top k: a wave keeps the 64 largest it has seen, sorted, a lane each, and a queue in LDS.  What does
+// not pass the k-th of them, which per 16-byte unit is one comparison with the unit's maximum, is done with;
+// the rest is queued, and a full queue is sorted and merged (bitonic).  The first bound is the k-th largest
+// of the lanes' maxima over the first units.  A wave's elements come in the order of their indices, so a
+// later one of equal value never counts, and the waves' lists are joined by their order as 64-bit numbers,
+// value before index: the result depends on no timing.
+//
+// Memory bounds it where logits are plenty (the logits are read once); the vector unit is close behind:
+// about ten instructions an element for 16-bit logits, of which the exponential takes four slots.
+#include <math.h>
+#include <stdint.h>
+
+#include "tv_internal.h"
+
+namespace tv {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kUnroll = 4;      // units a lane loads at a time
+constexpr int kMostTop = 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kMargin = 8.0f;
+// R is c x rounded to fp32, and c x - R has to stay near zero for the x it was made of: so up to 2^16.  Larger
+// logits (masks of -1e9 or the type's lowest value) are summed against references of their own, below, to
+// zero, and above all others.  A row left with such a one is summed again, by differences.
+constexpr float kFar = 65536.0f, kFarLow = -9.0e4f, kFarHigh = 1.0e5f;
+
+struct LogprobParams {
+    const char* logits;
+    int64_t stride;                 // elements
+    int64_t held, vocab;
+    const void* rows;
+    int32_t rows64;
+    const void* tokens;
+    int32_t tokens64;
+    int64_t num_rows;
+    int32_t given, top, splits;
+    float* logprobs;
+    float* entropy;
+    int64_t* top_ids;
+    float* top_logprobs;
+    float* ws_sums;                 // [rows * splits, 4]
+    uint64_t* ws_top;               // [rows * splits, top]
+    int32_t* status;
+};
+
+struct LogBf16 {
+    typedef uint16_t storage;
+    static constexpr uint32_t kNone = 0xff80ff80u;   // -inf in every element of a word
+    static __device__ __forceinline__ float load(storage s) { return __uint_as_float(static_cast<uint32_t>(s) << 16); }
+};
+struct LogF16 {
+    typedef uint16_t storage;
+    static constexpr uint32_t kNone = 0xfc00fc00u;
+    static __device__ __forceinline__ float load(storage s) { return static_cast<float>(__builtin_bit_cast(_Float16, s)); }
+};
+struct LogF32 {
+    typedef float storage;
+    static constexpr uint32_t kNone = 0xff800000u;
+    static __device__ __forceinline__ float load(storage s) { return s; }
+};
+
+__device__ __forceinline__ int64_t load_int(const void* p, int is64, int64_t i) {
+    return is64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
+}
+
+// Order-preserving map of floats to integers: -0 equals +0, a NaN lies above everything; never 0.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    if (x != x) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order) {
+    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+// A value that whatever has a higher order than `order` is not at or below.
+__device__ __forceinline__ float bound_of(uint32_t order) {
+    if (order == 0xffffffffu) return INFINITY;
+    return order == 0x7fffffffu ? -__uint_as_float(1u) : value_of(order);   // 0x7fffffff: -0, which no value has
+}
+
+__device__ __forceinline__ uint64_t entry_of(float x, int64_t index) {
+    return static_cast<uint64_t>(order_of(x)) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(index));
+}
+
+__device__ __forceinline__ uint64_t from_lane_xor(uint64_t v, int mask) {
+    return static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), mask));
+}
+
+// Bitonic steps over the wave's 64 lanes, largest first.
+__device__ __forceinline__ uint64_t merged(uint64_t v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 32; j > 0; j >>= 1) {
+        const uint64_t o = from_lane_xor(v, j);
+        v = ((lane & j) == 0) == (v > o) ? v : o;
+    }
+    return v;
+}
+__device__ __forceinline__ uint64_t sorted(uint64_t v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 2; k < 64; k <<= 1) {
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const uint64_t o = from_lane_xor(v, j);
+            v = (((lane & j) == 0) == ((lane & k) == 0)) == (v > o) ? v : o;
+        }
+    }
+    return merged(v);
+}
+
+// A wave's largest entries.  Entries are distinct, but for the empty one, 0.
+struct WaveTop {
+    uint64_t best = 0;     // sorted over the lanes
+    uint64_t kth = 0;      // the top-th of them
+    uint64_t* queue;       // LDS of the wave's own
+    int queued = 0, top;
+
+    // Merges the last 64 entries of the queue.
+    __device__ __forceinline__ void flush() {
+        const int lane = threadIdx.x & 63, from = queued > 64 ? queued - 64 : 0;
+        // One wave's exchange: its LDS operations run in order, the compiler's must too.
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const uint64_t mine = from + lane < queued ? queue[from + lane] : 0;
+        queued = from;
+        const uint64_t other = static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(sorted(mine)), 63 - lane));
+        best = merged(best > other ? best : other);
+        kth = static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(best), top - 1));
+    }
+    __device__ __forceinline__ void push(bool want, uint64_t entry) {
+        const uint64_t lanes = __ballot(want);
+        if (want) {
+            const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
+                                                         __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0));
+            queue[queued + before] = entry;
+        }
+        queued += __popcll(lanes);
+    }
+};
+
+// Sums over one row or a part of it.
+struct Sums {
+    float r = -INFINITY, z = 0.0f, e = 0.0f;   // the reference times log2 e, and the sums against it
+
+    // Against another reference, at or above this one's unless there is nothing to scale.
+    __device__ __forceinline__ void rescale(float to) {
+        if (r == to) return;
+        const float f = __builtin_amdgcn_exp2f(r - to);
+        const bool none = z == 0.0f || f == 0.0f;   // nothing yet, or nothing left
+        e = none ? 0.0f : (e - (to - r) * z) * f;
+        z = z != z ? z : none ? 0.0f : z * f;
+        r = to;
+    }
+    __device__ __forceinline__ void add(Sums o) {
+        const float top = fmaxf(r, o.r);
+        rescale(top);
+        o.rescale(top);
+        z += o.z;
+        e += o.e;
+    }
+};
+
+// Joins the waves' lists and sums in LDS: `list` gets the largest, thread 0 holds the sums.
+struct Joined {
+    uint64_t all[kThreads];
+    float sums[kWaves][3];
+    uint64_t list[kMostTop];
+};
+
+template <bool TOP>
+__device__ __forceinline__ Sums join(Joined& s, const WaveTop& t, Sums mine, int top) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mine.add({__shfl_xor(mine.r, o), __shfl_xor(mine.z, o), __shfl_xor(mine.e, o)});
+    if (lane == 0) {
+        s.sums[wave][0] = mine.r;
+        s.sums[wave][1] = mine.z;
+        s.sums[wave][2] = mine.e;
+    }
+    if constexpr (TOP) {
+        s.all[tid] = lane < top ? t.best : 0;
+        if (tid < kMostTop) s.list[tid] = 0;
+    }
+    __syncthreads();
+    Sums row;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) row.add({s.sums[w][0], s.sums[w][1], s.sums[w][2]});
+    if constexpr (TOP) {
+        if (lane < top && t.best != 0) {
+            int rank = 0;
+            for (int w = 0; w < kWaves; ++w) {
+                for (int i = 0; i < top; ++i) rank += s.all[64 * w + i] > t.best;
+            }
+            if (rank < top) s.list[rank] = t.best;
+        }
+        __syncthreads();
+    }
+    return row;
+}
+
+// A row's sums against its own largest logit, which it returns, differences first.  All threads call it.
+template <class T>
+__device__ __forceinline__ float sum_far(const LogprobParams& p, const typename T::storage* x, Sums& sums) {
+    __shared__ float parts[kWaves][2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float most = -INFINITY;
+    for (int64_t j = threadIdx.x; j < p.vocab; j += kThreads) most = __builtin_elementwise_maximum(most, T::load(x[j]));
+    for (int o = 1; o < 64; o <<= 1) most = __builtin_elementwise_maximum(most, __shfl_xor(most, o));
+    if (lane == 0) parts[wave][0] = most;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) most = __builtin_elementwise_maximum(most, parts[w][0]);
+    __syncthreads();
+    float z = 0.0f, e = 0.0f;
+    for (int64_t j = threadIdx.x; j < p.vocab; j += kThreads) {
+        const float d = fmaxf((T::load(x[j]) - most) * kLog2e, -200.0f), one = __builtin_amdgcn_exp2f(d);
+        z += one;
+        e = fmaf(one, d, e);
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+        z += __shfl_xor(z, o);
+        e += __shfl_xor(e, o);
+    }
+    if (lane == 0) {
+        parts[wave][0] = z;
+        parts[wave][1] = e;
+    }
+    __syncthreads();
+    sums.z = sums.e = 0.0f;
+    for (int w = 0; w < kWaves; ++w) {
+        sums.z += parts[w][0];
+        sums.e += parts[w][1];
+    }
+    if (!(most < INFINITY)) sums.z = NAN;
+    return most;
+}
+
+// What a row's sums and list say.  All threads call it; the list lies in LDS behind a barrier.
+template <class T, bool TOP>
+__device__ __forceinline__ void finish(const LogprobParams& p, int64_t i, int64_t row, Sums sums, const uint64_t* list) {
+    typedef typename T::storage S;
+    const S* x = reinterpret_cast<const S*>(p.logits) + row * p.stride;
+    double reference = static_cast<double>(sums.r) / static_cast<double>(kLog2e);
+    if (sums.r == kFarLow || sums.r == kFarHigh) reference = sum_far<T>(p, x, sums);
+    const double log_sum = static_cast<double>(log2f(sums.z)) / static_cast<double>(kLog2e);
+    // A sum over nothing but -inf has no distribution.
+    const bool none = !(sums.z > 0.0f);
+    if (threadIdx.x == 0) {
+        const float entropy = (log2f(sums.z) - sums.e / sums.z) / kLog2e;
+        p.entropy[i] = none ? NAN : entropy < 0.0f ? 0.0f : entropy;
+    }
+    for (int j = threadIdx.x; j < p.given; j += kThreads) {
+        const int64_t t = load_int(p.tokens, p.tokens64, i * p.given + j);
+        float value = t == -1 ? 0.0f : NAN;
+        if (t >= 0 && t < p.vocab) value = none ? NAN : static_cast<float>(static_cast<double>(T::load(x[t])) - reference - log_sum);
+        else if (t != -1) set_status(p.status, TV_STATUS_BAD_REQUEST);
+        p.logprobs[i * p.given + j] = value;
+    }
+    if constexpr (TOP) {
+        const int j = threadIdx.x;
+        if (j < p.top) {
+            const uint64_t entry = list[j];
+            p.top_ids[i * p.top + j] = static_cast<int64_t>(~static_cast<uint32_t>(entry));
+            const float value = value_of(static_cast<uint32_t>(entry >> 32));
+            p.top_logprobs[i * p.top + j] = none ? NAN : static_cast<float>(static_cast<double>(value) - reference - log_sum);
+        }
+    }
+}
+
+// The logits row of result row i; -1: none, and its results are written here.
+__device__ __forceinline__ int64_t find_row(const LogprobParams& p, int64_t i, bool write) {
+    const int64_t row = p.rows ? load_int(p.rows, p.rows64, i) : i;
+    if (row >= 0 && row < p.held) return row;
+    if (write) {
+        const float value = row == -1 ? 0.0f : NAN;
+        if (threadIdx.x == 0) {
+            p.entropy[i] = value;
+            if (row != -1) set_status(p.status, TV_STATUS_BAD_REQUEST);
+        }
+        for (int j = threadIdx.x; j < p.given; j += kThreads) p.logprobs[i * p.given + j] = value;
+        for (int j = threadIdx.x; j < p.top; j += kThreads) {
+            p.top_ids[i * p.top + j] = -1;
+            p.top_logprobs[i * p.top + j] = value;
+        }
+    }
+    return -1;
+}
+
+template <class T, bool TOP>
+__global__ void __launch_bounds__(kThreads)
+logprobs_kernel(const LogprobParams p) {
+    typedef typename T::storage S;
+    constexpr int VEC = 16 / sizeof(S);
+    __shared__ Joined joined;
+    __shared__ uint64_t queues[kWaves][TOP ? 64 * (VEC + 1) : 1];
+    const int64_t i = blockIdx.x / p.splits;
+    const int split = static_cast<int>(blockIdx.x - i * p.splits);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = find_row(p, i, p.splits == 1);
+    if (row < 0) return;
+    // A row has fewer than VEC elements before its first 16 bytes: those, the units, the rest.
+    const S* base = reinterpret_cast<const S*>(p.logits) + row * p.stride;
+    const uint32_t past = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base)) & 15u;
+    int64_t head = ((16u - past) & 15u) / sizeof(S);
+    head = head < p.vocab ? head : p.vocab;
+    const int64_t units = (p.vocab - head) / VEC;
+    const S* body = base + head;
+    const int64_t unit0 = units * split / p.splits, unit1 = units * (split + 1) / p.splits;
+
+    Sums sums;
+    float limit = -INFINITY;       // no logit seen passes it by much
+    WaveTop tops;
+    tops.queue = queues[wave];
+    tops.top = p.top;
+    uint32_t pass = 0;             // the order that a candidate has to pass
+    float bound = __uint_as_float(0x7fc00000u);   // its value; NaN: everything is one
+    // A lane's `count` elements x (the others -inf), the first of which has index `first`.
+    auto process = [&](const float (&x)[VEC], int64_t first, int count) {
+        float most = x[0];
+#pragma unroll
+        for (int e = 1; e < VEC; ++e) most = __builtin_elementwise_maximum(most, x[e]);   // NaN where one is
+        const bool raise = !(most <= limit), candidate = TOP && !(most <= bound);
+        if (__any(raise || candidate)) {
+            if (raise) {
+                if (!(most < INFINITY)) {
+                    sums.z = NAN;
+                    limit = INFINITY;
+                } else {
+                    sums.rescale(fabsf(most) < kFar ? most * kLog2e : most < 0.0f ? kFarLow : kFarHigh);
+                    limit = most + kMargin;
+                }
+            }
+            if constexpr (TOP) {
+                if (__any(candidate)) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) tops.push(e < count && order_of(x[e]) > pass, entry_of(x[e], first + e));
+                    while (tops.queued >= 64) tops.flush();
+                    // Elements to come have higher indices, so an equal value is not enough.
+                    const uint32_t kth = static_cast<uint32_t>(tops.kth >> 32);
+                    if (kth > pass) {
+                        pass = kth;
+                        bound = bound_of(kth);
+                    }
+                }
+            }
+        }
+        float z[VEC], z_e = 0.0f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float d = fmaxf(fmaf(x[e], kLog2e, -sums.r), -200.0f);
+            z[e] = __builtin_amdgcn_exp2f(d);
+            z_e = fmaf(z[e], d, z_e);
+        }
+#pragma unroll
+        for (int o = 1; o < VEC; o <<= 1) {
+#pragma unroll
+            for (int e = 0; e + o < VEC; e += 2 * o) z[e] += z[e + o];
+        }
+        sums.z += z[0];
+        sums.e += z_e;
+    };
+    auto lone = [&](int64_t index, bool live) {
+        float x[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = -INFINITY;
+        if (live) x[0] = T::load(base[index]);
+        process(x, index, live ? 1 : 0);
+    };
+    if (split == 0 && wave == 0 && head > 0) lone(lane < head ? lane : 0, lane < head);
+    bool begun = false;
+    for (int64_t u0 = unit0 + 64 * wave; u0 < unit1; u0 += 64 * kWaves * kUnroll) {
+        u32x4 raw[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            const int64_t u = u0 + 64 * kWaves * k + lane;
+            raw[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(body + (u < unit1 ? u : unit1 - 1) * VEC));
+        }
+        if (TOP && !begun) {
+            // The k-th largest of the lanes' maxima is at most the k-th largest element.
+            begun = true;
+            uint32_t most = 0;
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) {
+                S s[VEC];
+                __builtin_memcpy(s, &raw[k], 16);
+                const bool live = u0 + 64 * kWaves * k + lane < unit1;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) most = live ? max(most, order_of(T::load(s[e]))) : most;
+            }
+            const uint32_t kth = static_cast<uint32_t>(__shfl(static_cast<unsigned long long>(sorted(most)), p.top - 1));
+            if (kth > 0 && kth - 1 > pass) {
+                pass = kth - 1;
+                bound = bound_of(kth - 1);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            const int64_t u = u0 + 64 * kWaves * k + lane;
+            if (u - lane >= unit1) break;
+            if (u - lane + 64 > unit1 && u >= unit1) raw[k] = u32x4{T::kNone, T::kNone, T::kNone, T::kNone};
+            S s[VEC];
+            __builtin_memcpy(s, &raw[k], 16);
+            float x[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[e] = T::load(s[e]);
+            process(x, head + u * VEC, u < unit1 ? VEC : 0);
+        }
+    }
+    const int64_t rest = head + units * VEC;
+    if (split == p.splits - 1 && wave == kWaves - 1 && rest < p.vocab) {
+        lone(rest + lane < p.vocab ? rest + lane : rest, rest + lane < p.vocab);
+    }
+    if constexpr (TOP) tops.flush();
+    const Sums all = join<TOP>(joined, tops, sums, p.top);
+    if (p.splits == 1) {
+        finish<T, TOP>(p, i, row, all, joined.list);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        float* to = p.ws_sums + 4 * static_cast<int64_t>(blockIdx.x);
+        to[0] = all.r;
+        to[1] = all.z;
+        to[2] = all.e;
+    }
+    if constexpr (TOP) {
+        if (threadIdx.x < p.top) p.ws_top[static_cast<int64_t>(blockIdx.x) * p.top + threadIdx.x] = joined.list[threadIdx.x];
+    }
+}
+
+// Joins the parts of a row.
+template <class T, bool TOP>
+__global__ void __launch_bounds__(kThreads)
+logprobs_join_kernel(const LogprobParams p) {
+    __shared__ Joined joined;
+    __shared__ uint64_t queues[kWaves][TOP ? 128 : 1];
+    const int64_t i = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = find_row(p, i, true);
+    if (row < 0) return;
+    Sums sums;
+    for (int s = threadIdx.x; s < p.splits; s += kThreads) {
+        const float* from = p.ws_sums + 4 * (i * p.splits + s);
+        sums.add({from[0], from[1], from[2]});
+    }
+    WaveTop tops;
+    tops.queue = queues[wave];
+    tops.top = p.top;
+    if constexpr (TOP) {
+        const int entries = p.splits * p.top;
+        for (int at = 64 * wave; at < entries; at += kThreads) {
+            const uint64_t entry = at + lane < entries ? p.ws_top[i * entries + at + lane] : 0;
+            tops.push(entry > tops.kth, entry);
+            if (tops.queued >= 64) tops.flush();
+        }
+        tops.flush();
+    }
+    const Sums all = join<TOP>(joined, tops, sums, p.top);
+    finish<T, TOP>(p, i, row, all, joined.list);
+}
+
+// Parts of a row: the chip holds some 2048 of these workgroups; a part is at least 4 units a thread.
+int64_t splits_of(const tv_token_logprobs_args* a) {
+    const int64_t vec = a->dtype == TV_F32 ? 4 : 8;
+    const int64_t most = (a->vocab / vec + kThreads * kUnroll - 1) / (kThreads * kUnroll);
+    int64_t splits = (static_cast<int64_t>(a->compute_units) * 4 + a->num_rows - 1) / a->num_rows;
+    splits = splits < most ? splits : most;
+    return splits > 1 ? splits : 1;
+}
+
+template <class T, bool TOP>
+int enqueue(const LogprobParams& p, hipStream_t s) {
+    hipLaunchKernelGGL((logprobs_kernel<T, TOP>), dim3(static_cast<uint32_t>(p.num_rows * p.splits)), dim3(kThreads), 0, s, p);
+    const int launched = check_launch("token_logprobs");
+    if (launched != TV_OK || p.splits == 1) return launched;
+    hipLaunchKernelGGL((logprobs_join_kernel<T, TOP>), dim3(static_cast<uint32_t>(p.num_rows)), dim3(kThreads), 0, s, p);
+    return check_launch("token_logprobs join");
+}
+
+template <class T>
+int by_top(const LogprobParams& p, hipStream_t s) {
+    return p.top > 0 ? enqueue<T, true>(p, s) : enqueue<T, false>(p, s);
+}
+
+int check(const tv_token_logprobs_args* a) {
+    const char* what = "token_logprobs";
+    if (!a) return fail(TV_ERR_INVALID, "%s: null args", what);
+    if (a->num_rows < 0 || a->num_logits < 0 || a->vocab < 1 || a->logits_stride < a->vocab || a->tokens < 0 || a->compute_units < 1) {
+        return fail(TV_ERR_INVALID, "%s: invalid sizes", what);
+    }
+    if (a->dtype != TV_BF16 && a->dtype != TV_F16 && a->dtype != TV_F32) {
+        return fail(TV_ERR_UNSUPPORTED, "%s: logits must be bf16, f16 or fp32", what);
+    }
+    if (a->vocab > 0x7fffffff) return fail(TV_ERR_UNSUPPORTED, "%s: vocabularies of 2^31 words or more", what);
+    if (a->top < 0 || a->top > kMostTop || a->top > a->vocab) {
+        return fail(TV_ERR_INVALID, "%s: %d alternatives (at most 64, and the vocabulary)", what, a->top);
+    }
+    if (!a->rows && a->num_rows > a->num_logits) return fail(TV_ERR_INVALID, "%s: more results than logits rows", what);
+    // A launch has fewer than 2^32 threads.
+    if (a->num_rows > 0 && (a->num_rows > 0xffffff || a->num_rows * splits_of(a) > 0xffffff)) {
+        return fail(TV_ERR_UNSUPPORTED, "%s: too many rows", what);
+    }
+    return TV_OK;
+}
+
+}  // namespace
+}  // namespace tv
+
+using namespace tv;
+
+extern "C" int64_t tv_sizeof_token_logprobs_args(void) { return static_cast<int64_t>(sizeof(tv_token_logprobs_args)); }
+
+extern "C" int64_t tv_token_logprobs_workspace_bytes(const tv_token_logprobs_args* a) {
+    clear_error();
+    const int code = check(a);
+    if (code != TV_OK) return code;
+    if (a->num_rows == 0) return 0;
+    const int64_t splits = splits_of(a);
+    return splits == 1 ? 0 : a->num_rows * splits * (16 + 8ll * a->top);
+}
+
+extern "C" int tv_token_logprobs(const tv_token_logprobs_args* a, void* workspace, int64_t workspace_bytes, void* stream) {
+    clear_error();
+    const int code = check(a);
+    if (code != TV_OK) return code;
+    const char* what = "token_logprobs";
+    if (a->num_rows == 0) return TV_OK;
+    if ((!a->logits && a->num_logits > 0) || !a->entropy || (a->tokens > 0 && (!a->token_ids || !a->logprobs)) ||
+        (a->top > 0 && (!a->top_ids || !a->top_logprobs))) {
+        return fail(TV_ERR_INVALID, "%s: null pointer", what);
+    }
+    if (!aligned(a->logits, a->dtype == TV_F32 ? 4 : 2)) return fail(TV_ERR_INVALID, "%s: unaligned logits", what);
+    const int64_t splits = splits_of(a), bytes = splits == 1 ? 0 : a->num_rows * splits * (16 + 8ll * a->top);
+    if (bytes && (!workspace || !aligned(workspace, 16))) return fail(TV_ERR_INVALID, "%s: null or unaligned workspace", what);
+    if (workspace_bytes < bytes) {
+        return fail(TV_ERR_CAPACITY, "%s: workspace of %lld bytes, %lld needed", what, static_cast<long long>(workspace_bytes),
+                    static_cast<long long>(bytes));
+    }
+    LogprobParams p = {};
+    p.logits = static_cast<const char*>(a->logits);
+    p.stride = a->logits_stride;
+    p.held = a->num_logits;
+    p.vocab = a->vocab;
+    p.rows = a->rows;
+    p.rows64 = a->rows_is_int64 != 0;
+    p.tokens = a->token_ids;
+    p.tokens64 = a->tokens_is_int64 != 0;
+    p.num_rows = a->num_rows;
+    p.given = a->tokens;
+    p.top = a->top;
+    p.splits = static_cast<int32_t>(splits);
+    p.logprobs = a->logprobs;
+    p.entropy = a->entropy;
+    p.top_ids = a->top_ids;
+    p.top_logprobs = a->top_logprobs;
+    if (bytes) {
+        p.ws_sums = static_cast<float*>(workspace);
+        p.ws_top = reinterpret_cast<uint64_t*>(p.ws_sums + 4 * a->num_rows * splits);
+    }
+    p.status = a->status;
+    const hipStream_t s = as_stream(stream);
+    if (a->dtype == TV_BF16) return by_top<LogBf16>(p, s);
+    if (a->dtype == TV_F16) return by_top<LogF16>(p, s);
+    return by_top<LogF32>(p, s);
+}

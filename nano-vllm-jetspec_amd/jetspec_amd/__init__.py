@@ -12,6 +12,9 @@ Operators around them that the reference leaves to eager tensors or the host:
   build_block_tables, packed_slot_maps     page tables and slot maps from request lengths
   qk_norm_rope_scatter(_prevalidated)      per-head Q/K norm with the rotation and scatter
   store_kvcache_e4m3, packed_tree_attention_e4m3   an 8-bit cache: its append and its attention
+  rotary_scatter(_prevalidated), rotary_frequencies   other pair layouts, part of a head, scaled frequencies
+  packed_window_attention                  a sliding window with first tokens that stay visible
+  token_logprobs                           log probabilities, entropy and top alternatives of logits rows
 Each device operator is a hand-written gfx950 HIP kernel in libtreeverify.so.
 """
 from .packed_metadata import PackedTreeMetadata
@@ -29,6 +32,9 @@ from .attention import store_kvcache
 from .tree_fusion import rope_scatter, rope_scatter_prevalidated
 from .qk_norm import qk_norm_rope_scatter, qk_norm_rope_scatter_prevalidated
 from .cache_e4m3 import packed_tree_attention_e4m3, store_kvcache_e4m3
+from .rotary import rotary_frequencies, rotary_scatter, rotary_scatter_prevalidated
+from .window_attention import packed_window_attention
+from .logprobs import token_logprobs
 from .block_tables import build_block_tables, packed_slot_maps
 from .prefill import chain_tree_masks, offset_causal_mask
 from .state import commit_slots, copy_accepted_kv, _slots_for_blocks
@@ -56,6 +62,11 @@ __all__ = [
     "qk_norm_rope_scatter_prevalidated",
     "store_kvcache_e4m3",
     "packed_tree_attention_e4m3",
+    "rotary_frequencies",
+    "rotary_scatter",
+    "rotary_scatter_prevalidated",
+    "packed_window_attention",
+    "token_logprobs",
     "build_block_tables",
     "packed_slot_maps",
     "offset_causal_mask",

@@ -80,6 +80,14 @@ EXPORTED_SYMBOLS = (
     "tv_sizeof_tree_attention_e4m3_args",
     "tv_tree_attention_e4m3_workspace_bytes",
     "tv_tree_attention_e4m3",
+    "tv_sizeof_window_attention_args",
+    "tv_window_attention_workspace_bytes",
+    "tv_window_attention",
+    "tv_sizeof_rotary_args",
+    "tv_rotary_scatter",
+    "tv_sizeof_token_logprobs_args",
+    "tv_token_logprobs_workspace_bytes",
+    "tv_token_logprobs",
 )
 
 
@@ -239,6 +247,39 @@ class TreeAttentionE4m3Args(ctypes.Structure):
     ]
 
 
+class WindowAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_row", c_int64), ("q_stride_head", c_int64), ("in_dtype", c_int32),
+        ("k_pool", c_void_p), ("v_pool", c_void_p), ("k_stride", c_int64 * 4), ("v_stride", c_int64 * 4),
+        ("num_blocks", c_int64),
+        ("out", c_void_p), ("out_stride_row", c_int64), ("out_stride_head", c_int64), ("out_dtype", c_int32),
+        ("cu_seqlens_q", c_void_p), ("prefix_lens", c_void_p), ("node_counts", c_void_p),
+        ("block_tables", c_void_p), ("block_table_stride", c_int64), ("block_table_width", c_int32),
+        ("tree_slots", c_void_p), ("qq_bias", c_void_p), ("qq_bias_offsets", c_void_p), ("qq_bias_elems", c_int64),
+        ("positions", c_void_p), ("positions_is_int64", c_int32), ("window", c_int32), ("sinks", c_int32),
+        ("num_requests", c_int32), ("total_queries", c_int32), ("num_q_heads", c_int32), ("num_kv_heads", c_int32),
+        ("head_dim", c_int32), ("block_size", c_int32),
+        ("scale", c_float), ("compute_units", c_int32), ("status", c_void_p),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("rope", RopeScatterArgs),
+        ("frequencies", c_void_p), ("num_frequencies", c_int32), ("interleaved", c_int32), ("gain", c_float),
+    ]
+
+
+class TokenLogprobsArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p), ("logits_stride", c_int64), ("num_logits", c_int64), ("vocab", c_int64), ("dtype", c_int32),
+        ("rows", c_void_p), ("rows_is_int64", c_int32), ("token_ids", c_void_p), ("tokens_is_int64", c_int32),
+        ("num_rows", c_int64), ("tokens", c_int32), ("top", c_int32),
+        ("logprobs", c_void_p), ("entropy", c_void_p), ("top_ids", c_void_p), ("top_logprobs", c_void_p),
+        ("compute_units", c_int32), ("status", c_void_p),
+    ]
+
+
 def _fields_format(structure, base: int = 0) -> list[tuple[int, str, int]]:
     """(offset, struct code, size) of every scalar of a structure, nested ones and arrays laid out flat."""
     codes = {c_void_p: "P", c_int64: "q", c_int32: "i", c_float: "f"}
@@ -268,6 +309,9 @@ def packer(structure):
 pack_qk_norm = packer(QkNormArgs)
 pack_store_e4m3 = packer(StoreE4m3Args)
 pack_tree_attention_e4m3 = packer(TreeAttentionE4m3Args)
+pack_window_attention = packer(WindowAttentionArgs)
+pack_rotary = packer(RotaryArgs)
+pack_token_logprobs = packer(TokenLogprobsArgs)
 
 _lock = threading.Lock()
 _lib = None
@@ -372,6 +416,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.tv_tree_attention_e4m3_workspace_bytes.argtypes = [c_void_p]   # packed bytes or a structure by reference
     lib.tv_tree_attention_e4m3.restype = c_int32
     lib.tv_tree_attention_e4m3.argtypes = [c_void_p, c_void_p, c_int64, c_void_p]
+    # Packed bytes or a structure by reference.
+    for name in ("window_attention", "token_logprobs"):
+        size, space, entry = (getattr(lib, f) for f in (f"tv_sizeof_{name}_args", f"tv_{name}_workspace_bytes", f"tv_{name}"))
+        size.restype, size.argtypes = c_int64, []
+        space.restype, space.argtypes = c_int64, [c_void_p]
+        entry.restype, entry.argtypes = c_int32, [c_void_p, c_void_p, c_int64, c_void_p]
+    lib.tv_sizeof_rotary_args.restype = c_int64
+    lib.tv_sizeof_rotary_args.argtypes = []
+    lib.tv_rotary_scatter.restype = c_int32
+    lib.tv_rotary_scatter.argtypes = [c_void_p, c_void_p]
     lib.tv_build_block_tables.restype = c_int32
     lib.tv_build_block_tables.argtypes = [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
                                           *[c_int32] * 4, *[c_void_p] * 5]
@@ -413,6 +467,10 @@ def library() -> ctypes.CDLL:
             raise RuntimeError("tv_store_e4m3_args layout differs between library and binding")
         if lib.tv_sizeof_tree_attention_e4m3_args() != ctypes.sizeof(TreeAttentionE4m3Args):
             raise RuntimeError("tv_tree_attention_e4m3_args layout differs between library and binding")
+        for name, structure in (("window_attention", WindowAttentionArgs), ("rotary", RotaryArgs),
+                                ("token_logprobs", TokenLogprobsArgs)):
+            if getattr(lib, f"tv_sizeof_{name}_args")() != ctypes.sizeof(structure):
+                raise RuntimeError(f"tv_{name}_args layout differs between library and binding")
         _lib = lib
         return lib
 
