@@ -31,11 +31,12 @@ GROUPS_D256 = (1, 2, 4, 8, 16)
 ATTENTION_GROUP_SOURCES = (tuple(f"tv_attention_g{g}.hip" for g in GROUPS) +
                            tuple(f"tv_attention_d64_g{g}.hip" for g in GROUPS_D64) +
                            tuple(f"tv_attention_d256_g{g}.hip" for g in GROUPS_D256))
+WINDOW_SOURCES = ("tv_window_d64.hip", "tv_window_d128.hip", "tv_window_d256.hip")
 SOURCES = ("tv_common.cpp", "tv_plan.cpp", "tv_kvcache.hip", "tv_attention.hip", *ATTENTION_GROUP_SOURCES,
            "tv_attention_fp32.hip", "tv_attention_rows.hip",
            "tv_attention_e4m3.hip", "tv_attention_e4m3_d64.hip", "tv_attention_e4m3_d128.hip",
            "tv_attention_e4m3_d256.hip",
-           "tv_window.hip", "tv_window_d64.hip", "tv_window_d128.hip", "tv_window_d256.hip",
+           "tv_window.hip", *WINDOW_SOURCES,
            "tv_rope.hip", "tv_qk_norm.hip", "tv_rotary.hip", "tv_slots.hip", "tv_accept.hip",
            "tv_logprobs.hip", "tv_metadata.hip", "tv_plan_device.hip")
 
@@ -96,16 +97,16 @@ def _check_m0(source: str, tmp: Path) -> None:
 
 
 def check_m0_discipline(verbose: bool = False, jobs: int | None = None) -> None:
-    """The attention kernel issues its global->LDS DMA from inline asm that sets M0.
+    """The attention kernels issue their global->LDS DMA from inline asm that sets M0.
 
-    That is only sound while no compiler-generated instruction of the kernel uses M0,
-    so compile each translation unit holding an instance of the kernel to assembly and
+    That is only sound while no compiler-generated instruction of the kernels uses M0,
+    so compile each translation unit holding an instance of them to assembly and
     require every M0 reference to be one of those `s_mov_b32 m0, sN` writes.
     """
     import tempfile
 
     with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(jobs or _jobs()) as pool:
-        list(pool.map(lambda src: _check_m0(src, Path(tmp)), ATTENTION_GROUP_SOURCES))
+        list(pool.map(lambda src: _check_m0(src, Path(tmp)), (*ATTENTION_GROUP_SOURCES, *WINDOW_SOURCES)))
     if verbose:
         print("M0 discipline ok", flush=True)
 

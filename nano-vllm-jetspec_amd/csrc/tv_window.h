@@ -13,9 +13,10 @@
 // this order, are its work, in steps of SK.  Pages outside are never looked up.
 //
 // A workgroup takes one row block (ROWS score rows of one request and KV head), or an equal part of its
-// steps where the batch has too few blocks for the chip; a second launch joins the parts.  The request of
-// a block is found from the live lengths: its blocks have the numbers from cu[r] * G / ROWS + r on, of
-// which there are always enough, so a search in cu finds it and no plan or scan is needed.
+// steps where the batch has too few blocks for the chip; a second launch joins the parts.  Every workgroup
+// finds its block from the live lengths by a sum over the requests' blocks, so no plan is needed; blocks that
+// are not there come last in the launch, since they are what balances it when they lie between others
+// (every second one missing kept half of the shader engines idle: 1302 us for 652).
 //
 // A step: every wave moves its share of the keys from memory to registers one step ahead (page numbers
 // and slots two ahead) and from there to LDS, K and V as [key][dim] with the 16-byte chunks swizzled per
@@ -33,6 +34,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "tv_internal.h"
 
 namespace tv {
@@ -42,9 +45,11 @@ struct WindowParams {
     int64_t q_s0, q_s1;
     const char* k;
     const char* v;
-    int64_t k_s0, k_s1, k_s2, v_s0, v_s1, v_s2;   // page, slot and head strides in bytes
+    uint32_t k_s0, k_s1, v_s0, v_s1;              // page and slot strides in bytes
+    int64_t k_s2, v_s2;                           // head strides
     int32_t num_blocks, block_size;
     uint32_t div_mul, div_shift;                  // pos / block_size by multiplication (win_page_of)
+    int32_t same;                                 // K and V have the same page and slot strides
     void* out;
     int64_t o_s0, o_s1;
     int32_t out_f32;
@@ -66,6 +71,7 @@ struct WindowParams {
     float c;                       // scale * log2(e)
     int32_t block_ids;             // numbers that row blocks can have
     int32_t splits;                // workgroups a row block
+    int32_t row_slots;             // the merge gives a row a group of lanes, not a workgroup
     float* ws_o;
     float2* ws_ml;
     int32_t* status;
@@ -93,6 +99,7 @@ typedef _Float16 win_f16x8 __attribute__((ext_vector_type(8)));
 typedef float win_f32x16 __attribute__((ext_vector_type(16)));
 typedef float win_f32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t win_i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t win_u32x4u __attribute__((ext_vector_type(4), aligned(4)));   // at any element
 typedef short win_i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) win_i16x4 win_lds_i16x4;
 
@@ -132,29 +139,85 @@ __device__ __forceinline__ WinRequest win_request(const WindowParams& p, int r, 
     return q;
 }
 
-// The request that block number `id` belongs to (the last whose numbers begin at or below it), by a search
-// of 64 places at a time; whether it has such a block, the caller asks.
-template <int ROWS>
-__device__ __forceinline__ int win_first_id(const WindowParams& p, int r) {
-    const int64_t rows = static_cast<int64_t>(p.cu[r]) * p.groups;
-    const int64_t id = (rows < 0 ? 0 : rows / ROWS) + r;
-    return id < 0x7fffffff ? static_cast<int>(id) : 0x7fffffff;
-}
+// A row block: its request, and its place among the request's blocks.
+struct WinBlock {
+    int32_t r, b;
+    WinRequest req;
+};
 
-template <int ROWS>
-__device__ __forceinline__ int win_find(const WindowParams& p, int id) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, n = p.num_requests;
-    while (n > 1) {
-        const int step = (n + 63) / 64;
-        const int64_t at = static_cast<int64_t>(lane) * step;
-        const bool below = at < n && win_first_id<ROWS>(p, lo + static_cast<int>(at < n ? at : 0)) <= id;
-        const int found = __popcll(__ballot(below));
-        const int skip = (found > 0 ? found - 1 : 0) * step;
-        lo += skip;
-        n = n - skip < step ? n - skip : step;
+// Finds row block `id` of the batch, blocks of a request and requests following each other; false if there are
+// not so many.  All threads of the workgroup call it; `scratch` is LDS of its own, 3 + a word a wave.
+template <int ROWS, int THREADS>
+__device__ __forceinline__ bool win_find(const WindowParams& p, int id, int32_t* scratch, WinBlock& block) {
+    constexpr int WAVES = THREADS / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // The last workgroup of a launch reports what is wrong with the requests.
+    const bool report = blockIdx.x + 1 == gridDim.x;
+    bool bad;
+    if (p.num_requests <= 64) {
+        // A lane per request, in every wave by itself.
+        WinRequest q = {};
+        if (lane < p.num_requests) {
+            q = win_request<ROWS>(p, lane, bad);
+            if (bad && report) set_status(p.status, TV_STATUS_BAD_REQUEST);
+        }
+        int32_t end = q.blocks;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int32_t y = __shfl_up(end, o);
+            if (lane >= o) end += y;
+        }
+        const uint64_t behind = __ballot(end > id);
+        if (!behind) return false;
+        const int r = __ffsll(static_cast<unsigned long long>(behind)) - 1;
+        block.r = r;
+        block.b = id - __builtin_amdgcn_readlane(end - q.blocks, r);
+        block.req.prefix = __builtin_amdgcn_readlane(q.prefix, r);
+        block.req.nodes = __builtin_amdgcn_readlane(q.nodes, r);
+        block.req.first_row = __builtin_amdgcn_readlane(q.first_row, r);
+        block.req.blocks = __builtin_amdgcn_readlane(q.blocks, r);
+        block.req.bias = static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int32_t>(q.bias >> 32), r)) << 32 |
+                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int32_t>(q.bias), r));
+        return true;
     }
-    return __builtin_amdgcn_readfirstlane(lo);
+    const int per = (p.num_requests + THREADS - 1) / THREADS;
+    const int r0 = tid * per, r1 = r0 + per < p.num_requests ? r0 + per : p.num_requests;
+    int32_t mine = 0;   // the sum is at most block_ids
+    for (int i = r0; i < r1; ++i) {
+        mine += win_request<ROWS>(p, i, bad).blocks;
+        if (bad && report) set_status(p.status, TV_STATUS_BAD_REQUEST);
+    }
+    int32_t end = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int32_t y = __shfl_up(end, o);
+        if (lane >= o) end += y;
+    }
+    if (lane == 63) scratch[3 + wave] = end;
+    if (tid == 0) scratch[0] = -1;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) end += scratch[3 + w];
+    }
+    if (end - mine <= id && id < end) {   // this thread's requests hold it
+        int32_t first = end - mine;
+        for (int i = r0; i < r1; ++i) {
+            const int32_t next = first + win_request<ROWS>(p, i, bad).blocks;
+            if (id < next) {
+                scratch[0] = i;
+                scratch[1] = id - first;
+                break;
+            }
+            first = next;
+        }
+    }
+    __syncthreads();
+    block.r = __builtin_amdgcn_readfirstlane(scratch[0]);
+    block.b = __builtin_amdgcn_readfirstlane(scratch[1]);
+    if (block.r < 0) return false;
+    block.req = win_request<ROWS>(p, block.r, bad);
+    return true;
 }
 
 // A node's position: the prefix length plus a depth that its index bounds.
@@ -170,6 +233,11 @@ struct WinType<__bf16> {
     typedef win_bf16x8 vec;
     static constexpr uint32_t kExponent = 0x7f807f80u, kStep = 0x00800080u;
     static constexpr float kShift = 0.0f;
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ float add_pair(__bf16 a, __bf16 b, float sum) {
+        const pair x = {a, b}, one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+        return __builtin_amdgcn_fdot2_f32_bf16(x, one, sum, false);
+    }
     static __device__ __forceinline__ win_f32x16 run(vec a, vec b, win_f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
@@ -179,6 +247,11 @@ struct WinType<_Float16> {
     typedef win_f16x8 vec;
     static constexpr uint32_t kExponent = 0x7c007c00u, kStep = 0x04000400u;
     static constexpr float kShift = 7.0f;
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ float add_pair(_Float16 a, _Float16 b, float sum) {
+        const pair x = {a, b}, one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+        return __builtin_amdgcn_fdot2(x, one, sum, false);
+    }
     static __device__ __forceinline__ win_f32x16 run(vec a, vec b, win_f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
@@ -212,6 +285,43 @@ __device__ __forceinline__ float win_weight(float2 ml, float best) {
     return ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - best);
 }
 
+// f(0), f(1), ... with the numbers as types.
+template <int FROM, int TO, class F>
+__device__ __forceinline__ void win_each(F& f) {
+    if constexpr (FROM < TO) {
+        f(std::integral_constant<int, FROM>());
+        win_each<FROM + 1, TO>(f);
+    }
+}
+
+constexpr int kAhead = 4;      // products between an operand's read and its use
+constexpr int kWinTable = 512; // keys of a table
+
+// s_waitcnt immediates: vector memory operations down to n with nothing else, LDS operations down to none.
+template <int N>
+__device__ __forceinline__ void win_wait_loads() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+}
+// A workgroup barrier behind the wave's own LDS operations that leaves its loads under way.
+__device__ __forceinline__ void win_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// 16 bytes a lane from memory to LDS at `lds_addr` + 16 * lane.  Issued from inline asm so that the compiler does not
+// wait for it before every later LDS read; win_wait_loads and a barrier order it.  M0 has no other use in these
+// kernels, which build.py checks in their assembly.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void win_dma(const void* src, uint32_t lds_addr) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(lds_addr), "v"(src)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // Writes four consecutive output dims of a row.
 template <class T>
 __device__ __forceinline__ void win_store4(const WindowParams& p, int64_t row, int head, int dim, win_f32x4 v) {
@@ -238,16 +348,20 @@ window_attention_kernel(const WindowParams p) {
     constexpr int NK = D / 16, NB = D / 32;        // MFMAs of a tile's scores; output blocks
     constexpr float kShift = WinType<T>::kShift;
     const float kOver = __builtin_amdgcn_exp2f(8.0f + kShift);
-    static_assert(PASSES <= LPR, "a lane of its row for each pass's reach");
+    constexpr int AHEAD = WK == 1 ? 3 : NBUF;      // steps between a step's loads and its products
+    constexpr int TSTEPS = kWinTable / SK;         // steps of a table
     static_assert(SK % KPP == 0 && SK % (kWinTile * WK) == 0, "a step is whole passes and tiles");
-    static_assert(KPP % 16 == 0 || (KPP % 4 == 0 && D != 64), "the swizzle's period");
+    static_assert(TSTEPS > AHEAD, "a table is read no longer when the next but one is made");
     static_assert(WK == 1 || WK * 32 * D * 4 <= NBUF * 2 * KB, "the waves' results share the staging memory");
     typedef typename WinType<T>::vec V8;
 
     __shared__ __attribute__((aligned(1024))) char lds[NBUF * 2 * KB];
-    __shared__ __attribute__((aligned(16))) int32_t lds_reach[NBUF][SK];
+    // Of the keys of two tables: page and place in it, and the last position that sees the key, -1 if it is not there.
+    __shared__ __attribute__((aligned(16))) u32x2 tab_at[2][kWinTable];
+    __shared__ __attribute__((aligned(16))) int32_t tab_reach[2][kWinTable];
+    __shared__ __attribute__((aligned(4))) uint8_t tab_clear[2][kWinTable / kWinTile];   // every row sees the whole tile
     __shared__ float2 lds_ml[WM * WK][32];
-    __shared__ int lds_bad[NBUF];
+    __shared__ int32_t lds_find[3 + THREADS / 64];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -257,19 +371,10 @@ window_attention_kernel(const WindowParams p) {
     // --- the row block and its keys -------------------------------------------------------------
     const int unit = blockIdx.x / p.num_kv_heads, head = blockIdx.x - unit * p.num_kv_heads;
     const int id = unit / p.splits, split = unit - id * p.splits;
-    const int r = win_find<ROWS>(p, id);
-    bool bad_request;
-    const WinRequest req = win_request<ROWS>(p, r, bad_request);
-    const int b = id - win_first_id<ROWS>(p, r);
-    // The last number mostly names no block: its workgroup looks over all requests.
-    if (blockIdx.x + 1 == gridDim.x) {
-        for (int i = tid; i < p.num_requests; i += THREADS) {
-            bool bad;
-            win_request<ROWS>(p, i, bad);
-            if (bad) set_status(p.status, TV_STATUS_BAD_REQUEST);
-        }
-    }
-    if (b < 0 || b >= req.blocks) return;
+    WinBlock block;
+    if (!win_find<ROWS, THREADS>(p, id, lds_find, block)) return;
+    const int r = block.r, b = block.b;
+    const WinRequest req = block.req;
     const int rows_all = req.nodes * p.groups;
     const int node0 = b * ROWS / p.groups;
     const int node1 = (b * ROWS + ROWS < rows_all ? b * ROWS + ROWS - 1 : rows_all - 1) / p.groups;   // the last
@@ -311,110 +416,121 @@ window_attention_kernel(const WindowParams p) {
     const char* k_head = p.k + head * p.k_s2;
     const char* v_head = p.v + head * p.v_s2;
 
-    // The position of the v-th key of the prefix part.
-    auto position_of = [&](int v) { return v < n_first ? v : v - n_first + w0; };
-    // Keys [v, v + n) are all there, in the prefix, and seen by every row.
-    auto clear_run = [&](int v, int n) {
-        return v + n <= n_prefix && (v + n <= n_first || (v >= n_first && v - n_first + w0 >= from_high));
+    // Parameters that the steps do not need are read where they are used: held over the loop, with the others,
+    // they would not fit the scalar registers.
+    typedef const __attribute__((address_space(4))) WindowParams* Params;
+    auto cold = [&]() {
+        Params a = (Params)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(a));
+        return a;
     };
 
-    // --- moving a step's keys -------------------------------------------------------------------
-    const int my_key = tid / LPR, my_chunk = tid % LPR;
-    const bool my_dims = my_chunk * 8 < p.dim;
-    int32_t entry[PASSES], entry_high[PASSES];   // page numbers, or tree slots in two halves
-    u32x4 kreg[PASSES], vreg[PASSES];
-    int32_t node_at = 0;            // position of the tree key of pass my_chunk
-    uint32_t good = 0, wrong = 0;   // passes whose key is live and found / live and not found
+    // --- the tables: keys [run0 * SK + t * kWinTable, ...), a thread a key -------------------------
+    auto make_table = [&](int t) {
+        const Params a = cold();
+#pragma unroll 1
+        for (int kk = tid; kk < kWinTable; kk += THREADS) {
+            const int v = run0 * SK + t * kWinTable + kk;
+            const bool live = v < n_keys, tree = v >= n_prefix;
+            const int of = live ? v : n_keys - 1, t_of = of - n_prefix + t0;   // a key that is there
+            const int32_t pos = of < n_first ? of : of - n_first + w0;
+            const bool slot = of >= n_prefix;
+            int32_t page = win_page_of(a->div_mul, a->div_shift, slot ? 0 : pos);
+            const int32_t* from = slot ? reinterpret_cast<const int32_t*>(slots + t_of) : table + page;
+            const int32_t entry = from[0], entry_high = from[slot ? 1 : 0];
+            const int32_t given = positions[static_cast<int64_t>(slot ? t_of : 0) * a->pos_step];
+            uint32_t offset = static_cast<uint32_t>(pos - page * a->block_size);
+            if (slot) {
+                page = win_page_of(a->div_mul, a->div_shift, entry < 0 ? 0 : entry);
+                offset = static_cast<uint32_t>(entry - page * a->block_size);
+                if (entry < 0 || entry_high != 0) page = -1;
+            } else {
+                page = entry;
+            }
+            const bool there = page >= 0 && page < a->num_blocks, found = live && there;
+            if (live && !there) set_status(a->status, TV_STATUS_BAD_PAGE);
+            // Every lane loads: a key that is not there from the pool's first row.
+            tab_at[t & 1][kk] = found ? u32x2{static_cast<uint32_t>(page), offset} : u32x2{0, 0};
+            const int32_t at = tree ? win_position(req, t_of, given) : pos;
+            const int64_t until = at < a->sinks ? 0x7fffffff : static_cast<int64_t>(at) + a->window - 1;
+            tab_reach[t & 1][kk] = !found ? -1 : until < 0x7fffffff ? static_cast<int32_t>(until) : 0x7fffffff;
+            const uint64_t clear = __ballot(found && !tree && (pos < a->sinks || pos >= from_high));
+            if ((lane & 31) == 0) tab_clear[t & 1][kk / kWinTile] = static_cast<uint32_t>(clear >> lane) == 0xffffffffu;
+        }
+    };
+    // The tiles of step j that need no mask, a byte a tile.
+    auto clear_tiles = [&](int j) {
+        const uint8_t* at = &tab_clear[j / TSTEPS & 1][j % TSTEPS * (SK / kWinTile)];
+        uint32_t flags;
+        if constexpr (SK / kWinTile == 1) flags = *at;
+        else if constexpr (SK / kWinTile == 2) flags = *reinterpret_cast<const uint16_t*>(at);
+        else flags = *reinterpret_cast<const uint32_t*>(at);
+        return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(flags));
+    };
+    constexpr uint32_t kAllClear = SK / kWinTile == 1 ? 1u : SK / kWinTile == 2 ? 0x0101u : 0x01010101u;
 
-    const int k_put = my_key * 2 * D + 16 * win_k_chunk<D>(my_key, my_chunk);
-    const int v_put = my_key * 2 * D + 16 * win_v_chunk<D>(my_key, my_chunk);
+    // --- moving a step's keys -------------------------------------------------------------------
+    // Lane l of a load fills place l % LPR of a row, which holds the chunk that the swizzle puts there.
+    const int my_key = tid / LPR, my_place = tid % LPR;
+    const uint32_t lds_base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds))) + wave * (64 / LPR) * 2 * D;
+    auto k_chunk = [&](int n) { return win_k_chunk<D>(my_key + n * KPP, my_place); };
+    auto v_chunk = [&](int n) { return win_v_chunk<D>(my_key + n * KPP, my_place); };
+    auto issue = [&](int j) {
+        const uint32_t to = lds_base + j % NBUF * (2 * KB);
+        const u32x2* at = &tab_at[j / TSTEPS & 1][j % TSTEPS * SK + my_key];
+#pragma unroll
+        for (int n = 0; n < PASSES; ++n) {
+            const u32x2 e = at[n * KPP];
+            int kc = k_chunk(n), vc = v_chunk(n);
+            if (p.dim != D) {   // places behind the head's end: the first chunk, which mend() drops
+                kc = kc * 8 < p.dim ? kc : 0;
+                vc = vc * 8 < p.dim ? vc : 0;
+            }
+            const uint64_t row = static_cast<uint64_t>(e[0]) * p.k_s0 + static_cast<uint64_t>(e[1]) * p.k_s1;
+            uint64_t v_row = row;
+            if (!p.same) {
+                const Params a = cold();
+                v_row = static_cast<uint64_t>(e[0]) * a->v_s0 + static_cast<uint64_t>(e[1]) * a->v_s1;
+            }
+            win_dma(k_head + row + 16 * kc, to + n * KPP * 2 * D);
+            win_dma(v_head + v_row + 16 * vc, to + KB + n * KPP * 2 * D);
+        }
+    };
+    // Rows that do not see a key have to get zero from its V row, and zero times NaN or infinity is not.  So where a
+    // step's tiles are not all clear, each thread, behind its own loads, makes zeros of such elements, and the key's
+    // scores NaN instead, which hidden scores never show.  It also clears what lies behind a head's end.
+    auto mend = [&](int j) {
+        const bool whole = p.dim == D;
+        if (clear_tiles(j) == kAllClear && whole) return;
+        char* kb = lds + j % NBUF * (2 * KB) + my_key * 2 * D + 16 * my_place;
+        char* vb = kb + KB;
+#pragma unroll
+        for (int n = 0; n < PASSES; ++n) {
+            const int at = n * KPP * 2 * D;
+            u32x4 x = *reinterpret_cast<const u32x4*>(vb + at);
+            uint32_t odd = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) odd |= ((x[w] & WinType<T>::kExponent) + WinType<T>::kStep) & 0x80008000u;
+            const bool behind = !whole && v_chunk(n) * 8 >= p.dim;
+            const uint64_t lanes = __ballot(odd != 0 && !behind);
+            if (odd != 0 || behind) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t high = ((x[w] & WinType<T>::kExponent) + WinType<T>::kStep) & 0x80008000u;
+                    x[w] = behind ? 0 : x[w] & ~((high >> 15) * 0xffffu);
+                }
+                *reinterpret_cast<u32x4*>(vb + at) = x;
+            }
+            const bool poison = (lanes >> (lane & ~(LPR - 1))) & ((1ull << LPR) - 1);
+            if (poison || (!whole && k_chunk(n) * 8 >= p.dim)) {
+                const uint32_t word = poison ? 0x7fff7fffu : 0;
+                *reinterpret_cast<u32x4*>(kb + at) = u32x4{word, word, word, word};
+            }
+        }
+    };
     const int k_get = c * 2 * D + 16 * win_k_chunk<D>(c, half);
     const int v_key = 4 * half + ((lane & 15) >> 2), v_dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     const int v_get = v_key * 2 * D + 16 * win_v_chunk<D>(v_key, v_dim >> 3) + 2 * (v_dim & 7);
-
-    // Loads the page numbers (tree slots: both halves) of a step; nothing looks at them before fetch_keys().
-    auto fetch_entries = [&](int i) {
-#pragma unroll
-        for (int n = 0; n < PASSES; ++n) {
-            const int v = i * SK + n * KPP + my_key, of = v < n_keys ? v : n_keys - 1;
-            const bool tree = of >= n_prefix;
-            const int32_t* from = tree ? reinterpret_cast<const int32_t*>(slots + (of - n_prefix + t0))
-                                       : table + win_page_of(p.div_mul, p.div_shift, position_of(of));
-            entry[n] = from[0];
-            entry_high[n] = from[tree ? 1 : 0];
-        }
-    };
-    constexpr uint32_t kAll = (1u << PASSES) - 1;
-    auto fetch_keys = [&](int i) {
-        good = wrong = 0;
-        int64_t k_of[PASSES], v_of[PASSES];
-        int of_mine = 0;
-#pragma unroll
-        for (int n = 0; n < PASSES; ++n) {
-            const int v = i * SK + n * KPP + my_key;
-            const bool live = v < n_keys, tree = v >= n_prefix;
-            const int32_t pos = tree ? entry[n] : position_of(v);   // a slot or a position
-            const int32_t quotient = win_page_of(p.div_mul, p.div_shift, pos < 0 ? 0 : pos);
-            const int32_t page = !tree ? entry[n] : entry[n] < 0 || entry_high[n] != 0 ? -1 : quotient;
-            const bool found = live && page >= 0 && page < p.num_blocks;
-            if (found) good |= 1u << n;
-            if (live && !found) wrong |= 1u << n;
-            // Every lane loads, one whose key is past the end or not found from the pool's first row.
-            const int64_t at = found ? page : 0, offset = found ? pos - quotient * p.block_size : 0;
-            const int64_t chunk = my_dims ? 16 * my_chunk : 0;
-            k_of[n] = at * p.k_s0 + offset * p.k_s1 + chunk;
-            v_of[n] = at * p.v_s0 + offset * p.v_s1 + chunk;
-            if (my_chunk == n && live && tree) of_mine = v - n_prefix + t0;
-        }
-#pragma unroll
-        for (int n = 0; n < PASSES; ++n) {
-            kreg[n] = *reinterpret_cast<const u32x4*>(k_head + k_of[n]);
-            vreg[n] = *reinterpret_cast<const u32x4*>(v_head + v_of[n]);
-        }
-        if ((i + 1) * SK > n_prefix) node_at = positions[static_cast<int64_t>(of_mine) * p.pos_step];
-    };
-    auto stage = [&](int step, int buf, int mark) {
-        char* kb = lds + buf * 2 * KB;
-        char* vb = kb + KB;
-        const bool clear = clear_run(step * SK, SK) && p.dim == D;
-        if (!clear || __any(good != kAll)) {
-#pragma unroll
-            for (int i = 0; i < PASSES; ++i) {
-                const uint32_t keep = my_dims && ((good >> i) & 1) ? 0xffffffffu : 0u;
-                kreg[i] &= keep;
-                vreg[i] &= keep;
-                // Rows that do not see a key have to get zero from its V row, and zero times NaN or infinity is
-                // not.  So such elements become zeros, and the key's scores NaN instead, which hidden scores never show.
-                uint32_t odd = 0;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t high = ((vreg[i][w] & WinType<T>::kExponent) + WinType<T>::kStep) & 0x80008000u;
-                    vreg[i][w] &= ~((high >> 15) * 0xffffu);
-                    odd |= high;
-                }
-                const uint64_t lanes = __ballot(odd != 0);
-                if ((lanes >> (lane & ~(LPR - 1))) & ((1ull << LPR) - 1)) kreg[i] = u32x4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int at = i * KPP * 2 * D;
-            // Passes that are no multiple of 16 keys apart: the swizzle of this pass's key, an exclusive or away.
-            const int kx = KPP % 16 ? k_put ^ (16 * ((win_k_chunk<D>(my_key + i * KPP, 0) ^ win_k_chunk<D>(my_key, 0)))) : k_put;
-            *reinterpret_cast<u32x4*>(kb + at + kx) = kreg[i];
-            *reinterpret_cast<u32x4*>(vb + at + v_put) = vreg[i];
-            if (my_chunk == i) {
-                const int v = step * SK + i * KPP + my_key;
-                const int32_t pos = v < n_prefix ? position_of(v) : win_position(req, v - n_prefix + t0, node_at);
-                const int64_t until = pos < p.sinks ? 0x7fffffff : static_cast<int64_t>(pos) + p.window - 1;
-                lds_reach[buf][i * KPP + my_key] = !((good >> i) & 1) ? -1 : until < 0x7fffffff ? static_cast<int32_t>(until) : 0x7fffffff;
-            }
-        }
-        if (wrong) {
-            lds_bad[buf] = mark;
-            set_status(p.status, TV_STATUS_BAD_PAGE);
-        }
-    };
 
     // --- the rows -------------------------------------------------------------------------------
     const int row = b * ROWS + 32 * wm + c;
@@ -439,173 +555,248 @@ window_attention_kernel(const WindowParams p) {
     for (int i = 0; i < NB; ++i) acc[i] = win_f32x16{};
     float m = -INFINITY, l = 0.0f;
 
-    // K . Q^T of a tile (LDS at `kb`): element i is key 8*(i/4) + 4*half + i%4 of the tile.
-    auto products = [&](const char* kb) {
-        win_f32x16 x = {};
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(kb + (k_get ^ (32 * i)));
-            x = WinType<T>::run(__builtin_bit_cast(V8, a), qb[i], x);
-        }
-        return x;
-    };
     // Products to scores in units of log2, with the biases; those that the row does not see become -inf,
-    // whatever they are.  v0: the tile's first key.
-    auto mask = [&](int v0, int buf, int key0, win_f32x16& x) {
+    // whatever they are.  v0: the tile's first key, `reach_of` the reach of its keys.  Returns false, and leaves the
+    // products, where every row sees every key with no bias, as most tiles below a chain's diagonal do:
+    // 8 chunks of 1024 nodes and a window of 512 take 290 us without that test.
+    auto mask = [&](int v0, const int32_t* reach_of, win_f32x16& x) {
+        const Params a = cold();
         const bool tree = v0 + kWinTile > n_prefix;
+        const int of0 = v0 - n_prefix + t0 + 4 * half;   // the node of element 0, below t0 for prefix keys
+        const int last = node < 0 ? 0 : node;
+        // Four biases a load, of which those of prefix keys and behind the last node seen are dropped, unless
+        // they could lie outside all biases.
+        const bool wide = __all(bias + of0 + 28 <= a->bias + a->bias_elems && bias + of0 >= a->bias);
+        auto biases = [&](int g, uint32_t (&b)[4]) {
+            if (wide) {
+                const win_u32x4u four = *reinterpret_cast<const win_u32x4u*>(bias + of0 + 8 * g);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float add[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) add[i] = 0.0f;
-            if (tree) {
-                const int of0 = v0 - n_prefix + t0 + 16 * h + 4 * half;
-                const int last = node < 0 ? 0 : node;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int of = of0 + 8 * (i >> 2) + (i & 3);
-                    add[i] = bias[of < 0 ? 0 : of < last ? of : last];
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int of = of0 + 8 * (i >> 2) + (i & 3);
-                    float b2 = add[i] * 1.44269504088896340736f;   // a finite bias stays finite
-                    if (fabsf(b2) == INFINITY) b2 = copysignf(FLT_MAX, b2);
-                    add[i] = of < t0 ? 0.0f : of <= last && add[i] != -INFINITY ? b2 : -INFINITY;
-                }
-            }
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const win_i32x4 reach = *reinterpret_cast<const win_i32x4*>(&lds_reach[buf][key0 + 16 * h + 8 * g + 4 * half]);
+                for (int e = 0; e < 4; ++e) b[e] = four[e];
+            } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = 8 * h + 4 * g + e;
-                    const bool seen = my_pos <= reach[e] && add[4 * g + e] != -INFINITY;
-                    x[i] = seen ? fmaf(x[i], p.c, add[4 * g + e]) : -INFINITY;
+                    const int of = of0 + 8 * g + e;
+                    b[e] = __float_as_uint(bias[of < 0 ? 0 : of < last ? of : last]);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);   // eight biases in registers at a time
+        };
+        const int32_t* reaches = reach_of + 4 * half;
+        int32_t nearest = 0x7fffffff;
+        uint32_t any = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const win_i32x4 reach = *reinterpret_cast<const win_i32x4*>(reaches + 8 * g);
+            nearest = min(nearest, min(min(reach[0], reach[1]), min(reach[2], reach[3])));
         }
+        if (tree) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t b[4];
+                biases(g, b);
+                any |= (b[0] | b[1]) | (b[2] | b[3]);
+            }
+        }
+        const bool plain = (any << 1) == 0 && my_pos <= nearest && (!tree || (of0 >= t0 && of0 + 28 <= last + 4 * half));
+        if (__all(plain || node < 0)) return false;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            __builtin_amdgcn_sched_barrier(0);   // four biases in registers at a time
+            const win_i32x4 reach = *reinterpret_cast<const win_i32x4*>(reaches + 8 * g);
+            uint32_t b[4] = {0, 0, 0, 0};
+            if (tree) biases(g, b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * g + e, of = of0 + 8 * g + e;
+                bool seen = my_pos <= reach[e];
+                float add = 0.0f;
+                if (tree) {
+                    const float given = __uint_as_float(b[e]);
+                    const bool prefix = of < t0;
+                    add = given * 1.44269504088896340736f;   // a finite bias stays finite
+                    if (fabsf(add) == INFINITY) add = copysignf(FLT_MAX, add);
+                    add = prefix ? 0.0f : add;
+                    seen = seen && (prefix || (of <= last && given != -INFINITY));
+                }
+                x[i] = seen ? fmaf(x[i], a->c, add) : -INFINITY;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        return true;
     };
-    auto tiles_of = [&](int step, int buf, bool bad) {
-        const char* kb = lds + buf * 2 * KB + wk * kWinTile * 2 * D;
-        const char* vb = kb + KB;
-        const int left = n_keys - step * SK;
-        const int tiles = (left < SK ? left + kWinTile - 1 : SK) / kWinTile;
-        win_f32x16 x = products(kb);
+    // The factor that is left to the scores of tile t of step j (their products in x).
+    auto hide = [&](int j, int t, win_f32x16& x) {
+        const int32_t* reach_of = &tab_reach[j / TSTEPS & 1][j % TSTEPS * SK + t * kWinTile];
+        return mask((run0 + j) * SK + t * kWinTile, reach_of, x) ? 1.0f : p.c;
+    };
+    V8 pb[TERMS][2];
+    // The sum is of the probabilities as they are multiplied.
+    auto exponentials = [&](const win_f32x16& x, float cs, float negative) {
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int n = 0; n < TILES; ++n) {
-            const int t = n * WK + wk;
-            if (t >= tiles) break;
-            const int key = n * WK * kWinTile;   // of the tile, from the wave's first
-            const int v0 = step * SK + t * kWinTile;
-            float cs = p.c;
-            if (bad || !clear_run(v0, kWinTile)) {
-                mask(v0, buf, t * kWinTile, x);
-                cs = 1.0f;
-            }
-            // Probabilities against the row's reference, which is near the largest score seen: it is
-            // raised only when a tile's would pass 2^8, until when they cost no precision.
-            float negative = m == -INFINITY ? 0.0f : kShift - m;
-            win_f32x16 pr;
-            // Both times in one order: a row whose neighbours raise their reference is summed a second time.
-            auto exponentials = [&]() {
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < 16; i += 2) {
+            float a = __builtin_amdgcn_exp2f(fmaf(x[i], cs, negative)), b = __builtin_amdgcn_exp2f(fmaf(x[i + 1], cs, negative));
+            if constexpr (TERMS > 1) sum[(i >> 1) & 1] += a + b;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    pr[i] = __builtin_amdgcn_exp2f(fmaf(x[i], cs, negative));
-                    sum[i & 3] += pr[i];
-                }
-                return (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            };
-            float tile_sum = exponentials();
-            const bool over = !(tile_sum <= kOver) || m == -INFINITY;
-            if (__any(over)) {   // other rows of the wave keep their reference: no row depends on another
-                float top = x[0] * cs;
-#pragma unroll
-                for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i] * cs);
-                const float raised = win_pair_max(over ? 1.0f : 0.0f) != 0.0f ? fmaxf(m, win_pair_max(top)) : m;
-                const float factor = raised == m ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
-                m = raised;
-                l *= factor;
-#pragma unroll
-                for (int i = 0; i < NB; ++i) acc[i] *= factor;
-                negative = m == -INFINITY ? 0.0f : kShift - m;
-                tile_sum = exponentials();
-            }
-            l += tile_sum;
-            V8 pb[TERMS][2];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float pv = pr[i];
-#pragma unroll
-                for (int q = 0; q < TERMS; ++q) {
-                    pb[q][i >> 3][i & 7] = static_cast<T>(pv);
-                    if (q + 1 < TERMS) pv -= static_cast<float>(pb[q][i >> 3][i & 7]);
-                }
-            }
-            win_i16x4 va[NB][2];
-            auto read_values = [&](int kk) {
-#pragma unroll
-                for (int db = 0; db < NB; ++db) {
-                    const char* lo = vb + (key + 16 * kk) * 2 * D + (v_get ^ (64 * db));
-                    va[db][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((win_lds_i16x4*)lo);
-                    va[db][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((win_lds_i16x4*)(lo + 8 * 2 * D));
-                }
-            };
-            read_values(0);
-            if (n + 1 < TILES) x = products(kb + (key + WK * kWinTile) * 2 * D);
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                if (kk) read_values(kk);
-#pragma unroll
-                for (int db = 0; db < NB; ++db) {
-                    const V8 v8 = __builtin_bit_cast(V8, __builtin_shufflevector(va[db][0], va[db][1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int q = 0; q < TERMS; ++q) acc[db] = WinType<T>::run(v8, pb[q][kk], acc[db]);
+            for (int q = 0; q < TERMS; ++q) {
+                const T a1 = static_cast<T>(a), b1 = static_cast<T>(b);
+                pb[q][i >> 3][i & 7] = a1;
+                pb[q][i >> 3][(i & 7) + 1] = b1;
+                if constexpr (TERMS == 1) sum[(i >> 1) & 1] = WinType<T>::add_pair(a1, b1, sum[(i >> 1) & 1]);
+                if (q + 1 < TERMS) {
+                    a -= static_cast<float>(a1);
+                    b -= static_cast<float>(b1);
                 }
             }
         }
+        return sum[0] + sum[1];
     };
+    // Probabilities against the row's reference, which is near the largest score seen: it is raised only when
+    // a tile's would pass 2^8, until when they cost no precision.
+    auto reference = [&]() { return m == -INFINITY ? 0.0f : kShift - m; };
+    auto raise = [&](const win_f32x16& x, float cs, float& tile_sum) {
+        const bool over = !(tile_sum <= kOver) || m == -INFINITY;
+        if (__any(over)) {   // other rows of the wave keep their reference: no row depends on another
+            float top = x[0] * cs;
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i] * cs);
+            const float raised = win_pair_max(over ? 1.0f : 0.0f) != 0.0f ? fmaxf(m, win_pair_max(top)) : m;
+            const float factor = raised == m ? 1.0f : __builtin_amdgcn_exp2f(m - raised);
+            m = raised;
+            l *= factor;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) acc[i] *= factor;
+            // In the same order as before: a row whose neighbours raise their reference is summed a second time.
+            tile_sum = exponentials(x, cs, reference());
+        }
+        l += tile_sum;
+    };
+    // The matrix products of a tile step in a fixed order: K . Q^T of a tile (LDS at `kb`) into x, of which element i is
+    // key 8*(i/4) + 4*half + i%4, and V^T . P^T of another (at `vb`), in turn, each with its operands read from LDS
+    // kAhead products before.  `first` runs while the first operands are read.
+    auto multiply = [&](auto with_keys, const char* kb, win_f32x16& x, auto with_values, const char* vb, auto first) {
+        constexpr bool KEYS = decltype(with_keys)::value, VALUES = decltype(with_values)::value;
+        constexpr int NV = 2 * NB, SLOTS = (KEYS ? NK : 0) + (VALUES ? NV : 0);
+        static_assert(NK == NV, "as many products of either kind");
+        u32x4 operand[SLOTS];
+        auto read = [&](auto slot) {
+            constexpr int S = decltype(slot)::value;
+            if constexpr (S < SLOTS) {
+                constexpr bool KEY = KEYS && (!VALUES || S % 2 == 0);
+                constexpr int N = KEYS && VALUES ? S / 2 : S;
+                if constexpr (KEY) {
+                    operand[S] = *reinterpret_cast<const u32x4*>(kb + (k_get ^ (32 * N)));
+                } else {
+                    const char* lo = vb + 16 * (N / NB) * 2 * D + (v_get ^ (64 * (N % NB)));
+                    const win_i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((win_lds_i16x4*)lo);
+                    const win_i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((win_lds_i16x4*)(lo + 8 * 2 * D));
+                    operand[S] = __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+            }
+        };
+        auto product = [&](auto slot) {
+            constexpr int S = decltype(slot)::value;
+            constexpr bool KEY = KEYS && (!VALUES || S % 2 == 0);
+            constexpr int N = KEYS && VALUES ? S / 2 : S;
+            read(std::integral_constant<int, S + kAhead>());
+            const V8 a = __builtin_bit_cast(V8, operand[S]);
+            if constexpr (KEY) {
+                x = WinType<T>::run(a, qb[N], x);
+            } else {
+#pragma unroll
+                for (int q = 0; q < TERMS; ++q) acc[N % NB] = WinType<T>::run(a, pb[q][N / NB], acc[N % NB]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        win_each<0, kAhead>(read);
+        __builtin_amdgcn_sched_barrier(0);
+        first();
+        if constexpr (KEYS) x = win_f32x16{};
+        __builtin_amdgcn_sched_barrier(0);
+        win_each<0, SLOTS>(product);
+    };
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    auto nothing = []() {};
 
     // --- the steps ------------------------------------------------------------------------------
-    if (tid < NBUF) lds_bad[tid] = 0;
-    __syncthreads();
-    int count = 1;   // steps begun, the mark of a buffer with a missing page
-    auto compute = [&](int i, int buf) {
-        if (wave_rows) tiles_of(i, buf, lds_bad[buf] == count);
+    const int todo = run1 - run0;
+    make_table(0);
+    win_barrier();
+    // The table of the steps that are loaded from the next one on.
+    auto next_table = [&](int j) {
+        if ((j + AHEAD + 1) % TSTEPS == 0 && j + AHEAD + 1 < todo) make_table((j + AHEAD + 1) / TSTEPS);
     };
-    fetch_entries(run0);
-    fetch_keys(run0);
-    if (run0 + 1 < run1) fetch_entries(run0 + 1);
-    if constexpr (NBUF == 1) {
-        for (int i = run0; i < run1; ++i, ++count) {
-            __syncthreads();   // the last step's reads of the buffer are done
-            stage(i, 0, count);
-            if (i + 1 < run1) fetch_keys(i + 1);
-            if (i + 2 < run1) fetch_entries(i + 2);
-            __syncthreads();
-            compute(i, 0);
+    if constexpr (WK > 1) {
+#pragma unroll
+        for (int j = 0; j < NBUF; ++j) {
+            if (j < todo) issue(j);
+        }
+#pragma unroll 1
+        for (int j = 0; j < todo; ++j) {
+            if (j + NBUF <= todo) win_wait_loads<(NBUF - 1) * 2 * PASSES>();
+            else win_wait_loads<0>();
+            mend(j);
+            win_barrier();
+            if (wave_rows) {
+                const uint32_t clear = clear_tiles(j);
+                const char* kb = lds + j % NBUF * (2 * KB) + wk * kWinTile * 2 * D;
+                const int left = n_keys - (run0 + j) * SK, tiles = (left < SK ? left + kWinTile - 1 : SK) / kWinTile;
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) {
+                    const int t = n * WK + wk;
+                    if (t >= tiles) break;
+                    const char* at = kb + n * WK * kWinTile * 2 * D;
+                    win_f32x16 x;
+                    multiply(yes, at, x, no, nullptr, nothing);
+                    const float cs = (clear >> (8 * t)) & 1 ? p.c : hide(j, t, x);
+                    multiply(no, nullptr, x, yes, at + KB, [&]() {
+                        float tile_sum = exponentials(x, cs, reference());
+                        raise(x, cs, tile_sum);
+                    });
+                }
+            }
+            next_table(j);
+            win_barrier();   // the step's reads of its buffer are done
+            if (j + NBUF < todo) issue(j + NBUF);
         }
     } else {
-        // Two buffers: a step is staged while the one before it is computed, by half of the waves before
-        // their tiles and by the others after, so that a SIMD's matrix unit has work while the other wave moves.
-        static_assert(WK == 1, "the waves would join over buffers in use");
-        const bool late = wave >= WM / 2;
-        auto prepare = [&](int i, int buf, int mark) {
-            if (i >= run1) return;
-            stage(i, buf, mark);
-            if (i + 1 < run1) fetch_keys(i + 1);
-            if (i + 2 < run1) fetch_entries(i + 2);
-        };
-        prepare(run0, 0, count);
-        __syncthreads();
-        int buf = 0;
-        for (int i = run0; i < run1; ++i, ++count, buf ^= 1) {
-            if (!late) prepare(i + 1, buf ^ 1, count + 1);
-            compute(i, buf);
-            if (late) prepare(i + 1, buf ^ 1, count + 1);
-            __syncthreads();
+        // Four buffers: this step's, the next one's, whose first scores are multiplied with this one's last values, and
+        // two on their way.
+        static_assert(NBUF == 4, "a step is loaded into the buffer of the one before");
+        const int total = ((run1 * SK < n_keys ? run1 * SK : n_keys) - run0 * SK + kWinTile - 1) / kWinTile;   // tiles
+        issue(0);
+        if (1 < todo) issue(1);
+        if (2 < todo) issue(2);
+        if (2 < todo) win_wait_loads<2 * PASSES>();
+        else win_wait_loads<0>();
+        mend(0);
+        if (1 < todo) mend(1);
+        win_barrier();
+        win_f32x16 x;
+        if (wave_rows) multiply(yes, lds, x, no, nullptr, nothing);
+#pragma unroll 1
+        for (int j = 0; j < todo; ++j) {
+            const uint32_t clear = clear_tiles(j);
+            if (j + 3 < todo) issue(j + 3);
+            if (wave_rows) {
+                const char* at = lds + j % NBUF * (2 * KB);
+                const char* next = lds + (j + 1) % NBUF * (2 * KB);
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    if (j * TILES + t >= total) break;
+                    const float cs = (clear >> (8 * t)) & 1 ? p.c : hide(j, t, x);
+                    // Past the last tile the scores are of what the buffer holds, and not used.
+                    multiply(yes, t + 1 < TILES ? at + (t + 1) * kWinTile * 2 * D : next, x, yes, at + t * kWinTile * 2 * D + KB, [&]() {
+                        float tile_sum = exponentials(x, cs, reference());
+                        raise(x, cs, tile_sum);
+                    });
+                }
+            }
+            if (j + 3 < todo) win_wait_loads<2 * PASSES>();
+            else win_wait_loads<0>();
+            if (j + 2 < todo) mend(j + 2);
+            next_table(j);
+            win_barrier();
         }
     }
 

@@ -7,9 +7,9 @@ namespace {
 
 constexpr int kMergeThreads = 256;
 constexpr int kMostSplits = 64;
-// A row of up to so many pieces is joined by one group of lanes, others by a whole workgroup.
-constexpr int kFewPieces = 8;
+constexpr int kFewPieces = 4, kManyRows = 4096;
 constexpr int kMergeGroups = 2048;   // workgroups of the merge, about
+constexpr int kLeastKeys = 128;      // that a part of a block's keys is cut to
 // Scores are in units of log2: scale * log2(e) is an fp32 number, which it is up to 2.358e38.
 constexpr float kMaxScale = 2.3e38f;
 
@@ -20,13 +20,13 @@ window_merge_kernel(const WindowParams p) {
     constexpr int CH = D / 4, kSlots = kMergeThreads / CH;
     __shared__ win_f32x4 part[2][kMergeThreads];
     __shared__ float2 part_ml[2][kSlots];
+    __shared__ int32_t find[3 + kMergeThreads / 64];
     const int tid = threadIdx.x, ch = tid % CH, slot = tid / CH;
     const int id = blockIdx.x / p.num_kv_heads, head = blockIdx.x - id * p.num_kv_heads;
-    const int r = win_find<ROWS>(p, id);
-    bool bad;
-    const WinRequest req = win_request<ROWS>(p, r, bad);
-    const int b = id - win_first_id<ROWS>(p, r);
-    if (b < 0 || b >= req.blocks) return;
+    WinBlock block;
+    if (!win_find<ROWS, kMergeThreads>(p, id, find, block)) return;
+    const int b = block.b;
+    const WinRequest req = block.req;
     const int row0 = b * ROWS, left = req.nodes * p.groups - row0, rows = left < ROWS ? left : ROWS;
     const int64_t piece0 = static_cast<int64_t>(blockIdx.x) * p.splits;
     float best, sum;
@@ -68,7 +68,7 @@ window_merge_kernel(const WindowParams p) {
         const int of = row0 + row, node = of / p.groups;
         win_store4<T>(p, req.first_row + node, head * p.groups + of - node * p.groups, 4 * ch, v * scale);
     };
-    if (p.splits <= kFewPieces) {
+    if (p.row_slots) {
         for (int row = blockIdx.y * kSlots + slot; row < rows; row += gridDim.y * kSlots) {
             join(row, 0, 1);
             store(row);
@@ -101,7 +101,7 @@ template <int D, int ROWS>
 void launch_merge(const WindowParams& p, bool bf16, hipStream_t s) {
     constexpr int kSlots = kMergeThreads / (D / 4);
     const int64_t blocks = static_cast<int64_t>(p.block_ids) * p.num_kv_heads;
-    const int64_t most = p.splits <= kFewPieces ? (ROWS + kSlots - 1) / kSlots : ROWS;
+    const int64_t most = p.row_slots ? (ROWS + kSlots - 1) / kSlots : ROWS;
     int64_t parts = (kMergeGroups + blocks - 1) / blocks;
     parts = parts < most ? parts : most;
     const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(parts));
@@ -139,7 +139,8 @@ Launch launch_of(const tv_window_attention_args* a) {
     const int64_t reach = static_cast<int64_t>(a->block_table_width) * a->block_size;
     int64_t keys = static_cast<int64_t>(a->window) + a->sinks;
     keys = (keys < reach ? keys : reach) + average / groups;
-    const int64_t most = (keys + n.shape.step - 1) / n.shape.step;
+    const int64_t least = n.shape.step > kLeastKeys ? n.shape.step : kLeastKeys;
+    const int64_t most = (keys + least - 1) / least;
     int64_t splits = static_cast<int64_t>(a->compute_units) * n.shape.per_cu / blocks;
     splits = splits < most ? splits : most;
     splits = splits < kMostSplits ? splits : kMostSplits;
@@ -216,6 +217,9 @@ extern "C" int tv_window_attention(const tv_window_attention_args* a, void* work
     if (!ok) return fail(TV_ERR_UNSUPPORTED, "%s: query, pool and output rows must start at 16 bytes, head dim contiguous", what);
     for (int i = 0; i < 3; ++i) {
         if (a->k_stride[i] < 0 || a->v_stride[i] < 0) return fail(TV_ERR_INVALID, "%s: negative pool strides", what);
+        if (i < 2 && (a->k_stride[i] > 0x7fffffff || a->v_stride[i] > 0x7fffffff)) {
+            return fail(TV_ERR_UNSUPPORTED, "%s: page and slot strides must be below 2^31", what);
+        }
     }
     const Launch n = launch_of(a);
     if (n.bytes && (!workspace || !aligned(workspace, 16))) return fail(TV_ERR_INVALID, "%s: null or unaligned workspace", what);
@@ -229,12 +233,13 @@ extern "C" int tv_window_attention(const tv_window_attention_args* a, void* work
     p.q_s1 = a->q_stride_head;
     p.k = static_cast<const char*>(a->k_pool);
     p.v = static_cast<const char*>(a->v_pool);
-    p.k_s0 = 2 * a->k_stride[0];
-    p.k_s1 = 2 * a->k_stride[1];
+    p.k_s0 = static_cast<uint32_t>(2 * a->k_stride[0]);
+    p.k_s1 = static_cast<uint32_t>(2 * a->k_stride[1]);
     p.k_s2 = 2 * a->k_stride[2];
-    p.v_s0 = 2 * a->v_stride[0];
-    p.v_s1 = 2 * a->v_stride[1];
+    p.v_s0 = static_cast<uint32_t>(2 * a->v_stride[0]);
+    p.v_s1 = static_cast<uint32_t>(2 * a->v_stride[1]);
     p.v_s2 = 2 * a->v_stride[2];
+    p.same = p.k_s0 == p.v_s0 && p.k_s1 == p.v_s1;
     p.num_blocks = static_cast<int32_t>(a->num_blocks);
     p.block_size = a->block_size;
     uint32_t shift = 0;
@@ -268,6 +273,8 @@ extern "C" int tv_window_attention(const tv_window_attention_args* a, void* work
     p.c = a->scale * 1.44269504088896340736f;
     p.block_ids = static_cast<int32_t>(n.block_ids);
     p.splits = n.splits;
+    // A group of lanes joins a row where there are rows for all, or few pieces; else a workgroup does.
+    p.row_slots = n.splits <= kFewPieces || static_cast<int64_t>(a->total_queries) * a->num_q_heads >= kManyRows;
     if (n.bytes) {
         const int64_t pieces = n.block_ids * a->num_kv_heads * n.splits * n.shape.rows;
         p.ws_o = static_cast<float*>(workspace);
