@@ -16,14 +16,24 @@
 // steps where the batch has too few blocks for the chip; a second launch joins the parts.  Every workgroup
 // finds its block from the live lengths by a sum over the requests' blocks, so no plan is needed; blocks that
 // are not there come last in the launch, since they are what balances it when they lie between others
-// (every second one missing kept half of the shader engines idle: 1302 us for 652).
+// (every second one missing kept half of the shader engines idle, at twice the time).
 //
-// A step: every wave moves its share of the keys from memory to registers one step ahead (page numbers
-// and slots two ahead) and from there to LDS, K and V as [key][dim] with the 16-byte chunks swizzled per
-// key.  Wave (wm, wk) takes rows 32*wm.. and every WK-th 32-key tile: few rows put the waves side by side
+// A key's page, place and reach are looked up once, a thread a key, into tables of 256 or 512 keys in LDS,
+// made one step before their first use.  Tiles of 32 keys that every node of the block sees are found with
+// them by one vote; of the others a table holds a bit a node and key, from the reaches and the biases,
+// which are read there once, coalesced, instead of by every row of every step.  Between the tables a step
+// has no other loads than the DMA of K and V rows to LDS ([key][dim], 16-byte chunks swizzled per key),
+// which stays under way over barriers, up to three steps ahead.
+// Wave (wm, wk) takes rows 32*wm.. and every WK-th 32-key tile: few rows put the waves side by side
 // on the keys, many rows on the rows.  S^T = K . Q^T by 32x32x16 MFMAs leaves a row's scores in one lane
 // pair, and the S^T registers are the P^T operand as they stand: product slot t of lane half g is key
-// 16*kk + 8*(t/4) + 4*g + t%4, which the transposing reads of V deliver.
+// 16*kk + 8*(t/4) + 4*g + t%4, which the transposing reads of V deliver.  With the waves on the rows the scores of
+// the next tile are multiplied in turn with the values of this one, each operand read kAhead products before.
+// A row's reference is raised only when a tile's probabilities would pass 2^8, so most tiles rescale nothing.
+//
+// 32 query heads over 8 KV heads of 128, bf16: 64 trees of 64 nodes over 8192 keys each are bound by the matrix
+// units, 725 us at 0.76 PFLOP/s (keys through registers, and a reach test and a bias read for every score,
+// took 1302); 128 single tokens over 4096 keys by memory, 398 us at 5.4 TB/s (484).
 //
 // A probability is rounded to the operands' type once where the result is of that type, and kept in
 // more terms for fp32 results (bf16: 3, to 2^-26; f16: 2, to 2^-23).  f16 probabilities are held times
@@ -145,10 +155,11 @@ struct WinBlock {
     WinRequest req;
 };
 
-// Finds row block `id` of the batch, blocks of a request and requests following each other; false if there are
-// not so many.  All threads of the workgroup call it; `scratch` is LDS of its own, 3 + a word a wave.
-template <int ROWS, int THREADS>
-__device__ __forceinline__ bool win_find(const WindowParams& p, int id, int32_t* scratch, WinBlock& block) {
+// Counts the batch's row blocks, blocks of a request and requests following each other, and finds number
+// pick(count); false if that is no block.  All threads of the workgroup call it; `scratch` is LDS of its own, 3 + a
+// word a wave.
+template <int ROWS, int THREADS, class PICK>
+__device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch, WinBlock& block, PICK pick) {
     constexpr int WAVES = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // The last workgroup of a launch reports what is wrong with the requests.
@@ -167,8 +178,9 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int id, int32_t*
             const int32_t y = __shfl_up(end, o);
             if (lane >= o) end += y;
         }
+        const int id = pick(__builtin_amdgcn_readlane(end, 63));
+        if (id < 0) return false;
         const uint64_t behind = __ballot(end > id);
-        if (!behind) return false;
         const int r = __ffsll(static_cast<unsigned long long>(behind)) - 1;
         block.r = r;
         block.b = id - __builtin_amdgcn_readlane(end - q.blocks, r);
@@ -194,12 +206,15 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int id, int32_t*
         if (lane >= o) end += y;
     }
     if (lane == 63) scratch[3 + wave] = end;
-    if (tid == 0) scratch[0] = -1;
     __syncthreads();
+    int32_t total = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
         if (w < wave) end += scratch[3 + w];
+        total += scratch[3 + w];
     }
+    const int id = pick(__builtin_amdgcn_readfirstlane(total));
+    if (id < 0) return false;   // the same in every thread
     if (end - mine <= id && id < end) {   // this thread's requests hold it
         int32_t first = end - mine;
         for (int i = r0; i < r1; ++i) {
@@ -215,7 +230,6 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int id, int32_t*
     __syncthreads();
     block.r = __builtin_amdgcn_readfirstlane(scratch[0]);
     block.b = __builtin_amdgcn_readfirstlane(scratch[1]);
-    if (block.r < 0) return false;
     block.req = win_request<ROWS>(p, block.r, bad);
     return true;
 }
@@ -295,7 +309,6 @@ __device__ __forceinline__ void win_each(F& f) {
 }
 
 constexpr int kAhead = 4;      // products between an operand's read and its use
-constexpr int kWinTable = 512; // keys of a table
 
 // s_waitcnt immediates: vector memory operations down to n with nothing else, LDS operations down to none.
 template <int N>
@@ -337,7 +350,7 @@ __device__ __forceinline__ void win_store4(const WindowParams& p, int64_t row, i
 }
 
 template <int D, int WM, int WK, int SK, int NBUF, class T, int TERMS>
-__global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
+__global__ void __launch_bounds__(64 * WM * WK, D == 256 || WK == 4 ? 1 : 2)
 window_attention_kernel(const WindowParams p) {
     constexpr int THREADS = 64 * WM * WK, ROWS = 32 * WM;
     constexpr int LPR = D / 8;                     // lanes that move one key's row
@@ -349,18 +362,27 @@ window_attention_kernel(const WindowParams p) {
     constexpr float kShift = WinType<T>::kShift;
     const float kOver = __builtin_amdgcn_exp2f(8.0f + kShift);
     constexpr int AHEAD = WK == 1 ? 3 : NBUF;      // steps between a step's loads and its products
-    constexpr int TSTEPS = kWinTable / SK;         // steps of a table
+    constexpr int KT = WM == 8 || WK == 4 ? 512 : 256;   // keys of a table
+    constexpr int TSTEPS = KT / SK;                // steps of a table
+    constexpr int KBYTES = KT / 8, KTILES = KT / kWinTile;
+    constexpr int NODES = ROWS < 128 ? ROWS : 128;       // at most, of a block: 256 rows have two heads a node or more
     static_assert(SK % KPP == 0 && SK % (kWinTile * WK) == 0, "a step is whole passes and tiles");
     static_assert(TSTEPS > AHEAD, "a table is read no longer when the next but one is made");
     static_assert(WK == 1 || WK * 32 * D * 4 <= NBUF * 2 * KB, "the waves' results share the staging memory");
     typedef typename WinType<T>::vec V8;
 
     __shared__ __attribute__((aligned(1024))) char lds[NBUF * 2 * KB];
-    // Of the keys of two tables: page and place in it, and the last position that sees the key, -1 if it is not there.
-    __shared__ __attribute__((aligned(16))) u32x2 tab_at[2][kWinTable];
-    __shared__ __attribute__((aligned(16))) int32_t tab_reach[2][kWinTable];
-    __shared__ __attribute__((aligned(4))) uint8_t tab_clear[2][kWinTable / kWinTile];   // every row sees the whole tile
-    __shared__ float2 lds_ml[WM * WK][32];
+    // Of the keys of two tables, page and place in it; of those of the last one made, the last position that sees
+    // the key, -1 if it is not there.
+    __shared__ __attribute__((aligned(16))) u32x2 tab_at[2][KT];
+    __shared__ __attribute__((aligned(16))) int32_t tab_reach[KT];
+    // Which keys a node sees, a bit each; of a tile whether some node does not see all of it (kHides; kWhole: by
+    // looking, 0: without), and whether there is a bias that is neither zero nor -inf.
+    __shared__ __attribute__((aligned(16))) uint8_t tab_bits[2][NODES][KBYTES];
+    __shared__ __attribute__((aligned(4))) uint8_t tab_hides[2][KTILES], tab_other[2][KTILES];
+    __shared__ int32_t node_pos[NODES];
+    constexpr uint8_t kHides = 1, kWhole = 2;
+    __shared__ float2 lds_ml[WK > 1 ? WM * WK : 1][32];
     __shared__ int32_t lds_find[3 + THREADS / 64];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -369,10 +391,19 @@ window_attention_kernel(const WindowParams p) {
     const int c = lane & 31, half = lane >> 5;
 
     // --- the row block and its keys -------------------------------------------------------------
-    const int unit = blockIdx.x / p.num_kv_heads, head = blockIdx.x - unit * p.num_kv_heads;
-    const int id = unit / p.splits, split = unit - id * p.splits;
+    // Workgroups are dealt to the 8 XCDs in turn, so of 8 KV heads each has one, whose row blocks share its L2.  Runs of
+    // whole requests on an XCD gained nothing (64 trees over windows of 8192: 881 us and 889), and lose balance (8 ragged
+    // requests: 116 us and 75).
+    int id = 0, head = 0, split = 0;
     WinBlock block;
-    if (!win_find<ROWS, THREADS>(p, id, lds_find, block)) return;
+    const bool any = win_find<ROWS, THREADS>(p, lds_find, block, [&](int blocks) {
+        const int unit = blockIdx.x / p.num_kv_heads;
+        head = blockIdx.x - unit * p.num_kv_heads;
+        id = unit / p.splits;
+        split = unit - id * p.splits;
+        return id < blocks ? id : -1;
+    });
+    if (!any) return;
     const int r = block.r, b = block.b;
     const WinRequest req = block.req;
     const int rows_all = req.nodes * p.groups;
@@ -386,6 +417,7 @@ window_attention_kernel(const WindowParams p) {
         bool wrong = at != given;
         if (p.pos_step == 2) wrong |= positions[static_cast<int64_t>(n) * 2 + 1] != 0;
         if (wrong) set_status(p.status, TV_STATUS_BAD_POSITION);
+        node_pos[n - node0] = at;   // by every wave, the same
         lowest = at < lowest ? at : lowest;
         highest = at > highest ? at : highest;
     }
@@ -425,16 +457,21 @@ window_attention_kernel(const WindowParams p) {
         return a;
     };
 
-    // --- the tables: keys [run0 * SK + t * kWinTable, ...), a thread a key -------------------------
-    auto make_table = [&](int t) {
+    // --- the tables: keys [run0 * SK + t * KT, ...), a thread a key -------------------------------
+    auto table_keys = [&](int t) {
+        const int keys = (run1 - run0) * SK - t * KT;
+        return keys < KT ? keys : KT;
+    };
+    auto make_keys = [&](int t) {
         const Params a = cold();
+        const int keys = table_keys(t);
 #pragma unroll 1
-        for (int kk = tid; kk < kWinTable; kk += THREADS) {
-            const int v = run0 * SK + t * kWinTable + kk;
+        for (int kk = tid; kk < keys; kk += THREADS) {
+            const int v = run0 * SK + t * KT + kk;
             const bool live = v < n_keys, tree = v >= n_prefix;
             const int of = live ? v : n_keys - 1, t_of = of - n_prefix + t0;   // a key that is there
-            const int32_t pos = of < n_first ? of : of - n_first + w0;
             const bool slot = of >= n_prefix;
+            const int32_t pos = of < n_first ? of : of - n_first + w0;
             int32_t page = win_page_of(a->div_mul, a->div_shift, slot ? 0 : pos);
             const int32_t* from = slot ? reinterpret_cast<const int32_t*>(slots + t_of) : table + page;
             const int32_t entry = from[0], entry_high = from[slot ? 1 : 0];
@@ -453,21 +490,90 @@ window_attention_kernel(const WindowParams p) {
             tab_at[t & 1][kk] = found ? u32x2{static_cast<uint32_t>(page), offset} : u32x2{0, 0};
             const int32_t at = tree ? win_position(req, t_of, given) : pos;
             const int64_t until = at < a->sinks ? 0x7fffffff : static_cast<int64_t>(at) + a->window - 1;
-            tab_reach[t & 1][kk] = !found ? -1 : until < 0x7fffffff ? static_cast<int32_t>(until) : 0x7fffffff;
+            tab_reach[kk] = !found ? -1 : until < 0x7fffffff ? static_cast<int32_t>(until) : 0x7fffffff;
             const uint64_t clear = __ballot(found && !tree && (pos < a->sinks || pos >= from_high));
-            if ((lane & 31) == 0) tab_clear[t & 1][kk / kWinTile] = static_cast<uint32_t>(clear >> lane) == 0xffffffffu;
+            if ((lane & 31) == 0) {
+                tab_hides[t & 1][kk / kWinTile] = static_cast<uint32_t>(clear >> lane) == 0xffffffffu ? 0 : kWhole;
+                tab_other[t & 1][kk / kWinTile] = 0;
+            }
         }
+        win_wait_loads<0>();   // said here, or the compiler says it in every step, for registers that could be loaded yet
     };
-    // The tiles of step j that need no mask, a byte a tile.
-    auto clear_tiles = [&](int j) {
-        const uint8_t* at = &tab_clear[j / TSTEPS & 1][j % TSTEPS * (SK / kWinTile)];
+    // Behind a barrier: the bits of the tiles that are not clear, eight keys of a node a thread.  A chain's tiles below the
+    // diagonal turn out whole.  The biases are read once here, coalesced, and not by every row in the steps, where
+    // waiting for them would wait for the keys under way too.
+    auto make_bits = [&](int t, auto at_once) {
+        const Params a = cold();
+        const int bytes = table_keys(t) / 8, nodes = node1 - node0 + 1;
+        const int my_tile = lane < bytes / (kWinTile / 8) ? lane : 0;
+        if (!__any(tab_hides[t & 1][my_tile] != 0)) return;   // all clear, as most tables of a long window
+        const int v_table = run0 * SK + t * KT;
+        const bool trees = v_table + 8 * bytes > n_prefix, few = a->bias_elems < 8;
+        const float* biases = a->bias + req.bias + static_cast<int64_t>(node0) * req.nodes + (v_table - n_prefix + t0);
+        const float* last = a->bias + a->bias_elems - 8;   // eight can be read from here
+        constexpr int AT_ONCE = decltype(at_once)::value;   // places whose loads are under way
+#pragma unroll 1
+        for (int e0 = tid; e0 < nodes * KBYTES; e0 += AT_ONCE * THREADS) {
+            win_u32x4u b[AT_ONCE][2];
+            if (trees) {
+#pragma unroll
+                for (int q = 0; q < AT_ONCE; ++q) {
+                    const int e = e0 + q * THREADS, n = e / KBYTES, byte = e % KBYTES;
+                    const float* from = biases + (static_cast<int64_t>(n) * req.nodes + 8 * byte);
+                    const bool inside = n < nodes && byte < bytes && from >= a->bias && from <= last;
+                    from = few ? biases : inside ? from : a->bias;
+                    if (!few) {
+                        b[q][0] = *reinterpret_cast<const win_u32x4u*>(from);
+                        b[q][1] = *reinterpret_cast<const win_u32x4u*>(from + 4);
+                    }
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < AT_ONCE; ++q) {
+                const int e = e0 + q * THREADS, n = e / KBYTES, byte = e % KBYTES, tile = byte / (kWinTile / 8);
+                if (n >= nodes || byte >= bytes || tab_hides[t & 1][tile] == 0) continue;
+                const win_i32x4 *reach = reinterpret_cast<const win_i32x4*>(&tab_reach[8 * byte]), low = reach[0], high = reach[1];
+                const int32_t pos = node_pos[n];
+                uint32_t near = 0, other = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) near |= pos <= (i < 4 ? low[i % 4] : high[i % 4]) ? 1u << i : 0u;
+                const int first = v_table + 8 * byte - n_prefix, node = node0 + n;   // below 0: prefix keys
+                if (first + 8 > 0) {
+                    const float* from = biases + (static_cast<int64_t>(n) * req.nodes + 8 * byte);
+                    const bool inside = !few && from >= a->bias && from <= last;
+                    if (!inside) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int of = first + t0 + i;
+                            b[q][i / 4][i % 4] = __float_as_uint(from[of < t0 ? i + t0 - of : of < node ? i : i + node - of]);
+                        }
+                    }
+                    uint32_t hidden = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t bias = b[q][i / 4][i % 4], tree = first + i >= 0 ? 1u << i : 0u;
+                        hidden |= first + t0 + i > node || bias == 0xff800000u ? tree : 0u;
+                        other |= bias << 1 ? tree : 0u;
+                    }
+                    near &= ~hidden;
+                    other &= near;
+                }
+                tab_bits[t & 1][n][byte] = static_cast<uint8_t>(near);
+                if (near != 0xff || other) tab_hides[t & 1][tile] = kHides;
+                if (other) tab_other[t & 1][tile] = 1;
+            }
+        }
+        win_wait_loads<0>();
+    };
+    // Which tiles of step j some node does not see all of, a byte a tile.
+    auto hiding_tiles = [&](int j) {
+        const uint8_t* at = &tab_hides[j / TSTEPS & 1][j % TSTEPS * (SK / kWinTile)];
         uint32_t flags;
         if constexpr (SK / kWinTile == 1) flags = *at;
         else if constexpr (SK / kWinTile == 2) flags = *reinterpret_cast<const uint16_t*>(at);
         else flags = *reinterpret_cast<const uint32_t*>(at);
-        return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(flags));
+        return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(flags)) & 0x01010101u * kHides;
     };
-    constexpr uint32_t kAllClear = SK / kWinTile == 1 ? 1u : SK / kWinTile == 2 ? 0x0101u : 0x01010101u;
 
     // --- moving a step's keys -------------------------------------------------------------------
     // Lane l of a load fills place l % LPR of a row, which holds the chunk that the swizzle puts there.
@@ -496,12 +602,12 @@ window_attention_kernel(const WindowParams p) {
             win_dma(v_head + v_row + 16 * vc, to + KB + n * KPP * 2 * D);
         }
     };
-    // Rows that do not see a key have to get zero from its V row, and zero times NaN or infinity is not.  So where a
-    // step's tiles are not all clear, each thread, behind its own loads, makes zeros of such elements, and the key's
+    // Rows that do not see a key have to get zero from its V row, and zero times NaN or infinity is not.  So where some
+    // node does not see all of a step, each thread, behind its own loads, makes zeros of such elements, and the key's
     // scores NaN instead, which hidden scores never show.  It also clears what lies behind a head's end.
     auto mend = [&](int j) {
         const bool whole = p.dim == D;
-        if (clear_tiles(j) == kAllClear && whole) return;
+        if (hiding_tiles(j) == 0 && whole) return;
         char* kb = lds + j % NBUF * (2 * KB) + my_key * 2 * D + 16 * my_place;
         char* vb = kb + KB;
 #pragma unroll
@@ -537,8 +643,6 @@ window_attention_kernel(const WindowParams p) {
     const bool wave_rows = b * ROWS + 32 * wm < rows_all;   // any row of this wave
     const int node = row < rows_all ? row / p.groups : -1;  // -1: no row
     const int qhead = head * p.groups + row - (node < 0 ? 0 : node) * p.groups;
-    const int32_t my_pos = node < 0 ? 0 : win_position(req, node, positions[static_cast<int64_t>(node) * p.pos_step]);
-    const float* bias = p.bias + req.bias + static_cast<int64_t>(node < 0 ? 0 : node) * req.nodes;
     V8 qb[NK];
     {
         const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(req.first_row + (node < 0 ? 0 : node)) * p.q_s0 +
@@ -555,78 +659,46 @@ window_attention_kernel(const WindowParams p) {
     for (int i = 0; i < NB; ++i) acc[i] = win_f32x16{};
     float m = -INFINITY, l = 0.0f;
 
-    // Products to scores in units of log2, with the biases; those that the row does not see become -inf,
-    // whatever they are.  v0: the tile's first key, `reach_of` the reach of its keys.  Returns false, and leaves the
-    // products, where every row sees every key with no bias, as most tiles below a chain's diagonal do:
-    // 8 chunks of 1024 nodes and a window of 512 take 290 us without that test.
-    auto mask = [&](int v0, const int32_t* reach_of, win_f32x16& x) {
+    // Products of tile t of step j to scores in units of log2; those that the row does not see become -inf,
+    // whatever they are.
+    const int my_node = node < 0 ? 0 : node - node0;
+    auto mask = [&](int j, int t, win_f32x16& x) {
+        const int tile = j % TSTEPS * (SK / kWinTile) + t;
+        const uint32_t bits = *reinterpret_cast<const uint32_t*>(&tab_bits[j / TSTEPS & 1][my_node][4 * tile]) >> (4 * half);
+        if (!__builtin_amdgcn_readfirstlane(tab_other[j / TSTEPS & 1][tile])) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = bits & (1u << (8 * (i >> 2) + (i & 3))) ? x[i] * p.c : -INFINITY;
+            return;
+        }
         const Params a = cold();
-        const bool tree = v0 + kWinTile > n_prefix;
-        const int of0 = v0 - n_prefix + t0 + 4 * half;   // the node of element 0, below t0 for prefix keys
+        const float* bias = a->bias + req.bias + static_cast<int64_t>(node < 0 ? 0 : node) * req.nodes;
+        const int of0 = (run0 + j) * SK + t * kWinTile - n_prefix + t0 + 4 * half;   // the node of element 0
         const int last = node < 0 ? 0 : node;
-        // Four biases a load, of which those of prefix keys and behind the last node seen are dropped, unless
-        // they could lie outside all biases.
-        const bool wide = __all(bias + of0 + 28 <= a->bias + a->bias_elems && bias + of0 >= a->bias);
-        auto biases = [&](int g, uint32_t (&b)[4]) {
-            if (wide) {
-                const win_u32x4u four = *reinterpret_cast<const win_u32x4u*>(bias + of0 + 8 * g);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) b[e] = four[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int of = of0 + 8 * g + e;
-                    b[e] = __float_as_uint(bias[of < 0 ? 0 : of < last ? of : last]);
-                }
-            }
-        };
-        const int32_t* reaches = reach_of + 4 * half;
-        int32_t nearest = 0x7fffffff;
-        uint32_t any = 0;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const win_i32x4 reach = *reinterpret_cast<const win_i32x4*>(reaches + 8 * g);
-            nearest = min(nearest, min(min(reach[0], reach[1]), min(reach[2], reach[3])));
-        }
-        if (tree) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                uint32_t b[4];
-                biases(g, b);
-                any |= (b[0] | b[1]) | (b[2] | b[3]);
-            }
-        }
-        const bool plain = (any << 1) == 0 && my_pos <= nearest && (!tree || (of0 >= t0 && of0 + 28 <= last + 4 * half));
-        if (__all(plain || node < 0)) return false;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             __builtin_amdgcn_sched_barrier(0);   // four biases in registers at a time
-            const win_i32x4 reach = *reinterpret_cast<const win_i32x4*>(reaches + 8 * g);
-            uint32_t b[4] = {0, 0, 0, 0};
-            if (tree) biases(g, b);
+            float b[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = 4 * g + e, of = of0 + 8 * g + e;
-                bool seen = my_pos <= reach[e];
-                float add = 0.0f;
-                if (tree) {
-                    const float given = __uint_as_float(b[e]);
-                    const bool prefix = of < t0;
-                    add = given * 1.44269504088896340736f;   // a finite bias stays finite
-                    if (fabsf(add) == INFINITY) add = copysignf(FLT_MAX, add);
-                    add = prefix ? 0.0f : add;
-                    seen = seen && (prefix || (of <= last && given != -INFINITY));
-                }
-                x[i] = seen ? fmaf(x[i], a->c, add) : -INFINITY;
+                const int of = of0 + 8 * g + e;
+                b[e] = bias[of < 0 ? 0 : of < last ? of : last];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * g + e;
+                float add = b[e] * 1.44269504088896340736f;   // a finite bias stays finite
+                if (fabsf(add) == INFINITY) add = copysignf(FLT_MAX, add);
+                x[i] = bits & (1u << (8 * g + e)) ? fmaf(x[i], a->c, of0 + 8 * g + e < t0 ? 0.0f : add) : -INFINITY;
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        return true;
+        win_wait_loads<0>();
     };
-    // The factor that is left to the scores of tile t of step j (their products in x).
-    auto hide = [&](int j, int t, win_f32x16& x) {
-        const int32_t* reach_of = &tab_reach[j / TSTEPS & 1][j % TSTEPS * SK + t * kWinTile];
-        return mask((run0 + j) * SK + t * kWinTile, reach_of, x) ? 1.0f : p.c;
+    // The factor that is left to the scores.
+    auto hide = [&](uint32_t hiding, int j, int t, win_f32x16& x) {
+        if (!((hiding >> (8 * t)) & kHides)) return p.c;
+        mask(j, t, x);
+        return 1.0f;
     };
     V8 pb[TERMS][2];
     // The sum is of the probabilities as they are multiplied.
@@ -720,17 +792,23 @@ window_attention_kernel(const WindowParams p) {
 
     // --- the steps ------------------------------------------------------------------------------
     const int todo = run1 - run0;
-    make_table(0);
+    make_keys(0);
     win_barrier();
-    // The table of the steps that are loaded from the next one on.
+    // The table of the steps that are loaded from the next one on, and a step later its bits.
     auto next_table = [&](int j) {
-        if ((j + AHEAD + 1) % TSTEPS == 0 && j + AHEAD + 1 < todo) make_table((j + AHEAD + 1) / TSTEPS);
+        const int of = j + AHEAD;
+        if ((of + 1) % TSTEPS == 0 && of + 1 < todo) make_keys((of + 1) / TSTEPS);
+        if (of % TSTEPS == 0 && of < todo) make_bits(of / TSTEPS, std::integral_constant<int, 2>());   // beside the results' registers
     };
+    // Biases of the first table are waited for with the first step's keys.
+    issue(0);
+    make_bits(0, std::integral_constant<int, 8>());
     if constexpr (WK > 1) {
 #pragma unroll
-        for (int j = 0; j < NBUF; ++j) {
+        for (int j = 1; j < NBUF; ++j) {
             if (j < todo) issue(j);
         }
+        win_barrier();
 #pragma unroll 1
         for (int j = 0; j < todo; ++j) {
             if (j + NBUF <= todo) win_wait_loads<(NBUF - 1) * 2 * PASSES>();
@@ -738,7 +816,7 @@ window_attention_kernel(const WindowParams p) {
             mend(j);
             win_barrier();
             if (wave_rows) {
-                const uint32_t clear = clear_tiles(j);
+                const uint32_t hiding = hiding_tiles(j);
                 const char* kb = lds + j % NBUF * (2 * KB) + wk * kWinTile * 2 * D;
                 const int left = n_keys - (run0 + j) * SK, tiles = (left < SK ? left + kWinTile - 1 : SK) / kWinTile;
 #pragma unroll
@@ -748,7 +826,7 @@ window_attention_kernel(const WindowParams p) {
                     const char* at = kb + n * WK * kWinTile * 2 * D;
                     win_f32x16 x;
                     multiply(yes, at, x, no, nullptr, nothing);
-                    const float cs = (clear >> (8 * t)) & 1 ? p.c : hide(j, t, x);
+                    const float cs = hide(hiding, j, t, x);
                     multiply(no, nullptr, x, yes, at + KB, [&]() {
                         float tile_sum = exponentials(x, cs, reference());
                         raise(x, cs, tile_sum);
@@ -764,9 +842,9 @@ window_attention_kernel(const WindowParams p) {
         // two on their way.
         static_assert(NBUF == 4, "a step is loaded into the buffer of the one before");
         const int total = ((run1 * SK < n_keys ? run1 * SK : n_keys) - run0 * SK + kWinTile - 1) / kWinTile;   // tiles
-        issue(0);
         if (1 < todo) issue(1);
         if (2 < todo) issue(2);
+        win_barrier();
         if (2 < todo) win_wait_loads<2 * PASSES>();
         else win_wait_loads<0>();
         mend(0);
@@ -776,7 +854,7 @@ window_attention_kernel(const WindowParams p) {
         if (wave_rows) multiply(yes, lds, x, no, nullptr, nothing);
 #pragma unroll 1
         for (int j = 0; j < todo; ++j) {
-            const uint32_t clear = clear_tiles(j);
+            const uint32_t hiding = hiding_tiles(j);
             if (j + 3 < todo) issue(j + 3);
             if (wave_rows) {
                 const char* at = lds + j % NBUF * (2 * KB);
@@ -784,7 +862,7 @@ window_attention_kernel(const WindowParams p) {
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
                     if (j * TILES + t >= total) break;
-                    const float cs = (clear >> (8 * t)) & 1 ? p.c : hide(j, t, x);
+                    const float cs = hide(hiding, j, t, x);
                     // Past the last tile the scores are of what the buffer holds, and not used.
                     multiply(yes, t + 1 < TILES ? at + (t + 1) * kWinTile * 2 * D : next, x, yes, at + t * kWinTile * 2 * D + KB, [&]() {
                         float tile_sum = exponentials(x, cs, reference());

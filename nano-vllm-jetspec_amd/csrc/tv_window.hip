@@ -7,6 +7,7 @@ namespace {
 
 constexpr int kMergeThreads = 256;
 constexpr int kMostSplits = 64;
+constexpr int kLongRun = 1024;       // keys of a block, from which on 256 rows pay
 constexpr int kFewPieces = 4, kManyRows = 4096;
 constexpr int kMergeGroups = 2048;   // workgroups of the merge, about
 constexpr int kLeastKeys = 128;      // that a part of a block's keys is cut to
@@ -24,7 +25,7 @@ window_merge_kernel(const WindowParams p) {
     const int tid = threadIdx.x, ch = tid % CH, slot = tid / CH;
     const int id = blockIdx.x / p.num_kv_heads, head = blockIdx.x - id * p.num_kv_heads;
     WinBlock block;
-    if (!win_find<ROWS, kMergeThreads>(p, id, find, block)) return;
+    if (!win_find<ROWS, kMergeThreads>(p, find, block, [&](int blocks) { return id < blocks ? id : -1; })) return;
     const int b = block.b;
     const WinRequest req = block.req;
     const int row0 = b * ROWS, left = req.nodes * p.groups - row0, rows = left < ROWS ? left : ROWS;
@@ -129,16 +130,23 @@ struct Launch {
 // keys of a block cut where the blocks alone would leave compute units idle.
 Launch launch_of(const tv_window_attention_args* a) {
     const int64_t groups = a->num_q_heads / a->num_kv_heads, rows = a->total_queries * groups;
-    const int64_t average = (rows + a->num_requests - 1) / a->num_requests;
+    int64_t average = (rows + a->num_requests - 1) / a->num_requests;
+    const int64_t reach = static_cast<int64_t>(a->block_table_width) * a->block_size;
+    // Keys of a block, about: what its window spans and its own nodes, or all that there are.
+    const int64_t nodes = average / groups;
+    int64_t keys = static_cast<int64_t>(a->window) + a->sinks + (average < 256 ? average : 256) / groups;
+    keys = keys < reach + nodes ? keys : reach + nodes;
+    // Blocks have at most 128 nodes.  256 rows read their keys once for twice the rows, 128 are two workgroups a compute
+    // unit, one of which fills the other's start and end: 32 query heads over 8 KV heads of 128, 4 chains of 1024 nodes,
+    // window 128 / 512 / 1024 / 4096: 128 rows 55 / 97 / 149 / 393 us, 256 rows 70 / 108 / 142 / 329; 64 trees of 64 nodes,
+    // 512 / 1024 / 4096: 85 / 142 / 408 and 93 / 141 / 358.
+    if (average > 128 && (groups == 1 || keys < kLongRun)) average = 128;
     Launch n;
     n.width = a->head_dim <= 64 ? 64 : a->head_dim <= 128 ? 128 : 256;
     n.shape = n.width == 64 ? window_shape_d64(average) : n.width == 128 ? window_shape_d128(average) : window_shape_d256(average);
     n.block_ids = rows / n.shape.rows + a->num_requests;
     int64_t blocks = (rows + n.shape.rows - 1) / n.shape.rows;
     blocks = (blocks > a->num_requests ? blocks : a->num_requests) * a->num_kv_heads;
-    const int64_t reach = static_cast<int64_t>(a->block_table_width) * a->block_size;
-    int64_t keys = static_cast<int64_t>(a->window) + a->sinks;
-    keys = (keys < reach ? keys : reach) + average / groups;
     const int64_t least = n.shape.step > kLeastKeys ? n.shape.step : kLeastKeys;
     const int64_t most = (keys + least - 1) / least;
     int64_t splits = static_cast<int64_t>(a->compute_units) * n.shape.per_cu / blocks;

@@ -88,6 +88,31 @@ def test_every_shape_of_launch(dim):
         check(attend(b), b, f"{requests} {prefix} {window} {dim}")
 
 
+@pytest.mark.parametrize("page", [1, 16, 48])
+@pytest.mark.parametrize("groups", [1, 2, 3, 8])
+def test_long_blocks(groups, page):
+    # Keys of many tables, blocks of 128 nodes and of 256 rows, the first tokens before and inside the tree.
+    for prefixes, sizes, window, sinks in (([2300], [300], 1500, 5), ([1200, 0], [300, 270], 2000, 1300), ([40], [600], 2 ** 20, 0)):
+        b = Batch(prefixes, [chain(n) for n in sizes], window=window, sinks=sinks, groups=groups, kv_heads=1, dim=64, page=page,
+                  seed=groups)
+        check(attend(b), b, f"{groups} {page} {prefixes}")
+
+
+@pytest.mark.parametrize("groups, dtype", [(1, BF16), (2, F16), (4, BF16)])
+def test_finite_biases_in_long_trees(groups, dtype):
+    # A few rows' biases are neither zero nor -inf, in tiles that are whole otherwise.
+    sizes, rng = [300, 130], np.random.default_rng(groups)
+    bias = []
+    for n in sizes:
+        x = np.where(np.tril(np.ones((n, n))) > 0, 0.0, -np.inf).astype(np.float32)
+        x[::37] += np.where(rng.random(x[::37].shape) < 0.5, 0.0, rng.normal(size=x[::37].shape)).astype(np.float32)
+        bias.append(x)
+    for window, sinks in ((2000, 4), (90, 50)):
+        b = Batch([1300, 20], [chain(n) for n in sizes], window=window, sinks=sinks, groups=groups, kv_heads=1, dtype=dtype,
+                  seed=groups, bias=np.concatenate([x.reshape(-1) for x in bias]))
+        check(attend(b), b, f"{groups} {window}")
+
+
 def test_rows_that_see_nothing_and_finite_biases():
     sizes = [6, 40]
     rng = np.random.default_rng(1)
