@@ -19,6 +19,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "tv_internal.h"
 
 namespace tv {
@@ -27,6 +29,7 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kUnroll = 4;      // units a lane loads at a time
 constexpr int kMostTop = 64;
+constexpr int kFull = 32;       // entries of a wave's queue that are merged into its list
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kMargin = 8.0f;
 // R is c x rounded to fp32, and c x - R has to stay near zero for the x it was made of: so up to 2^16.  Larger
@@ -92,31 +95,82 @@ __device__ __forceinline__ uint64_t entry_of(float x, int64_t index) {
     return static_cast<uint64_t>(order_of(x)) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(index));
 }
 
-__device__ __forceinline__ uint64_t from_lane_xor(uint64_t v, int mask) {
-    return static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), mask));
+// The value of lane ^ M: by a row's own permutations up to 8, and by swaps of half rows and rows above, which take a
+// tenth of the latency of an exchange through LDS.  All lanes call it.
+template <int CTRL>
+__device__ __forceinline__ uint32_t row_moved(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xf, 0xf, false));
+}
+template <int M>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    if constexpr (M == 1) return row_moved<0xB1>(v);                        // quad_perm [1, 0, 3, 2]
+    else if constexpr (M == 2) return row_moved<0x4E>(v);                   // quad_perm [2, 3, 0, 1]
+    else if constexpr (M == 4) return row_moved<0x1B>(row_moved<0x141>(v)); // half row mirrored, quad_perm [3, 2, 1, 0]
+    else if constexpr (M == 8) return row_moved<0x128>(v);                  // row rotated by 8
+    else if constexpr (M == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? r[0] : r[1];
+    } else {
+        static_assert(M == 32, "a power of two below 64");
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return threadIdx.x & 32 ? r[0] : r[1];
+    }
+}
+template <int M>
+__device__ __forceinline__ float lane_xor(float v) {
+    return __uint_as_float(lane_xor<M>(__float_as_uint(v)));
+}
+template <int M>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+    return static_cast<uint64_t>(lane_xor<M>(static_cast<uint32_t>(v >> 32))) << 32 | lane_xor<M>(static_cast<uint32_t>(v));
+}
+// v, joined by `f` over the wave's lanes in a fixed order, in all of them.
+template <class V, class F>
+__device__ __forceinline__ V over_lanes(V v, F f) {
+    v = f(v, lane_xor<1>(v));
+    v = f(v, lane_xor<2>(v));
+    v = f(v, lane_xor<4>(v));
+    v = f(v, lane_xor<8>(v));
+    v = f(v, lane_xor<16>(v));
+    return f(v, lane_xor<32>(v));
 }
 
-// Bitonic steps over the wave's 64 lanes, largest first.
-__device__ __forceinline__ uint64_t merged(uint64_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int j = 32; j > 0; j >>= 1) {
-        const uint64_t o = from_lane_xor(v, j);
-        v = ((lane & j) == 0) == (v > o) ? v : o;
+// Bitonic steps over the wave's 64 lanes, largest first: halves of J lanes compared, in blocks of K.
+template <int J, int K, class V>
+__device__ __forceinline__ void merge_step(V& v) {
+    if constexpr (J > 0) {
+        const V o = lane_xor<J>(v);
+        const int lane = threadIdx.x & 63;
+        const bool larger = ((lane & J) == 0) == ((lane & K) == 0);
+        v = larger == (v > o) ? v : o;
+        merge_step<J / 2, K>(v);
     }
+}
+template <class V>
+__device__ __forceinline__ V merged(V v) {
+    merge_step<32, 64>(v);
     return v;
 }
-__device__ __forceinline__ uint64_t sorted(uint64_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int k = 2; k < 64; k <<= 1) {
-#pragma unroll
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            const uint64_t o = from_lane_xor(v, j);
-            v = (((lane & j) == 0) == ((lane & k) == 0)) == (v > o) ? v : o;
-        }
-    }
+template <class V>
+__device__ __forceinline__ V sorted(V v) {
+    merge_step<1, 2>(v);
+    merge_step<2, 4>(v);
+    merge_step<4, 8>(v);
+    merge_step<8, 16>(v);
+    merge_step<16, 32>(v);
     return merged(v);
+}
+template <class V>
+__device__ __forceinline__ V lane_reversed(V v) {
+    v = lane_xor<32>(lane_xor<16>(v));
+    return lane_xor<8>(lane_xor<4>(lane_xor<2>(lane_xor<1>(v))));
+}
+// A lane's value in all; the lane is the same for all.
+__device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+__device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) {
+    return static_cast<uint64_t>(of_lane(static_cast<uint32_t>(v >> 32), lane)) << 32 | of_lane(static_cast<uint32_t>(v), lane);
 }
 
 // A wave's largest entries.  Entries are distinct, but for the empty one, 0.
@@ -135,12 +189,17 @@ struct WaveTop {
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         const uint64_t mine = from + lane < queued ? queue[from + lane] : 0;
         queued = from;
-        const uint64_t other = static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(sorted(mine)), 63 - lane));
+        merge(sorted(mine));
+    }
+    // Merges another sorted list.
+    __device__ __forceinline__ void merge(uint64_t list) {
+        const uint64_t other = lane_reversed(list);
         best = merged(best > other ? best : other);
-        kth = static_cast<uint64_t>(__shfl(static_cast<unsigned long long>(best), top - 1));
+        kth = of_lane(best, top - 1);
     }
     __device__ __forceinline__ void push(bool want, uint64_t entry) {
         const uint64_t lanes = __ballot(want);
+        if (lanes == 0) return;
         if (want) {
             const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
                                                          __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0));
@@ -172,40 +231,33 @@ struct Sums {
     }
 };
 
-// Joins the waves' lists and sums in LDS: `list` gets the largest, thread 0 holds the sums.
+// Joins the waves' sums and lists: all threads get the sums, the first wave the list.
 struct Joined {
-    uint64_t all[kThreads];
     float sums[kWaves][3];
-    uint64_t list[kMostTop];
+    uint64_t all[kWaves][64];
 };
 
 template <bool TOP>
-__device__ __forceinline__ Sums join(Joined& s, const WaveTop& t, Sums mine, int top) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mine.add({__shfl_xor(mine.r, o), __shfl_xor(mine.z, o), __shfl_xor(mine.e, o)});
+__device__ __forceinline__ Sums join(Joined& s, WaveTop& t, Sums mine) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    mine.rescale(over_lanes(mine.r, [](float a, float b) { return fmaxf(a, b); }));
+    mine.z = over_lanes(mine.z, [](float a, float b) { return a + b; });
+    mine.e = over_lanes(mine.e, [](float a, float b) { return a + b; });
     if (lane == 0) {
         s.sums[wave][0] = mine.r;
         s.sums[wave][1] = mine.z;
         s.sums[wave][2] = mine.e;
     }
-    if constexpr (TOP) {
-        s.all[tid] = lane < top ? t.best : 0;
-        if (tid < kMostTop) s.list[tid] = 0;
-    }
+    if constexpr (TOP) s.all[wave][lane] = t.best;
     __syncthreads();
     Sums row;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) row.add({s.sums[w][0], s.sums[w][1], s.sums[w][2]});
     if constexpr (TOP) {
-        if (lane < top && t.best != 0) {
-            int rank = 0;
-            for (int w = 0; w < kWaves; ++w) {
-                for (int i = 0; i < top; ++i) rank += s.all[64 * w + i] > t.best;
-            }
-            if (rank < top) s.list[rank] = t.best;
+        if (wave == 0) {
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) t.merge(s.all[w][lane]);
         }
-        __syncthreads();
     }
     return row;
 }
@@ -217,7 +269,7 @@ __device__ __forceinline__ float sum_far(const LogprobParams& p, const typename 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float most = -INFINITY;
     for (int64_t j = threadIdx.x; j < p.vocab; j += kThreads) most = __builtin_elementwise_maximum(most, T::load(x[j]));
-    for (int o = 1; o < 64; o <<= 1) most = __builtin_elementwise_maximum(most, __shfl_xor(most, o));
+    most = over_lanes(most, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
     if (lane == 0) parts[wave][0] = most;
     __syncthreads();
     for (int w = 0; w < kWaves; ++w) most = __builtin_elementwise_maximum(most, parts[w][0]);
@@ -228,10 +280,8 @@ __device__ __forceinline__ float sum_far(const LogprobParams& p, const typename 
         z += one;
         e = fmaf(one, d, e);
     }
-    for (int o = 1; o < 64; o <<= 1) {
-        z += __shfl_xor(z, o);
-        e += __shfl_xor(e, o);
-    }
+    z = over_lanes(z, [](float a, float b) { return a + b; });
+    e = over_lanes(e, [](float a, float b) { return a + b; });
     if (lane == 0) {
         parts[wave][0] = z;
         parts[wave][1] = e;
@@ -246,9 +296,9 @@ __device__ __forceinline__ float sum_far(const LogprobParams& p, const typename 
     return most;
 }
 
-// What a row's sums and list say.  All threads call it; the list lies in LDS behind a barrier.
+// What a row's sums and list say.  All threads call it; lane j of the first wave holds the list's j-th `entry`.
 template <class T, bool TOP>
-__device__ __forceinline__ void finish(const LogprobParams& p, int64_t i, int64_t row, Sums sums, const uint64_t* list) {
+__device__ __forceinline__ void finish(const LogprobParams& p, int64_t i, int64_t row, Sums sums, uint64_t entry) {
     typedef typename T::storage S;
     const S* x = reinterpret_cast<const S*>(p.logits) + row * p.stride;
     double reference = static_cast<double>(sums.r) / static_cast<double>(kLog2e);
@@ -270,7 +320,6 @@ __device__ __forceinline__ void finish(const LogprobParams& p, int64_t i, int64_
     if constexpr (TOP) {
         const int j = threadIdx.x;
         if (j < p.top) {
-            const uint64_t entry = list[j];
             p.top_ids[i * p.top + j] = static_cast<int64_t>(~static_cast<uint32_t>(entry));
             const float value = value_of(static_cast<uint32_t>(entry >> 32));
             p.top_logprobs[i * p.top + j] = none ? NAN : static_cast<float>(static_cast<double>(value) - reference - log_sum);
@@ -304,6 +353,8 @@ logprobs_kernel(const LogprobParams p) {
     constexpr int VEC = 16 / sizeof(S);
     __shared__ Joined joined;
     __shared__ uint64_t queues[kWaves][TOP ? 64 * (VEC + 1) : 1];
+    // A wave reads what others have written so far.
+    __shared__ volatile uint32_t shared_full[kWaves], shared_quarter[kWaves];
     const int64_t i = blockIdx.x / p.splits;
     const int split = static_cast<int>(blockIdx.x - i * p.splits);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -323,10 +374,36 @@ logprobs_kernel(const LogprobParams p) {
     WaveTop tops;
     tops.queue = queues[wave];
     tops.top = p.top;
-    uint32_t pass = 0;             // the order that a candidate has to pass
-    float bound = __uint_as_float(0x7fc00000u);   // its value; NaN: everything is one
-    // A lane's `count` elements x (the others -inf), the first of which has index `first`.
-    auto process = [&](const float (&x)[VEC], int64_t first, int count) {
+    uint32_t pass = 0;             // whatever has this order or a lower one is not among the row's largest
+    float bound = __uint_as_float(0x7fc00000u);   // its value; NaN: everything is a candidate
+    auto raise_pass = [&](uint32_t to) {
+        if (to <= pass) return;
+        pass = to;
+        bound = bound_of(to);
+    };
+    // What a wave's sorted list says to all: its top-th entry has top elements from it on, and where every wave has a
+    // quarter of them at some value, so have they all together.  Another wave's equal value can come first.
+    auto publish = [&](auto list) {
+        constexpr int kShift = sizeof(list) == 8 ? 32 : 0;
+        const uint32_t full = static_cast<uint32_t>(of_lane(list, p.top - 1) >> kShift);
+        const uint32_t quarter = static_cast<uint32_t>(of_lane(list, (p.top + kWaves - 1) / kWaves - 1) >> kShift);
+        if (lane == 0) {
+            shared_full[wave] = full;
+            shared_quarter[wave] = quarter;
+        }
+    };
+    auto look = [&]() {
+        uint32_t most = shared_full[0], least = shared_quarter[0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            most = max(most, static_cast<uint32_t>(shared_full[w]));
+            least = min(least, static_cast<uint32_t>(shared_quarter[w]));
+        }
+        most = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(max(most, least))));
+        if (most > 0) raise_pass(most - 1);
+    };
+    // A lane's `count` elements x (the others -inf), the first of which has index `first`; all -inf where it is not live.
+    auto process = [&](const float (&x)[VEC], int64_t first, bool live, auto count) {
         float most = x[0];
 #pragma unroll
         for (int e = 1; e < VEC; ++e) most = __builtin_elementwise_maximum(most, x[e]);   // NaN where one is
@@ -344,23 +421,22 @@ logprobs_kernel(const LogprobParams p) {
             if constexpr (TOP) {
                 if (__any(candidate)) {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) tops.push(e < count && order_of(x[e]) > pass, entry_of(x[e], first + e));
-                    while (tops.queued >= 64) tops.flush();
-                    // Elements to come have higher indices, so an equal value is not enough.
-                    const uint32_t kth = static_cast<uint32_t>(tops.kth >> 32);
-                    if (kth > pass) {
-                        pass = kth;
-                        bound = bound_of(kth);
+                    for (int e = 0; e < decltype(count)::value; ++e) tops.push(live && !(x[e] <= bound), entry_of(x[e], first + e));
+                    if (tops.queued >= kFull) {
+                        while (tops.queued >= kFull) tops.flush();
+                        // This wave's elements to come have higher indices, so an equal value is not enough.
+                        raise_pass(static_cast<uint32_t>(tops.kth >> 32));
+                        publish(tops.best);
                     }
                 }
             }
         }
-        float z[VEC], z_e = 0.0f;
+        float z[VEC], z_e[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const float d = fmaxf(fmaf(x[e], kLog2e, -sums.r), -200.0f);
             z[e] = __builtin_amdgcn_exp2f(d);
-            z_e = fmaf(z[e], d, z_e);
+            z_e[e & 1] = fmaf(z[e], d, z_e[e & 1]);
         }
 #pragma unroll
         for (int o = 1; o < VEC; o <<= 1) {
@@ -368,63 +444,76 @@ logprobs_kernel(const LogprobParams p) {
             for (int e = 0; e + o < VEC; e += 2 * o) z[e] += z[e + o];
         }
         sums.z += z[0];
-        sums.e += z_e;
+        sums.e += z_e[0] + z_e[1];
     };
     auto lone = [&](int64_t index, bool live) {
         float x[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) x[e] = -INFINITY;
         if (live) x[0] = T::load(base[index]);
-        process(x, index, live ? 1 : 0);
+        process(x, index, live, std::integral_constant<int, 1>());
     };
-    if (split == 0 && wave == 0 && head > 0) lone(lane < head ? lane : 0, lane < head);
-    bool begun = false;
-    for (int64_t u0 = unit0 + 64 * wave; u0 < unit1; u0 += 64 * kWaves * kUnroll) {
-        u32x4 raw[kUnroll];
+    constexpr int kStride = 64 * kWaves;    // units between a lane's
+    u32x4 raw[kUnroll];
+    auto load = [&](int64_t u0) {
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k) {
-            const int64_t u = u0 + 64 * kWaves * k + lane;
+            const int64_t u = u0 + kStride * k + lane;
             raw[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(body + (u < unit1 ? u : unit1 - 1) * VEC));
         }
-        if (TOP && !begun) {
-            // The k-th largest of the lanes' maxima is at most the k-th largest element.
-            begun = true;
-            uint32_t most = 0;
+        if (u0 + kStride * (kUnroll - 1) + 64 > unit1) {
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k) {
-                S s[VEC];
-                __builtin_memcpy(s, &raw[k], 16);
-                const bool live = u0 + 64 * kWaves * k + lane < unit1;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) most = live ? max(most, order_of(T::load(s[e]))) : most;
-            }
-            const uint32_t kth = static_cast<uint32_t>(__shfl(static_cast<unsigned long long>(sorted(most)), p.top - 1));
-            if (kth > 0 && kth - 1 > pass) {
-                pass = kth - 1;
-                bound = bound_of(kth - 1);
+                if (u0 + kStride * k + lane >= unit1) raw[k] = u32x4{T::kNone, T::kNone, T::kNone, T::kNone};
             }
         }
+    };
+    auto values = [&](u32x4 from, float (&x)[VEC]) {
+        S s[VEC];
+        __builtin_memcpy(s, &from, 16);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = T::load(s[e]);
+    };
+    int64_t u0 = unit0 + 64 * wave;
+    if (u0 < unit1) load(u0);
+    if constexpr (TOP) {
+        // The k-th largest of the lanes' maxima is at most the k-th largest element.
+        uint32_t most = 0;
+        if (u0 < unit1) {
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) {
+                float x[VEC];
+                values(raw[k], x);
+                float top = x[0];
+#pragma unroll
+                for (int e = 1; e < VEC; ++e) top = __builtin_elementwise_maximum(top, x[e]);
+                if (u0 + kStride * k + lane < unit1) most = max(most, order_of(top));
+            }
+        }
+        publish(sorted(most));
+        __syncthreads();
+    }
+    if (split == 0 && wave == 0 && head > 0) lone(lane < head ? lane : 0, lane < head);
+    while (u0 < unit1) {
+        if constexpr (TOP) look();
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k) {
-            const int64_t u = u0 + 64 * kWaves * k + lane;
-            if (u - lane >= unit1) break;
-            if (u - lane + 64 > unit1 && u >= unit1) raw[k] = u32x4{T::kNone, T::kNone, T::kNone, T::kNone};
-            S s[VEC];
-            __builtin_memcpy(s, &raw[k], 16);
+            const int64_t u = u0 + kStride * k + lane;
             float x[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) x[e] = T::load(s[e]);
-            process(x, head + u * VEC, u < unit1 ? VEC : 0);
+            values(raw[k], x);
+            process(x, head + u * VEC, u < unit1, std::integral_constant<int, VEC>());
         }
+        u0 += kStride * kUnroll;
+        if (u0 < unit1) load(u0);
     }
     const int64_t rest = head + units * VEC;
     if (split == p.splits - 1 && wave == kWaves - 1 && rest < p.vocab) {
         lone(rest + lane < p.vocab ? rest + lane : rest, rest + lane < p.vocab);
     }
     if constexpr (TOP) tops.flush();
-    const Sums all = join<TOP>(joined, tops, sums, p.top);
+    const Sums all = join<TOP>(joined, tops, sums);
     if (p.splits == 1) {
-        finish<T, TOP>(p, i, row, all, joined.list);
+        finish<T, TOP>(p, i, row, all, tops.best);
         return;
     }
     if (threadIdx.x == 0) {
@@ -434,7 +523,7 @@ logprobs_kernel(const LogprobParams p) {
         to[2] = all.e;
     }
     if constexpr (TOP) {
-        if (threadIdx.x < p.top) p.ws_top[static_cast<int64_t>(blockIdx.x) * p.top + threadIdx.x] = joined.list[threadIdx.x];
+        if (threadIdx.x < p.top) p.ws_top[static_cast<int64_t>(blockIdx.x) * p.top + threadIdx.x] = tops.best;
     }
 }
 
@@ -465,8 +554,8 @@ logprobs_join_kernel(const LogprobParams p) {
         }
         tops.flush();
     }
-    const Sums all = join<TOP>(joined, tops, sums, p.top);
-    finish<T, TOP>(p, i, row, all, joined.list);
+    const Sums all = join<TOP>(joined, tops, sums);
+    finish<T, TOP>(p, i, row, all, tops.best);
 }
 
 // Parts of a row: the chip holds some 2048 of these workgroups; a part is at least 4 units a thread.
