@@ -33,7 +33,7 @@
 //
 // 32 query heads over 8 KV heads of 128, bf16: 64 trees of 64 nodes over 8192 keys each are bound by the matrix
 // units, 725 us at 0.76 PFLOP/s (keys through registers, and a reach test and a bias read for every score,
-// took 1302); 128 single tokens over 4096 keys by memory, 398 us at 5.4 TB/s (484).
+// took 1302); 128 single tokens over 4096 keys by memory, 385 us at 5.6 TB/s (484).
 //
 // A probability is rounded to the operands' type once where the result is of that type, and kept in
 // more terms for fp32 results (bf16: 3, to 2^-26; f16: 2, to 2^-23).  f16 probabilities are held times
@@ -350,7 +350,7 @@ __device__ __forceinline__ void win_store4(const WindowParams& p, int64_t row, i
 }
 
 template <int D, int WM, int WK, int SK, int NBUF, class T, int TERMS>
-__global__ void __launch_bounds__(64 * WM * WK, D == 256 || WK == 4 ? 1 : 2)
+__global__ void __launch_bounds__(64 * WM * WK, D == 256 || (D == 128 && WM == 1) ? 1 : 2)
 window_attention_kernel(const WindowParams p) {
     constexpr int THREADS = 64 * WM * WK, ROWS = 32 * WM;
     constexpr int LPR = D / 8;                     // lanes that move one key's row
@@ -362,7 +362,7 @@ window_attention_kernel(const WindowParams p) {
     constexpr float kShift = WinType<T>::kShift;
     const float kOver = __builtin_amdgcn_exp2f(8.0f + kShift);
     constexpr int AHEAD = WK == 1 ? 3 : NBUF;      // steps between a step's loads and its products
-    constexpr int KT = WM == 8 || WK == 4 ? 512 : 256;   // keys of a table
+    constexpr int KT = WM == 8 ? 512 : 256;   // keys of a table
     constexpr int TSTEPS = KT / SK;                // steps of a table
     constexpr int KBYTES = KT / 8, KTILES = KT / kWinTile;
     constexpr int NODES = ROWS < 128 ? ROWS : 128;       // at most, of a block: 256 rows have two heads a node or more
@@ -436,8 +436,9 @@ window_attention_kernel(const WindowParams p) {
     const int32_t t0 = req.prefix < p.sinks || from_low <= req.prefix ? 0 : from_low - req.prefix;
     const int32_t n_keys = n_prefix + (node1 + 1 - t0);
     const int steps = (n_keys + SK - 1) / SK;
-    const int run0 = static_cast<int>(static_cast<int64_t>(steps) * split / p.splits);
-    const int run1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / p.splits);
+    const int part = steps / p.splits, longer = steps - part * p.splits;   // the first parts have a step more
+    const int run0 = split * part + (split < longer ? split : longer);
+    const int run1 = run0 + part + (split < longer ? 1 : 0);
     const int64_t piece = (static_cast<int64_t>(id) * p.num_kv_heads + head) * p.splits + split;
     if (run0 >= run1) {   // fewer steps than workgroups
         for (int i = tid; i < ROWS; i += THREADS) p.ws_ml[piece * ROWS + i] = make_float2(-INFINITY, 0.0f);
