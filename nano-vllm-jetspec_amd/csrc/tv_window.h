@@ -13,9 +13,9 @@
 // this order, are its work, in steps of SK.  Pages outside are never looked up.
 //
 // A workgroup takes one row block (ROWS score rows of one request and KV head), or an equal part of its
-// steps where the batch has too few blocks for the chip; a second launch joins the parts.  Every workgroup
-// finds its block from the live lengths by a sum over the requests' blocks, so no plan is needed; blocks that
-// are not there come last in the launch, since they are what balances it when they lie between others
+// steps where the batch has too few blocks for the chip (win_parts); a second launch joins the parts.  Every
+// workgroup finds its block from the live lengths by a sum over the requests' blocks, so no plan is needed;
+// blocks that are not there come last in the launch, since they are what balances it when they lie between others
 // (every second one missing kept half of the shader engines idle, at twice the time).
 //
 // A key's page, place and reach are looked up once, a thread a key, into tables of 256 or 512 keys in LDS,
@@ -80,7 +80,9 @@ struct WindowParams {
     int32_t window, sinks;
     float c;                       // scale * log2(e)
     int32_t block_ids;             // numbers that row blocks can have
-    int32_t splits;                // workgroups a row block
+    int32_t units;                 // workgroups of a KV head
+    int32_t splits;                // of a row block, if each has as many
+    int32_t least_steps;           // of a part
     int32_t row_slots;             // the merge gives a row a group of lanes, not a workgroup
     float* ws_o;
     float2* ws_ml;
@@ -149,17 +151,63 @@ __device__ __forceinline__ WinRequest win_request(const WindowParams& p, int r, 
     return q;
 }
 
-// A row block: its request, and its place among the request's blocks.
+// A row block: its request, its place among the request's blocks, the parts that its keys are cut into, the first
+// part's number among those of all blocks, and the part that was asked for.
 struct WinBlock {
-    int32_t r, b;
+    int32_t r, b, parts, first, split;
     WinRequest req;
 };
 
-// Counts the batch's row blocks, blocks of a request and requests following each other, and finds number
-// pick(count); false if that is no block.  All threads of the workgroup call it; `scratch` is LDS of its own, 3 + a
-// word a wave.
-template <int ROWS, int THREADS, class PICK>
-__device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch, WinBlock& block, PICK pick) {
+// Sum over the wave's lanes, in all of them.
+__device__ __forceinline__ int32_t win_wave_sum(int32_t v) {
+    v += __builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, false);    // quad_perm [1, 0, 3, 2]
+    v += __builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, false);    // quad_perm [2, 3, 0, 1]
+    v += __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, false);   // half row mirrored
+    v += __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, false);   // row mirrored
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = static_cast<int32_t>(r[0] + r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return static_cast<int32_t>(h[0] + h[1]);
+}
+
+// Inclusive sums over the wave's lanes: within rows of 16, then from row to row.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int32_t win_shifted(int32_t v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
+}
+__device__ __forceinline__ int32_t win_wave_scan(int32_t v) {
+    v += win_shifted<0x111, 0xf>(v);   // row_shr by 1, 2, 4, 8
+    v += win_shifted<0x112, 0xf>(v);
+    v += win_shifted<0x114, 0xf>(v);
+    v += win_shifted<0x118, 0xf>(v);
+    v += win_shifted<0x142, 0xa>(v);   // lane 15 of the row before to rows 1 and 3
+    v += win_shifted<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
+    return v;
+}
+
+// Parts that a request's row blocks are cut into, a lane per request: one each, and the workgroups that are left
+// over by their keys, but no part shorter than the least.  All in integers: the merge has to find the same.
+constexpr int32_t kMostSplits = 64;
+template <int ROWS, int SK>
+__device__ __forceinline__ int32_t win_parts(const WindowParams& p, const WinRequest& q) {
+    if (p.splits == 1) return 1;
+    // Keys of a block, about: all that there are, or what its window spans and its own nodes.
+    const int64_t own = q.nodes < ROWS ? q.nodes : ROWS, all = static_cast<int64_t>(q.prefix) + q.nodes;
+    const int64_t most = static_cast<int64_t>(p.window) + p.sinks + own, keys = all < most ? all : most;
+    const int32_t steps = keys < (SK << 14) ? static_cast<int32_t>(keys + SK - 1) / SK : 1 << 14;   // sums stay below 2^31
+    const int32_t total = win_wave_sum(q.blocks * steps), left = p.units - win_wave_sum(q.blocks);
+    int32_t parts = total > 0 && left > 0 ? static_cast<int32_t>(static_cast<uint32_t>(steps) * left / total) + 1 : 1;
+    const int32_t limit = p.least_steps == 1 ? steps : steps / p.least_steps;
+    parts = parts < limit ? parts : limit;
+    parts = parts < kMostSplits ? parts : kMostSplits;
+    return parts > 1 ? parts : 1;
+}
+
+// Finds part `unit` (BY_PART) of the batch's row blocks, or their block number `unit`: blocks of a request and requests
+// follow each other; false if there is none.  All threads of the workgroup call it; `scratch` is LDS of its own, 3 +
+// a word a wave.
+template <int ROWS, int SK, int THREADS, bool BY_PART>
+__device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch, WinBlock& block, int unit) {
     constexpr int WAVES = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // The last workgroup of a launch reports what is wrong with the requests.
@@ -172,18 +220,24 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch
             q = win_request<ROWS>(p, lane, bad);
             if (bad && report) set_status(p.status, TV_STATUS_BAD_REQUEST);
         }
-        int32_t end = q.blocks;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int32_t y = __shfl_up(end, o);
-            if (lane >= o) end += y;
-        }
-        const int id = pick(__builtin_amdgcn_readlane(end, 63));
-        if (id < 0) return false;
-        const uint64_t behind = __ballot(end > id);
+        const int32_t parts = win_parts<ROWS, SK>(p, q), mine = q.blocks * parts, end = win_wave_scan(mine);
+        const int32_t found = BY_PART || p.splits == 1 ? end : win_wave_scan(q.blocks);
+        const uint64_t behind = __ballot(found > unit);
+        if (behind == 0) return false;
         const int r = __ffsll(static_cast<unsigned long long>(behind)) - 1;
         block.r = r;
-        block.b = id - __builtin_amdgcn_readlane(end - q.blocks, r);
+        block.parts = __builtin_amdgcn_readlane(parts, r);
+        const int32_t first = __builtin_amdgcn_readlane(end - mine, r);
+        if constexpr (BY_PART) {
+            block.b = (unit - first) / block.parts;
+            block.split = unit - first - block.b * block.parts;
+        } else {
+            block.b = unit - __builtin_amdgcn_readlane(found - q.blocks, r);
+            block.split = 0;
+        }
+        block.first = first + block.b * block.parts;
+        // Requests that overlap can have more blocks than rows have.
+        if (block.first + block.parts > p.units) return false;
         block.req.prefix = __builtin_amdgcn_readlane(q.prefix, r);
         block.req.nodes = __builtin_amdgcn_readlane(q.nodes, r);
         block.req.first_row = __builtin_amdgcn_readlane(q.first_row, r);
@@ -199,12 +253,7 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch
         mine += win_request<ROWS>(p, i, bad).blocks;
         if (bad && report) set_status(p.status, TV_STATUS_BAD_REQUEST);
     }
-    int32_t end = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int32_t y = __shfl_up(end, o);
-        if (lane >= o) end += y;
-    }
+    int32_t end = win_wave_scan(mine);
     if (lane == 63) scratch[3 + wave] = end;
     __syncthreads();
     int32_t total = 0;
@@ -213,8 +262,8 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch
         if (w < wave) end += scratch[3 + w];
         total += scratch[3 + w];
     }
-    const int id = pick(__builtin_amdgcn_readfirstlane(total));
-    if (id < 0) return false;   // the same in every thread
+    const int id = BY_PART ? unit / p.splits : unit;
+    if (id >= __builtin_amdgcn_readfirstlane(total)) return false;   // the same in every thread
     if (end - mine <= id && id < end) {   // this thread's requests hold it
         int32_t first = end - mine;
         for (int i = r0; i < r1; ++i) {
@@ -231,6 +280,9 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch
     block.r = __builtin_amdgcn_readfirstlane(scratch[0]);
     block.b = __builtin_amdgcn_readfirstlane(scratch[1]);
     block.req = win_request<ROWS>(p, block.r, bad);
+    block.parts = p.splits;
+    block.first = id * p.splits;
+    block.split = unit - (BY_PART ? block.first : unit);
     return true;
 }
 
@@ -391,19 +443,12 @@ window_attention_kernel(const WindowParams p) {
     const int c = lane & 31, half = lane >> 5;
 
     // --- the row block and its keys -------------------------------------------------------------
-    // Workgroups are dealt to the 8 XCDs in turn, so of 8 KV heads each has one, whose row blocks share its L2.  Runs of
+    // Heads fastest: workgroups are dealt to the 8 XCDs in turn, so of 8 KV heads each has one, whose row blocks share its L2.  Runs of
     // whole requests on an XCD gained nothing (64 trees over windows of 8192: 881 us and 889), and lose balance (8 ragged
     // requests: 116 us and 75).
-    int id = 0, head = 0, split = 0;
     WinBlock block;
-    const bool any = win_find<ROWS, THREADS>(p, lds_find, block, [&](int blocks) {
-        const int unit = blockIdx.x / p.num_kv_heads;
-        head = blockIdx.x - unit * p.num_kv_heads;
-        id = unit / p.splits;
-        split = unit - id * p.splits;
-        return id < blocks ? id : -1;
-    });
-    if (!any) return;
+    const int unit = blockIdx.x / p.num_kv_heads, head = blockIdx.x - unit * p.num_kv_heads;
+    if (!win_find<ROWS, SK, THREADS, true>(p, lds_find, block, unit)) return;
     const int r = block.r, b = block.b;
     const WinRequest req = block.req;
     const int rows_all = req.nodes * p.groups;
@@ -436,10 +481,10 @@ window_attention_kernel(const WindowParams p) {
     const int32_t t0 = req.prefix < p.sinks || from_low <= req.prefix ? 0 : from_low - req.prefix;
     const int32_t n_keys = n_prefix + (node1 + 1 - t0);
     const int steps = (n_keys + SK - 1) / SK;
-    const int part = steps / p.splits, longer = steps - part * p.splits;   // the first parts have a step more
+    const int split = block.split, part = steps / block.parts, longer = steps - part * block.parts;   // the first have a step more
     const int run0 = split * part + (split < longer ? split : longer);
     const int run1 = run0 + part + (split < longer ? 1 : 0);
-    const int64_t piece = (static_cast<int64_t>(id) * p.num_kv_heads + head) * p.splits + split;
+    const int64_t piece = static_cast<int64_t>(block.first) * p.num_kv_heads + head * block.parts + split;
     if (run0 >= run1) {   // fewer steps than workgroups
         for (int i = tid; i < ROWS; i += THREADS) p.ws_ml[piece * ROWS + i] = make_float2(-INFINITY, 0.0f);
         return;
@@ -880,7 +925,7 @@ window_attention_kernel(const WindowParams p) {
     }
 
     // --- the result: the row's output, or its unnormalised sum with (m, l) for the merge ---------
-    const bool whole = p.splits == 1;
+    const bool whole = block.parts == 1;
     auto put = [&](int row_in_block, int row_node, int row_head, int dim, win_f32x4 v, float row_l) {
         if (whole) {
             const float scale = row_l == 0.0f ? 0.0f : 1.0f / row_l;   // a row that sees nothing is zero
@@ -948,7 +993,7 @@ window_attention_kernel(const WindowParams p) {
 
 template <int D, int WM, int WK, int SK, int NBUF>
 void win_launch(const WindowParams& p, bool bf16, hipStream_t s) {
-    const dim3 grid(static_cast<uint32_t>(p.block_ids) * p.splits * p.num_kv_heads), block(64 * WM * WK);
+    const dim3 grid(static_cast<uint32_t>(p.units) * p.num_kv_heads), block(64 * WM * WK);
     if (bf16 && !p.out_f32) hipLaunchKernelGGL((window_attention_kernel<D, WM, WK, SK, NBUF, __bf16, 1>), grid, block, 0, s, p);
     else if (bf16) hipLaunchKernelGGL((window_attention_kernel<D, WM, WK, SK, NBUF, __bf16, 3>), grid, block, 0, s, p);
     else if (!p.out_f32) hipLaunchKernelGGL((window_attention_kernel<D, WM, WK, SK, NBUF, _Float16, 1>), grid, block, 0, s, p);

@@ -6,7 +6,6 @@ namespace tv {
 namespace {
 
 constexpr int kMergeThreads = 256;
-constexpr int kMostSplits = 64;
 constexpr int kLongRun = 1024;       // keys of a block, from which on 256 rows pay
 constexpr int kFewPieces = 4, kManyRows = 4096;
 constexpr int kMergeGroups = 2048;   // workgroups of the merge, about
@@ -15,7 +14,7 @@ constexpr int kLeastKeys = 128;      // that a part of a block's keys is cut to
 constexpr float kMaxScale = 2.3e38f;
 
 // Joins the pieces of a row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m).
-template <int D, int ROWS, class T>
+template <int D, int ROWS, int SK, class T>
 __global__ void __launch_bounds__(kMergeThreads)
 window_merge_kernel(const WindowParams p) {
     constexpr int CH = D / 4, kSlots = kMergeThreads / CH;
@@ -25,11 +24,12 @@ window_merge_kernel(const WindowParams p) {
     const int tid = threadIdx.x, ch = tid % CH, slot = tid / CH;
     const int id = blockIdx.x / p.num_kv_heads, head = blockIdx.x - id * p.num_kv_heads;
     WinBlock block;
-    if (!win_find<ROWS, kMergeThreads>(p, find, block, [&](int blocks) { return id < blocks ? id : -1; })) return;
+    if (!win_find<ROWS, SK, kMergeThreads, false>(p, find, block, id) || block.parts == 1) return;
     const int b = block.b;
     const WinRequest req = block.req;
     const int row0 = b * ROWS, left = req.nodes * p.groups - row0, rows = left < ROWS ? left : ROWS;
-    const int64_t piece0 = static_cast<int64_t>(blockIdx.x) * p.splits;
+    const int64_t piece0 = static_cast<int64_t>(block.first) * p.num_kv_heads + head * block.parts;
+    const int splits = block.parts;
     float best, sum;
     win_f32x4 v;
     // Pieces i0, i0 + step, ... of a row.
@@ -37,12 +37,12 @@ window_merge_kernel(const WindowParams p) {
         best = -INFINITY;
         sum = 0.0f;
         v = win_f32x4{0, 0, 0, 0};
-        for (; i0 < p.splits; i0 += 4 * step) {
+        for (; i0 < splits; i0 += 4 * step) {
             float2 ml[4];
             win_f32x4 o[4];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                const int i = i0 + n * step < p.splits ? i0 + n * step : i0;
+                const int i = i0 + n * step < splits ? i0 + n * step : i0;
                 const int64_t of = (piece0 + i) * ROWS + row;
                 ml[n] = p.ws_ml[of];
                 o[n] = *reinterpret_cast<const win_f32x4*>(p.ws_o + of * D + 4 * ch);
@@ -57,7 +57,7 @@ window_merge_kernel(const WindowParams p) {
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 // A piece without steps has written no sums.
-                if (i0 + n * step >= p.splits || ml[n].y == 0.0f) continue;
+                if (i0 + n * step >= splits || ml[n].y == 0.0f) continue;
                 const float f = win_weight(ml[n], best);
                 sum += f * ml[n].y;
                 v += f * o[n];
@@ -98,7 +98,7 @@ window_merge_kernel(const WindowParams p) {
     }
 }
 
-template <int D, int ROWS>
+template <int D, int ROWS, int SK>
 void launch_merge(const WindowParams& p, bool bf16, hipStream_t s) {
     constexpr int kSlots = kMergeThreads / (D / 4);
     const int64_t blocks = static_cast<int64_t>(p.block_ids) * p.num_kv_heads;
@@ -106,23 +106,24 @@ void launch_merge(const WindowParams& p, bool bf16, hipStream_t s) {
     int64_t parts = (kMergeGroups + blocks - 1) / blocks;
     parts = parts < most ? parts : most;
     const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(parts));
-    if (bf16) hipLaunchKernelGGL((window_merge_kernel<D, ROWS, __bf16>), grid, dim3(kMergeThreads), 0, s, p);
-    else hipLaunchKernelGGL((window_merge_kernel<D, ROWS, _Float16>), grid, dim3(kMergeThreads), 0, s, p);
+    if (bf16) hipLaunchKernelGGL((window_merge_kernel<D, ROWS, SK, __bf16>), grid, dim3(kMergeThreads), 0, s, p);
+    else hipLaunchKernelGGL((window_merge_kernel<D, ROWS, SK, _Float16>), grid, dim3(kMergeThreads), 0, s, p);
 }
 
 template <int D>
 void launch_merge_d(const WindowParams& p, int rows, bool bf16, hipStream_t s) {
-    if (rows == 32) launch_merge<D, 32>(p, bf16, s);
-    else if (rows == 64) launch_merge<D, 64>(p, bf16, s);
-    else if (rows == 128) launch_merge<D, 128>(p, bf16, s);
-    else launch_merge<D, 256>(p, bf16, s);
+    if (rows == 32) launch_merge<D, 32, 64>(p, bf16, s);
+    else if (rows == 64) launch_merge<D, 64, 64>(p, bf16, s);
+    else if (rows == 128) launch_merge<D, 128, 32>(p, bf16, s);
+    else launch_merge<D, 256, 64>(p, bf16, s);
 }
 
 struct Launch {
     WindowShape shape;
     int32_t width;     // of the head-size template
     int64_t block_ids;
-    int32_t splits;
+    int64_t units;     // workgroups of a KV head
+    int32_t splits, least_steps;
     int64_t bytes;     // of the workspace
 };
 
@@ -149,11 +150,22 @@ Launch launch_of(const tv_window_attention_args* a) {
     blocks = (blocks > a->num_requests ? blocks : a->num_requests) * a->num_kv_heads;
     const int64_t least = n.shape.step > kLeastKeys ? n.shape.step : kLeastKeys;
     const int64_t most = (keys + least - 1) / least;
-    int64_t splits = static_cast<int64_t>(a->compute_units) * n.shape.per_cu / blocks;
+    const int64_t room = static_cast<int64_t>(a->compute_units) * n.shape.per_cu;
+    int64_t splits = room / blocks;
     splits = splits < most ? splits : most;
     splits = splits < kMostSplits ? splits : kMostSplits;
     n.splits = static_cast<int32_t>(splits > 1 ? splits : 1);
-    n.bytes = n.splits == 1 ? 0 : n.block_ids * a->num_kv_heads * n.splits * n.shape.rows * (n.width * 4ll + 8);
+    n.least_steps = static_cast<int32_t>(least / n.shape.step);
+    // The parts are dealt out on the device, by the lengths there; a block takes one at least, and as many as its keys
+    // allow at most.  32 query heads over 8 KV heads of 128, as many parts for every block in brackets: 8 requests of 40
+    // nodes over 4096 keys 66 us (80), 4 of 8 to 60 nodes over 100 to 8192 keys 53 (61).
+    n.units = n.block_ids * n.splits;
+    if (n.splits > 1 && a->num_requests <= 64) {
+        n.units = n.block_ids * (most < kMostSplits ? most : kMostSplits);
+        n.units = n.units < room / a->num_kv_heads ? n.units : room / a->num_kv_heads;
+        n.units = n.units > n.block_ids ? n.units : n.block_ids;
+    }
+    n.bytes = n.splits == 1 ? 0 : n.units * a->num_kv_heads * n.shape.rows * (n.width * 4ll + 8);
     return n;
 }
 
@@ -186,7 +198,7 @@ int check(const tv_window_attention_args* a) {
     if (a->num_requests > 0 && a->total_queries > 0) {
         const Launch n = launch_of(a);
         // A launch has fewer than 2^32 threads.
-        if (n.block_ids * n.splits > 0xffffffffll / n.shape.threads / a->num_kv_heads) {
+        if (n.units > 0xffffffffll / n.shape.threads / a->num_kv_heads) {
             return fail(TV_ERR_UNSUPPORTED, "%s: too many row blocks", what);
         }
     }
@@ -280,11 +292,13 @@ extern "C" int tv_window_attention(const tv_window_attention_args* a, void* work
     p.sinks = a->sinks;
     p.c = a->scale * 1.44269504088896340736f;
     p.block_ids = static_cast<int32_t>(n.block_ids);
+    p.units = static_cast<int32_t>(n.units);
     p.splits = n.splits;
+    p.least_steps = n.least_steps;
     // A group of lanes joins a row where there are rows for all, or few pieces; else a workgroup does.
     p.row_slots = n.splits <= kFewPieces || static_cast<int64_t>(a->total_queries) * a->num_q_heads >= kManyRows;
     if (n.bytes) {
-        const int64_t pieces = n.block_ids * a->num_kv_heads * n.splits * n.shape.rows;
+        const int64_t pieces = n.units * a->num_kv_heads * n.shape.rows;
         p.ws_o = static_cast<float*>(workspace);
         p.ws_ml = reinterpret_cast<float2*>(p.ws_o + pieces * n.width);
     }
