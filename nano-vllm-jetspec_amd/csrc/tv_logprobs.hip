@@ -9,17 +9,17 @@
 //
 // The top k: a wave keeps the 64 largest it has seen, sorted, a lane each, and a queue in LDS.  What does
 // not pass the k-th of them, which per 16-byte unit is one comparison with the unit's maximum, is done with;
-// the rest is queued, and a full queue is sorted and merged (bitonic).  The first bound is the k-th largest
-// of the lanes' maxima over the first units.  A wave's elements come in the order of their indices, so a
+// other units are queued, and when there are 64 what still passes is sorted and merged (bitonic).  The first bound is
+// the k-th largest of the lanes' maxima over the first units, and all waves of a row share theirs.  A wave's elements come in the order of their indices, so a
 // later one of equal value never counts, and the waves' lists are joined by their order as 64-bit numbers,
 // value before index: the result depends on no timing.
 //
-// Memory bounds it where logits are plenty (the logits are read once); the vector unit is close behind:
-// about ten instructions an element for 16-bit logits, of which the exponential takes four slots.
+// Memory bounds it where no alternatives are asked for (4096 rows of 151936 bf16 logits, 1.25 GB: 197 us, 6.3 TB/s);
+// the vector unit is as busy, ten instruction slots an element, of which the exponential takes four, and bounds it
+// with 20 alternatives (226 us; 316 with every element of a unit looked at where one passes, exchanges through LDS
+// and bounds of a wave's own).  8 rows with 5: 14 us, two launches' latencies.
 #include <math.h>
 #include <stdint.h>
-
-#include <type_traits>
 
 #include "tv_internal.h"
 
@@ -29,7 +29,6 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kUnroll = 4;      // units a lane loads at a time
 constexpr int kMostTop = 64;
-constexpr int kFull = 32;       // entries of a wave's queue that are merged into its list
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kMargin = 8.0f;
 // R is c x rounded to fp32, and c x - R has to stay near zero for the x it was made of: so up to 2^16.  Larger
@@ -173,20 +172,28 @@ __device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) {
     return static_cast<uint64_t>(of_lane(static_cast<uint32_t>(v >> 32), lane)) << 32 | of_lane(static_cast<uint32_t>(v), lane);
 }
 
+// How many of `lanes` lie before this one.
+__device__ __forceinline__ int lanes_before(uint64_t lanes) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0));
+}
+
 // A wave's largest entries.  Entries are distinct, but for the empty one, 0.
 struct WaveTop {
     uint64_t best = 0;     // sorted over the lanes
     uint64_t kth = 0;      // the top-th of them
-    uint64_t* queue;       // LDS of the wave's own
+    uint64_t* queue;       // LDS of the wave's own: fewer than 64, and a push of up to 64
     int queued = 0, top;
 
-    // Merges the last 64 entries of the queue.
-    __device__ __forceinline__ void flush() {
-        const int lane = threadIdx.x & 63, from = queued > 64 ? queued - 64 : 0;
-        // One wave's exchange: its LDS operations run in order, the compiler's must too.
+    // One wave's exchange through LDS: its operations run in order, the compiler's must too.
+    static __device__ __forceinline__ void settle() {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    // Merges the last 64 entries of the queue.
+    __device__ __forceinline__ void flush() {
+        const int lane = threadIdx.x & 63, from = queued > 64 ? queued - 64 : 0;
+        settle();
         const uint64_t mine = from + lane < queued ? queue[from + lane] : 0;
         queued = from;
         merge(sorted(mine));
@@ -200,11 +207,7 @@ struct WaveTop {
     __device__ __forceinline__ void push(bool want, uint64_t entry) {
         const uint64_t lanes = __ballot(want);
         if (lanes == 0) return;
-        if (want) {
-            const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
-                                                         __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0));
-            queue[queued + before] = entry;
-        }
+        if (want) queue[queued + lanes_before(lanes)] = entry;
         queued += __popcll(lanes);
     }
 };
@@ -352,7 +355,10 @@ logprobs_kernel(const LogprobParams p) {
     typedef typename T::storage S;
     constexpr int VEC = 16 / sizeof(S);
     __shared__ Joined joined;
-    __shared__ uint64_t queues[kWaves][TOP ? 64 * (VEC + 1) : 1];
+    __shared__ uint64_t queues[kWaves][TOP ? 128 : 1];
+    // Units with a candidate in them: fewer than 64, and those of a step.
+    __shared__ u32x4 unit_of[kWaves][TOP ? 128 : 1];
+    __shared__ int32_t unit_at[kWaves][TOP ? 128 : 1];
     // A wave reads what others have written so far.
     __shared__ volatile uint32_t shared_full[kWaves], shared_quarter[kWaves];
     const int64_t i = blockIdx.x / p.splits;
@@ -402,8 +408,39 @@ logprobs_kernel(const LogprobParams p) {
         most = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(max(most, least))));
         if (most > 0) raise_pass(most - 1);
     };
-    // A lane's `count` elements x (the others -inf), the first of which has index `first`; all -inf where it is not live.
-    auto process = [&](const float (&x)[VEC], int64_t first, bool live, auto count) {
+    auto values = [&](u32x4 from, float (&x)[VEC]) {
+        S s[VEC];
+        __builtin_memcpy(s, &from, 16);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = T::load(s[e]);
+    };
+    int units_queued = 0;
+    auto merge_queue = [&]() {
+        tops.flush();
+        // This wave's elements to come have higher indices, so an equal value is not enough.
+        raise_pass(static_cast<uint32_t>(tops.kth >> 32));
+        publish(tops.best);
+    };
+    // The elements of all queued units that are candidates yet, to the list; the bound stays until all are through.
+    auto expand = [&]() {
+        WaveTop::settle();
+        for (int u0 = 0; u0 < units_queued; u0 += 64) {
+            const bool live = u0 + lane < units_queued;
+            const int at = live ? u0 + lane : 0;
+            const int64_t first = head + static_cast<int64_t>(unit_at[wave][at]) * VEC;
+            float x[VEC];
+            values(unit_of[wave][at], x);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                tops.push(live && !(x[e] <= bound), entry_of(x[e], first + e));
+                if (tops.queued >= 64) tops.flush();
+            }
+        }
+        units_queued = 0;
+        merge_queue();
+    };
+    // A lane's elements x; `found` gets those of lanes that are `live` and can be among the largest.
+    auto process = [&](const float (&x)[VEC], bool live, auto found) {
         float most = x[0];
 #pragma unroll
         for (int e = 1; e < VEC; ++e) most = __builtin_elementwise_maximum(most, x[e]);   // NaN where one is
@@ -418,18 +455,7 @@ logprobs_kernel(const LogprobParams p) {
                     limit = most + kMargin;
                 }
             }
-            if constexpr (TOP) {
-                if (__any(candidate)) {
-#pragma unroll
-                    for (int e = 0; e < decltype(count)::value; ++e) tops.push(live && !(x[e] <= bound), entry_of(x[e], first + e));
-                    if (tops.queued >= kFull) {
-                        while (tops.queued >= kFull) tops.flush();
-                        // This wave's elements to come have higher indices, so an equal value is not enough.
-                        raise_pass(static_cast<uint32_t>(tops.kth >> 32));
-                        publish(tops.best);
-                    }
-                }
-            }
+            if constexpr (TOP) found(live && candidate);
         }
         float z[VEC], z_e[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -451,7 +477,10 @@ logprobs_kernel(const LogprobParams p) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) x[e] = -INFINITY;
         if (live) x[0] = T::load(base[index]);
-        process(x, index, live, std::integral_constant<int, 1>());
+        process(x, live, [&](bool candidate) {
+            tops.push(candidate, entry_of(x[0], index));
+            if (tops.queued >= 64) merge_queue();
+        });
     };
     constexpr int kStride = 64 * kWaves;    // units between a lane's
     u32x4 raw[kUnroll];
@@ -467,12 +496,6 @@ logprobs_kernel(const LogprobParams p) {
                 if (u0 + kStride * k + lane >= unit1) raw[k] = u32x4{T::kNone, T::kNone, T::kNone, T::kNone};
             }
         }
-    };
-    auto values = [&](u32x4 from, float (&x)[VEC]) {
-        S s[VEC];
-        __builtin_memcpy(s, &from, 16);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[e] = T::load(s[e]);
     };
     int64_t u0 = unit0 + 64 * wave;
     if (u0 < unit1) load(u0);
@@ -501,11 +524,21 @@ logprobs_kernel(const LogprobParams p) {
             const int64_t u = u0 + kStride * k + lane;
             float x[VEC];
             values(raw[k], x);
-            process(x, head + u * VEC, u < unit1, std::integral_constant<int, VEC>());
+            process(x, u < unit1, [&](bool candidate) {
+                const uint64_t lanes = __ballot(candidate);
+                if (candidate) {
+                    const int at = units_queued + lanes_before(lanes);
+                    unit_of[wave][at] = raw[k];
+                    unit_at[wave][at] = static_cast<int32_t>(u);
+                }
+                units_queued += __popcll(lanes);
+                if (units_queued >= 64) expand();
+            });
         }
         u0 += kStride * kUnroll;
         if (u0 < unit1) load(u0);
     }
+    if constexpr (TOP) expand();
     const int64_t rest = head + units * VEC;
     if (split == p.splits - 1 && wave == kWaves - 1 && rest < p.vocab) {
         lone(rest + lane < p.vocab ? rest + lane : rest, rest + lane < p.vocab);
