@@ -33,7 +33,7 @@
 //
 // 32 query heads over 8 KV heads of 128, bf16: 64 trees of 64 nodes over 8192 keys each are bound by the matrix
 // units, 725 us at 0.76 PFLOP/s (keys through registers, and a reach test and a bias read for every score,
-// took 1302); 128 single tokens over 4096 keys by memory, 385 us at 5.6 TB/s (484).
+// took 1302); 128 single tokens over 4096 keys by memory, 376 us at 5.7 TB/s (484).
 //
 // A probability is rounded to the operands' type once where the result is of that type, and kept in
 // more terms for fp32 results (bf16: 3, to 2^-26; f16: 2, to 2^-23).  f16 probabilities are held times
@@ -89,7 +89,8 @@ struct WindowParams {
     int32_t* status;
 };
 
-// How a launch of average `rows` score rows per request and KV head is shaped.
+// How a launch is shaped: by the score rows of an average request and KV head, and by how many of these there are a
+// compute unit.
 struct WindowShape {
     int32_t rows;          // score rows of a row block
     int32_t threads;
@@ -97,9 +98,9 @@ struct WindowShape {
     int32_t step;          // keys of a step
 };
 
-WindowShape window_shape_d64(int64_t average_rows);
+WindowShape window_shape_d64(int64_t average_rows, int64_t per_cu);
 WindowShape window_shape_d128(int64_t average_rows);
-WindowShape window_shape_d256(int64_t average_rows);
+WindowShape window_shape_d256(int64_t average_rows, int64_t per_cu);
 void launch_window_d64(const WindowParams& p, const WindowShape& shape, bool bf16, hipStream_t s);
 void launch_window_d128(const WindowParams& p, const WindowShape& shape, bool bf16, hipStream_t s);
 void launch_window_d256(const WindowParams& p, const WindowShape& shape, bool bf16, hipStream_t s);
@@ -402,7 +403,7 @@ __device__ __forceinline__ void win_store4(const WindowParams& p, int64_t row, i
 }
 
 template <int D, int WM, int WK, int SK, int NBUF, class T, int TERMS>
-__global__ void __launch_bounds__(64 * WM * WK, D == 256 || (D == 128 && WM == 1) ? 1 : 2)
+__global__ void __launch_bounds__(64 * WM * WK, D == 256 ? 1 : 2)
 window_attention_kernel(const WindowParams p) {
     constexpr int THREADS = 64 * WM * WK, ROWS = 32 * WM;
     constexpr int LPR = D / 8;                     // lanes that move one key's row

@@ -112,10 +112,13 @@ void launch_merge(const WindowParams& p, bool bf16, hipStream_t s) {
 
 template <int D>
 void launch_merge_d(const WindowParams& p, int rows, bool bf16, hipStream_t s) {
-    if (rows == 32) launch_merge<D, 32, 64>(p, bf16, s);
-    else if (rows == 64) launch_merge<D, 64, 64>(p, bf16, s);
-    else if (rows == 128) launch_merge<D, 128, 32>(p, bf16, s);
-    else launch_merge<D, 256, 64>(p, bf16, s);
+    if constexpr (D != 128) {   // shapes of up to 32 rows are for more blocks than are cut
+        if (rows == 64) return launch_merge<D, 64, 64>(p, bf16, s);
+    }
+    if constexpr (D != 256) {
+        if (rows == 256) return launch_merge<D, 256, 64>(p, bf16, s);
+    }
+    launch_merge<D, 128, 32>(p, bf16, s);
 }
 
 struct Launch {
@@ -144,7 +147,10 @@ Launch launch_of(const tv_window_attention_args* a) {
     if (average > 128 && (groups == 1 || keys < kLongRun)) average = 128;
     Launch n;
     n.width = a->head_dim <= 64 ? 64 : a->head_dim <= 128 ? 128 : 256;
-    n.shape = n.width == 64 ? window_shape_d64(average) : n.width == 128 ? window_shape_d128(average) : window_shape_d256(average);
+    const int64_t per_cu = static_cast<int64_t>(a->num_requests) * a->num_kv_heads / a->compute_units;
+    n.shape = n.width == 64    ? window_shape_d64(average, per_cu)
+              : n.width == 128 ? window_shape_d128(average)
+                               : window_shape_d256(average, per_cu);
     n.block_ids = rows / n.shape.rows + a->num_requests;
     int64_t blocks = (rows + n.shape.rows - 1) / n.shape.rows;
     blocks = (blocks > a->num_requests ? blocks : a->num_requests) * a->num_kv_heads;
@@ -295,7 +301,8 @@ extern "C" int tv_window_attention(const tv_window_attention_args* a, void* work
     p.units = static_cast<int32_t>(n.units);
     p.splits = n.splits;
     p.least_steps = n.least_steps;
-    // A group of lanes joins a row where there are rows for all, or few pieces; else a workgroup does.
+    // A group of lanes joins a row where there are rows for all, or few pieces; else a workgroup does.  One request of 1 /
+    // 16 nodes over 8192 keys 19 / 28 us (with groups of lanes 30 / 39), 4 of 64 69 (with workgroups 82), 8 of 40 56 (66).
     p.row_slots = n.splits <= kFewPieces || static_cast<int64_t>(a->total_queries) * a->num_q_heads >= kManyRows;
     if (n.bytes) {
         const int64_t pieces = n.units * a->num_kv_heads * n.shape.rows;

@@ -3,10 +3,11 @@
 
 namespace tv {
 
-// Up to 32 rows: two workgroups of two waves and one buffer a compute unit; 44 single tokens over 5 keys, 128 over 512,
-// 48 and 16 over 4096: 16 / 132 / 317 / 115 us (64 rows, four waves, two buffers: 27 / 148 / 338 / 103).
-WindowShape window_shape_d256(int64_t average_rows) {
-    if (average_rows <= 32) return {32, 128, 2, 64};
+// Up to 32 rows: two workgroups of two waves and one buffer a compute unit where there are as many, else larger ones.
+// 100 trees of 4 nodes over 1024 keys and 8 KV heads 190 us, 64 single tokens over 512 57 (with 64 rows 214 and 64); 32
+// trees of 8 nodes over 4096 182, 32 single tokens over 512 33 (with 32 rows 264 and 44).
+WindowShape window_shape_d256(int64_t average_rows, int64_t per_cu) {
+    if (average_rows <= 32 && per_cu >= 2) return {32, 128, 2, 64};
     if (average_rows <= 64) return {64, 256, 1, 64};
     return {128, 256, 1, 32};
 }

@@ -3,11 +3,14 @@
 
 namespace tv {
 
-// Up to 32 rows: four workgroups of two waves a compute unit; 128 single tokens over 512 keys 34 us, 64 over 4096 118 us
-// (one of four waves with three buffers of 128 keys: 66 and 124).  From 129 rows on 256: 32 requests of 33 / 40 / 56
-// nodes and 4 heads a group over 4096 keys 112 / 114 / 128 us (with 128: 134 / 136 / 128).
-WindowShape window_shape_d64(int64_t average_rows) {
-    if (average_rows <= 32) return {32, 128, 4, 64};
+// Up to 32 rows: four workgroups of two waves a compute unit where there are as many, else larger ones, which have more
+// keys on their way.  128 single tokens over 512 keys and 8 KV heads 32 us, 200 trees of 4 nodes over 1024 106 (with 64
+// rows 40 and 117); 64 single tokens over 512 20, 64 trees of 8 nodes over 4096 114 (with 32 rows 26 and 149).
+// Up to 64: 64 trees of 16 nodes over 4096 115 (with 128 rows 130).
+// From 129 on 256: 32 requests of 33 / 40 / 56 nodes and 4 heads a group over 4096 112 / 114 / 128 us (with 128:
+// 134 / 136 / 128).
+WindowShape window_shape_d64(int64_t average_rows, int64_t per_cu) {
+    if (average_rows <= 32 && per_cu >= 4) return {32, 128, 4, 64};
     if (average_rows <= 64) return {64, 256, 2, 64};
     if (average_rows <= 128) return {128, 256, 2, 32};
     return {256, 512, 1, 64};

@@ -88,6 +88,23 @@ def test_every_shape_of_launch(dim):
         check(attend(b), b, f"{requests} {prefix} {window} {dim}")
 
 
+@pytest.mark.parametrize("dim, out", [(64, BF16), (64, F32), (128, BF16), (256, BF16), (256, F32)])
+def test_many_short_requests(dim, out):
+    # More blocks than the chip holds, of few rows.
+    sizes, prefixes = [1 + i % 4 for i in range(140)], [(37 * i) % 170 for i in range(140)]
+    b = Batch(prefixes, trees(sizes, 9), window=90, sinks=2, dim=dim, kv_heads=8, groups=2, seed=dim)
+    check(attend(b, output_dtype=out), b, f"{dim} {out}")
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_parts_of_unlike_requests(dim):
+    # Keys cut into parts by each request's length: up to 64 requests, above, and one long among short ones.
+    for prefixes, sizes in (([5000, 1, 700, 33], [3, 9, 40, 1]), ([0] * 20 + [6000] + [3] * 20, [2] * 41),
+                            ([300 + 13 * i for i in range(70)], [1 + i % 3 for i in range(70)]), ([9000, 9000], [150, 20])):
+        b = Batch(prefixes, trees(sizes, 11), window=4000, sinks=4, dim=dim, kv_heads=1, groups=4, page=32, seed=dim)
+        check(attend(b), b, f"{dim} {len(sizes)}")
+
+
 @pytest.mark.parametrize("page", [1, 16, 48])
 @pytest.mark.parametrize("groups", [1, 2, 3, 8])
 def test_long_blocks(groups, page):
