@@ -256,6 +256,7 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch
     }
     int32_t end = win_wave_scan(mine);
     if (lane == 63) scratch[3 + wave] = end;
+    if (tid == 0) scratch[0] = -1;
     __syncthreads();
     int32_t total = 0;
 #pragma unroll
@@ -279,6 +280,7 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch
     }
     __syncthreads();
     block.r = __builtin_amdgcn_readfirstlane(scratch[0]);
+    if (block.r < 0) return false;   // requests that overlap can have more blocks than are counted
     block.b = __builtin_amdgcn_readfirstlane(scratch[1]);
     block.req = win_request<ROWS>(p, block.r, bad);
     block.parts = p.splits;

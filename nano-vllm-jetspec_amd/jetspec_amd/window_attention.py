@@ -11,6 +11,7 @@ import torch
 
 from . import _device, _lib
 from .cache_e4m3 import _vector
+from .tree_fusion import _one_address_per_element, _share_bytes
 
 _MOST = 0x7fffffff
 
@@ -64,6 +65,8 @@ def packed_window_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     if out is not None:
         if out.shape != shape or out.dtype is not dtype or out.stride(2) != 1:
             raise ValueError("out must be [rows,heads,dim] in the output dtype, its last dimension contiguous")
+        if not _one_address_per_element(out) or any(_share_bytes(out, t) for t in (q, k_pool, v_pool, positions) if t.numel()):
+            raise ValueError("out must not overlap itself, the queries, the pools or the positions")
         index = _device.one_gpu("packed_window_attention", q, k_pool, v_pool, positions, out)
     else:
         index = _device.one_gpu("packed_window_attention", q, k_pool, v_pool, positions)

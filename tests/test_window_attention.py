@@ -46,6 +46,14 @@ def test_refuses(change, message):
         packed_window_attention(**(operands() | change))
 
 
+def test_refuses_outputs_that_overlap():
+    given = operands()
+    pool = given["k_pool"].view(-1)
+    for out in (given["q"], given["q"][:1].expand(4, 8, 64), pool[:2048].view(4, 8, 64)):
+        with pytest.raises(ValueError, match="out must"):
+            packed_window_attention(**given, out=out)
+
+
 @pytest.mark.parametrize("dim", [4, 20, 264, 512])
 def test_refuses_head_sizes(dim):
     with pytest.raises(ValueError, match="multiples of 8 up to 256"):
