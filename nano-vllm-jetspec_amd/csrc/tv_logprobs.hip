@@ -359,8 +359,9 @@ logprobs_kernel(const LogprobParams p) {
     // Units with a candidate in them: fewer than 64, and those of a step.
     __shared__ u32x4 unit_of[kWaves][TOP ? 128 : 1];
     __shared__ int32_t unit_at[kWaves][TOP ? 128 : 1];
-    // A wave reads what others have written so far.
-    __shared__ volatile uint32_t shared_full[kWaves], shared_quarter[kWaves];
+    // A wave reads what others have written so far.  (Relaxed accesses: through volatile ones the compiler goes by flat
+    // addresses, one at a time.)
+    __shared__ uint32_t shared_full[kWaves], shared_quarter[kWaves];
     const int64_t i = blockIdx.x / p.splits;
     const int split = static_cast<int>(blockIdx.x - i * p.splits);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -394,16 +395,16 @@ logprobs_kernel(const LogprobParams p) {
         const uint32_t full = static_cast<uint32_t>(of_lane(list, p.top - 1) >> kShift);
         const uint32_t quarter = static_cast<uint32_t>(of_lane(list, (p.top + kWaves - 1) / kWaves - 1) >> kShift);
         if (lane == 0) {
-            shared_full[wave] = full;
-            shared_quarter[wave] = quarter;
+            __hip_atomic_store(&shared_full[wave], full, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            __hip_atomic_store(&shared_quarter[wave], quarter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
     };
     auto look = [&]() {
-        uint32_t most = shared_full[0], least = shared_quarter[0];
+        uint32_t most = 0, least = 0xffffffffu;
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) {
-            most = max(most, static_cast<uint32_t>(shared_full[w]));
-            least = min(least, static_cast<uint32_t>(shared_quarter[w]));
+        for (int w = 0; w < kWaves; ++w) {
+            most = max(most, __hip_atomic_load(&shared_full[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+            least = min(least, __hip_atomic_load(&shared_quarter[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
         }
         most = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(max(most, least))));
         if (most > 0) raise_pass(most - 1);
