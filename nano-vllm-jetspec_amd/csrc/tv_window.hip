@@ -7,9 +7,9 @@ namespace {
 
 constexpr int kMergeThreads = 256;
 constexpr int kLongRun = 1024;       // keys of a block, from which on 256 rows pay
-constexpr int kFewPieces = 4, kManyRows = 4096;
+constexpr int kFewPieces = 8, kManyRows = 1024;
 constexpr int kMergeGroups = 2048;   // workgroups of the merge, about
-constexpr int kLeastKeys = 128;      // that a part of a block's keys is cut to
+constexpr int kLeastKeys = 128, kFewKeys = 2048;   // that a part of a block's keys is cut to; of short blocks
 // Scores are in units of log2: scale * log2(e) is an fp32 number, which it is up to 2.358e38.
 constexpr float kMaxScale = 2.3e38f;
 
@@ -154,13 +154,17 @@ Launch launch_of(const tv_window_attention_args* a) {
     n.block_ids = rows / n.shape.rows + a->num_requests;
     int64_t blocks = (rows + n.shape.rows - 1) / n.shape.rows;
     blocks = (blocks > a->num_requests ? blocks : a->num_requests) * a->num_kv_heads;
-    const int64_t least = n.shape.step > kLeastKeys ? n.shape.step : kLeastKeys;
+    // Few rows have small pieces, and their keys' latency is what they wait for: one request of 1 / 16 nodes over 1024 keys
+    // 12.8 / 15.7 us (with parts of 128 14.3 / 16.9), but 4 of 16 nodes over 1000 18.7 with 128 (23.2), 2 of 16 over 2820
+    // keys and 16 heads 21.3 (24.6).  Two parts of 128 do not pay for the merge: one request over 200 keys 14.1 (16.4).
+    const bool few = static_cast<int64_t>(a->total_queries) * a->num_q_heads < kManyRows && keys <= kFewKeys;
+    const int64_t least = few ? kLeastKeys / 2 : kLeastKeys;
     const int64_t most = (keys + least - 1) / least;
     const int64_t room = static_cast<int64_t>(a->compute_units) * n.shape.per_cu;
     int64_t splits = room / blocks;
     splits = splits < most ? splits : most;
     splits = splits < kMostSplits ? splits : kMostSplits;
-    n.splits = static_cast<int32_t>(splits > 1 ? splits : 1);
+    n.splits = static_cast<int32_t>(splits > 1 && most > 2 ? splits : 1);
     n.least_steps = static_cast<int32_t>(least / n.shape.step);
     // The parts are dealt out on the device, by the lengths there; a block takes one at least, and as many as its keys
     // allow at most.  32 query heads over 8 KV heads of 128, as many parts for every block in brackets: 8 requests of 40
@@ -302,7 +306,8 @@ extern "C" int tv_window_attention(const tv_window_attention_args* a, void* work
     p.splits = n.splits;
     p.least_steps = n.least_steps;
     // A group of lanes joins a row where there are rows for all, or few pieces; else a workgroup does.  One request of 1 /
-    // 16 nodes over 8192 keys 19 / 28 us (with groups of lanes 30 / 39), 4 of 64 69 (with workgroups 82), 8 of 40 56 (66).
+    // 16 nodes over 8192 keys 19 / 28 us (with groups of lanes 30 / 39), 4 of 64 69 (with workgroups 82), 8 of 40 56 (66), 32
+    // of 8 over 777 keys and one KV head 15.9 (20.2).
     p.row_slots = n.splits <= kFewPieces || static_cast<int64_t>(a->total_queries) * a->num_q_heads >= kManyRows;
     if (n.bytes) {
         const int64_t pieces = n.units * a->num_kv_heads * n.shape.rows;
