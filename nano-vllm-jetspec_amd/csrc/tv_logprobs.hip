@@ -16,7 +16,7 @@
 //
 // Memory bounds it where no alternatives are asked for (4096 rows of 151936 bf16 logits, 1.25 GB: 197 us, 6.3 TB/s);
 // the vector unit is as busy, ten instruction slots an element, of which the exponential takes four, and bounds it
-// with 20 alternatives (226 us; 316 with every element of a unit looked at where one passes, exchanges through LDS
+// with 20 alternatives (212 us; 316 with every element of a unit looked at where one passes, exchanges through LDS
 // and bounds of a wave's own).  8 rows with 5: 14 us, two launches' latencies.
 #include <math.h>
 #include <stdint.h>
