@@ -16,8 +16,8 @@
 //
 // Memory bounds it where no alternatives are asked for (4096 rows of 151936 bf16 logits, 1.25 GB: 197 us, 6.3 TB/s);
 // the vector unit is as busy, ten instruction slots an element, of which the exponential takes four, and bounds it
-// with 20 alternatives (212 us; 316 with every element of a unit looked at where one passes, exchanges through LDS
-// and bounds of a wave's own).  8 rows with 5: 14 us, two launches' latencies.
+// with 20 alternatives (207 us; 316 with every element of a unit looked at where one passes, exchanges through LDS
+// and bounds of a wave's own).  8 rows with 5: 12.7 us, two launches' latencies.
 #include <math.h>
 #include <stdint.h>
 
@@ -183,6 +183,7 @@ struct WaveTop {
     uint64_t kth = 0;      // the top-th of them
     uint64_t* queue;       // LDS of the wave's own: fewer than 64, and a push of up to 64
     int queued = 0, top;
+    bool held = false;     // anything in the list
 
     // One wave's exchange through LDS: its operations run in order, the compiler's must too.
     static __device__ __forceinline__ void settle() {
@@ -192,6 +193,7 @@ struct WaveTop {
     }
     // Merges the last 64 entries of the queue.
     __device__ __forceinline__ void flush() {
+        if (queued == 0) return;
         const int lane = threadIdx.x & 63, from = queued > 64 ? queued - 64 : 0;
         settle();
         const uint64_t mine = from + lane < queued ? queue[from + lane] : 0;
@@ -200,8 +202,12 @@ struct WaveTop {
     }
     // Merges another sorted list.
     __device__ __forceinline__ void merge(uint64_t list) {
-        const uint64_t other = lane_reversed(list);
-        best = merged(best > other ? best : other);
+        if (held) {
+            const uint64_t other = lane_reversed(list);
+            list = merged(best > other ? best : other);
+        }
+        held = true;
+        best = list;
         kth = of_lane(best, top - 1);
     }
     __device__ __forceinline__ void push(bool want, uint64_t entry) {
