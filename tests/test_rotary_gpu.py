@@ -97,7 +97,7 @@ def test_far_positions_and_scaled_frequencies():
     assert (np.abs(have - want) <= bound + 2.0 ** -20 * np.abs(s.q.double().cpu().numpy()).max()).all()
 
 
-def test_frequencies_gpu_free_formula():
+def test_frequencies_of_stretched_contexts():
     plain = rotary_frequencies(64, base=1e6)
     assert plain.dtype is torch.float64 and plain[0] == 1.0 and plain.shape == (32,)
     np.testing.assert_allclose(plain.numpy(), 1e6 ** (-np.arange(32) / 32), rtol=1e-14)
