@@ -33,8 +33,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kMargin = 8.0f;
 // R is c x rounded to fp32, and c x - R has to stay near zero for the x it was made of: so up to 2^16.  Larger
 // logits (masks of -1e9 or the type's lowest value) are summed against references of their own, below, to
-// zero, and above all others.  A row left with such a one is summed again, by differences.
-constexpr float kFar = 65536.0f, kFarLow = -9.0e4f, kFarHigh = 1.0e5f;
+// zero, and above all others.  A row left with such a one is summed again, by differences, and so is one whose largest
+// logit is within 100 of the far ones below it (its reference under kNearLow), whose terms a lane has lost when it saw
+// them before a near one.  Above that they are less than 2^-130 of the largest.
+constexpr float kFar = 65536.0f, kFarLow = -9.0e4f, kFarHigh = 1.0e5f, kNearLow = -9.44e4f;
 
 struct LogprobParams {
     const char* logits;
@@ -311,7 +313,7 @@ __device__ __forceinline__ void finish(const LogprobParams& p, int64_t i, int64_
     typedef typename T::storage S;
     const S* x = reinterpret_cast<const S*>(p.logits) + row * p.stride;
     double reference = static_cast<double>(sums.r) / static_cast<double>(kLog2e);
-    if (sums.r == kFarLow || sums.r == kFarHigh) reference = sum_far<T>(p, x, sums);
+    if (sums.r == kFarLow || sums.r == kFarHigh || (sums.r < kNearLow && sums.r > -INFINITY)) reference = sum_far<T>(p, x, sums);
     const double log_sum = static_cast<double>(log2f(sums.z)) / static_cast<double>(kLog2e);
     // A sum over nothing but -inf has no distribution.
     const bool none = !(sums.z > 0.0f);
