@@ -73,7 +73,7 @@ struct WindowParams {
     const float* bias;
     const int64_t* bias_off;
     int64_t bias_elems;
-    const int32_t* positions;      // low words
+    const int32_t* positions;      // int32, or int64 as its words
     int32_t pos_step;              // words from one to the next: 1 or 2
     int32_t num_requests, total_queries, num_kv_heads, groups;
     int32_t dim;                   // head size, a multiple of 8 up to the template's
@@ -289,6 +289,13 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch
     return true;
 }
 
+// Position i as it is given, in 32 bits: one that they do not hold is as far outside as they say.
+__device__ __forceinline__ int32_t win_given(const int32_t* positions, int32_t step, int64_t i) {
+    const int32_t low = positions[i * step], high = positions[i * step + step - 1];   // step 1: the same word
+    if (step == 1 || high == low >> 31) return low;
+    return high < 0 ? -0x7fffffff - 1 : 0x7fffffff;
+}
+
 // A node's position: the prefix length plus a depth that its index bounds.
 __device__ __forceinline__ int32_t win_position(const WinRequest& q, int node, int32_t given) {
     const int32_t most = q.prefix + node;
@@ -460,11 +467,9 @@ window_attention_kernel(const WindowParams p) {
     const int32_t* positions = p.positions + static_cast<int64_t>(req.first_row) * p.pos_step;
     int32_t lowest = 0x7fffffff, highest = 0;
     for (int n = node0 + lane; n <= node1; n += 64) {
-        const int32_t given = positions[static_cast<int64_t>(n) * p.pos_step];
+        const int32_t given = win_given(positions, p.pos_step, n);
         const int32_t at = win_position(req, n, given);
-        bool wrong = at != given;
-        if (p.pos_step == 2) wrong |= positions[static_cast<int64_t>(n) * 2 + 1] != 0;
-        if (wrong) set_status(p.status, TV_STATUS_BAD_POSITION);
+        if (at != given) set_status(p.status, TV_STATUS_BAD_POSITION);
         node_pos[n - node0] = at;   // by every wave, the same
         lowest = at < lowest ? at : lowest;
         highest = at > highest ? at : highest;
@@ -524,7 +529,7 @@ window_attention_kernel(const WindowParams p) {
             int32_t page = win_page_of(a->div_mul, a->div_shift, slot ? 0 : pos);
             const int32_t* from = slot ? reinterpret_cast<const int32_t*>(slots + t_of) : table + page;
             const int32_t entry = from[0], entry_high = from[slot ? 1 : 0];
-            const int32_t given = positions[static_cast<int64_t>(slot ? t_of : 0) * a->pos_step];
+            const int32_t given = win_given(positions, a->pos_step, slot ? t_of : 0);
             uint32_t offset = static_cast<uint32_t>(pos - page * a->block_size);
             if (slot) {
                 page = win_page_of(a->div_mul, a->div_shift, entry < 0 ? 0 : entry);
