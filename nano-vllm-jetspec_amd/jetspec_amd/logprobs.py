@@ -59,7 +59,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, *, top: int = 
     if count == 0:
         return logprobs, entropy, top_ids, top_logprobs
     args = _lib.pack_token_logprobs(
-        logits.data_ptr(), logits.stride(0), held, vocab, _device.dtype_code(logits.dtype),
+        # One row may have any row stride and still be contiguous; none is then used.
+        logits.data_ptr(), max(logits.stride(0), vocab), held, vocab, _device.dtype_code(logits.dtype),
         0 if rows is None else rows.data_ptr(), rows is not None and rows.dtype is torch.int64, token_ids.data_ptr(),
         token_ids.dtype is torch.int64, count, shape[1] if len(shape) == 2 else 1, top, logprobs.data_ptr(),
         entropy.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(), _device.compute_units(index),

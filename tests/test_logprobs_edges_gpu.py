@@ -1,10 +1,12 @@
-"""token_logprobs where its sums change their reference, against 64 bits (tolerances as derived in test_logprobs_gpu.py)."""
+"""token_logprobs where its sums change their reference, and single rows of any stride, against 64 bits (tolerances as
+derived in test_logprobs_gpu.py)."""
 from __future__ import annotations
 
 import pytest
 import torch
 
-from test_logprobs_gpu import DEV, F32, check, make
+from jetspec_amd import token_logprobs
+from test_logprobs_gpu import BF16, DEV, F32, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +44,22 @@ def test_rows_around_the_borders_of_far_values(centre):
     for rows in (x, x.repeat(100, 1)):
         tokens = torch.randint(0, 9001, (rows.shape[0],), device=DEV, generator=torch.Generator(DEV).manual_seed(2))
         check(rows, tokens, 7, label=f"around {centre}")
+
+
+@pytest.mark.parametrize("vocab", [1, 9, 2049, 50257])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_row_of_any_row_stride(vocab, dtype):
+    # A column of a product, transposed: [1, vocab] with strides (1, 1), which torch counts as contiguous.
+    column = make(vocab, 1, dtype, seed=vocab)
+    tokens = torch.tensor([[0, vocab - 1, vocab // 2]], device=DEV)
+    row = column.t()
+    assert row.stride() == (1, 1) and row.is_contiguous()
+    check(row, tokens, min(vocab, 5), label="transposed column")
+    same = row.clone(memory_format=torch.contiguous_format)
+    assert all(torch.equal(a, b) for a, b in zip(token_logprobs(row, tokens, top=1), token_logprobs(same, tokens, top=1)))
+    check(same.expand(4, vocab)[:1], tokens, 1, label="one of a broadcast row")      # a row stride of 0
+    picked = torch.tensor([0, -1, 0], device=DEV)
+    logp = token_logprobs(row, tokens.repeat(3, 1), rows=picked)[0]
+    assert torch.equal(logp[0], logp[2]) and (logp[1] == 0).all()
+    wide = make(vocab, 3, dtype, seed=7).t()[1:2]                                    # strides (1, 3)
+    check(wide, tokens, 1, label="strided column")
