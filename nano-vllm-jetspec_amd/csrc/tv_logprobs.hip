@@ -317,6 +317,11 @@ __device__ __forceinline__ void finish(const LogprobParams& p, int64_t i, int64_
     const double log_sum = static_cast<double>(log2f(sums.z)) / static_cast<double>(kLog2e);
     // A sum over nothing but -inf has no distribution.
     const bool none = !(sums.z > 0.0f);
+    // No logarithm of a probability is above zero, which the sum's rounding would make of a nearly certain word's.
+    auto logprob = [&](float logit) {
+        const float value = static_cast<float>(static_cast<double>(logit) - reference - log_sum);
+        return none ? NAN : value > 0.0f ? 0.0f : value;
+    };
     if (threadIdx.x == 0) {
         const float entropy = (log2f(sums.z) - sums.e / sums.z) / kLog2e;
         p.entropy[i] = none ? NAN : entropy < 0.0f ? 0.0f : entropy;
@@ -324,7 +329,7 @@ __device__ __forceinline__ void finish(const LogprobParams& p, int64_t i, int64_
     for (int j = threadIdx.x; j < p.given; j += kThreads) {
         const int64_t t = load_int(p.tokens, p.tokens64, i * p.given + j);
         float value = t == -1 ? 0.0f : NAN;
-        if (t >= 0 && t < p.vocab) value = none ? NAN : static_cast<float>(static_cast<double>(T::load(x[t])) - reference - log_sum);
+        if (t >= 0 && t < p.vocab) value = logprob(T::load(x[t]));
         else if (t != -1) set_status(p.status, TV_STATUS_BAD_REQUEST);
         p.logprobs[i * p.given + j] = value;
     }
@@ -332,8 +337,7 @@ __device__ __forceinline__ void finish(const LogprobParams& p, int64_t i, int64_
         const int j = threadIdx.x;
         if (j < p.top) {
             p.top_ids[i * p.top + j] = static_cast<int64_t>(~static_cast<uint32_t>(entry));
-            const float value = value_of(static_cast<uint32_t>(entry >> 32));
-            p.top_logprobs[i * p.top + j] = none ? NAN : static_cast<float>(static_cast<double>(value) - reference - log_sum);
+            p.top_logprobs[i * p.top + j] = logprob(value_of(static_cast<uint32_t>(entry >> 32)));
         }
     }
 }

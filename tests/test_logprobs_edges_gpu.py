@@ -1,12 +1,12 @@
-"""token_logprobs where its sums change their reference, and single rows of any stride, against 64 bits (tolerances as
-derived in test_logprobs_gpu.py)."""
+"""token_logprobs where its sums change their reference, where a row is nearly certain, and single rows of any stride,
+against 64 bits (tolerances as derived in test_logprobs_gpu.py)."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 from jetspec_amd import token_logprobs
-from test_logprobs_gpu import BF16, DEV, F32, check, make
+from test_logprobs_gpu import BF16, DEV, F16, F32, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -44,6 +44,22 @@ def test_rows_around_the_borders_of_far_values(centre):
     for rows in (x, x.repeat(100, 1)):
         tokens = torch.randint(0, 9001, (rows.shape[0],), device=DEV, generator=torch.Generator(DEV).manual_seed(2))
         check(rows, tokens, 7, label=f"around {centre}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_no_log_probability_is_above_zero(dtype):
+    rows, vocab = 4096, 1009
+    x = make(rows, vocab, dtype, gain=1.0, seed=3)
+    largest = torch.arange(rows, device=DEV) % vocab
+    margin = 18 + 20 * torch.rand(rows, device=DEV, generator=torch.Generator(DEV).manual_seed(4))
+    x[torch.arange(rows, device=DEV), largest] = margin.to(dtype)
+    x[7], x[7, 7] = -1.0e4, 0.0
+    if dtype is not F16:
+        x[8], x[8, 8] = -1.0e9, 3.0e6      # summed by differences
+    logp, entropy, ids, values = token_logprobs(x, largest, top=3)
+    assert (logp <= 0).all() and (values <= 0).all() and (entropy >= 0).all()
+    assert torch.equal(ids[:, 0], largest) and torch.equal(values[:, 0], logp)
+    check(x, largest, 3, label=f"certain {dtype}")
 
 
 @pytest.mark.parametrize("vocab", [1, 9, 2049, 50257])
