@@ -146,7 +146,7 @@ __device__ __forceinline__ WinRequest win_request(const WindowParams& p, int r, 
     // The rows, the bias and the table row have to hold what the lengths say.
     const int64_t square = static_cast<int64_t>(q.nodes) * q.nodes;
     bad = q.prefix < 0 || q.prefix > p.max_prefix || q.nodes < 0 || q.first_row < 0 || next > p.total_queries ||
-          q.first_row > next - q.nodes || q.bias < 0 || q.bias > p.bias_elems - square ||
+          static_cast<int64_t>(q.first_row) + q.nodes > next || q.bias < 0 || q.bias > p.bias_elems - square ||
           static_cast<int64_t>(q.prefix) + q.nodes > kWinMaxKeys;
     if (!bad) q.blocks = (q.nodes * p.groups + ROWS - 1) / ROWS;   // nodes * groups <= Q * heads < 2^31
     return q;

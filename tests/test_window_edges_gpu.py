@@ -1,11 +1,11 @@
-"""The windowed tree attention: positions that int32 does not hold."""
+"""The windowed tree attention: positions that int32 does not hold, and row offsets at its ends."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 from jetspec_amd import _lib, read_and_clear_status
-from test_window_attention_gpu import DEV, attend
+from test_window_attention_gpu import DEV, attend, trees
 from window_helpers import Batch, chain
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +28,27 @@ def test_int64_positions_outside_are_the_nearer_end(position, nearest):
     assert read_and_clear_status(DEV) == 0
     p[7] = 122 - nearest    # the other end, which would show
     assert not torch.equal(got, attend(b, positions=p))
+
+
+def test_offsets_of_rows_at_the_ends_of_int32():
+    # A request's rows begin past the batch and end at int32's lowest: left out, whatever the difference wraps to.
+    def fresh():
+        read_and_clear_status(DEV)
+        return Batch([50, 60, 70], trees([5, 5, 5]), window=30, seed=7)
+
+    good = attend(fresh())
+    for first, last in ((2 ** 30, -2 ** 31), (2 ** 31 - 1, -2 ** 31), (2 ** 31 - 1, 2 ** 31 - 1), (16, -2 ** 31 + 4), (5, -2 ** 31)):
+        b = fresh()
+        b.meta.cu_seqlens_q[1:3] = torch.tensor([first, last], dtype=torch.int32)
+        out = torch.full_like(b.q, 9.0)
+        attend(b, out=out)
+        assert read_and_clear_status(DEV) == _lib.TV_STATUS_BAD_REQUEST
+        if first == 5:
+            assert torch.equal(out[:5], good[:5])
+        assert (out[0 if first != 5 else 5:] == 9.0).all(), (first, last)
+    b = fresh()
+    b.meta.node_counts[1] = 2 ** 31 - 1
+    out = torch.full_like(b.q, 9.0)
+    attend(b, out=out)
+    assert read_and_clear_status(DEV) == _lib.TV_STATUS_BAD_REQUEST
+    assert torch.equal(out[:5], good[:5]) and torch.equal(out[10:], good[10:]) and (out[5:10] == 9.0).all()
