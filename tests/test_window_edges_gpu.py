@@ -1,12 +1,14 @@
-"""The windowed tree attention: positions that int32 does not hold, and row offsets at its ends."""
+"""The windowed tree attention: positions that int32 does not hold, requests of fewer nodes than rows, offsets past int32's
+ends, and infinities and NaN at every launch shape (tolerances as derived in test_window_attention_gpu.py)."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
 from jetspec_amd import _lib, read_and_clear_status
-from test_window_attention_gpu import DEV, attend, trees
-from window_helpers import Batch, chain
+from test_window_attention_gpu import BF16, DEV, F16, F32, attend, trees
+from window_helpers import Batch, chain, check
 
 pytestmark = pytest.mark.gpu
 
@@ -28,6 +30,89 @@ def test_int64_positions_outside_are_the_nearer_end(position, nearest):
     assert read_and_clear_status(DEV) == 0
     p[7] = 122 - nearest    # the other end, which would show
     assert not torch.equal(got, attend(b, positions=p))
+
+
+def staged(sizes, live, dim, seed, **options):
+    """A batch packed for `sizes` nodes a request of which `live` are counted."""
+    rng = np.random.default_rng(seed)
+    b = Batch([int(rng.integers(0, 90)) for _ in sizes], trees(sizes, seed), window=30, sinks=2, seed=seed, dim=dim, **options)
+    offsets = b.meta.qq_bias_offsets.tolist()
+    left = []
+    for r, (n, count) in enumerate(zip(sizes, live)):
+        square = b.meta.qq_bias[offsets[r]:offsets[r + 1]].view(n, n)[:count, :count].clone()
+        b.meta.qq_bias[offsets[r]:offsets[r + 1]].fill_(float("nan"))
+        b.meta.qq_bias[offsets[r]:offsets[r] + count * count] = square.reshape(-1)
+        left.append(torch.arange(n) >= count)
+    b.meta.node_counts.copy_(torch.tensor(live, dtype=torch.int32))
+    left = torch.cat(left).to(DEV)
+    b.meta.tree_slots[left] = -1
+    b.q[left] = float("nan")
+    return b, left
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("sizes, live", [([5, 5], [5, 3]), ([5, 5], [1, 4]), ([64, 40, 64], [64, 1, 33]), ([200, 140], [3, 129]),
+                                         ([6] * 70, [i % 7 for i in range(70)])])
+def test_requests_of_fewer_nodes_than_rows(sizes, live, dim):
+    b, left = staged(sizes, live, dim, len(sizes) + live[1])
+    out = torch.full_like(b.q, 9.0)
+    read_and_clear_status(DEV)
+    attend(b, out=out)
+    assert read_and_clear_status(DEV) == 0
+    assert (out[left] == 9.0).all()
+    # The rows that count, as a batch of their own for the 64-bit results.
+    b.q = b.q[~left]
+    b.keys = [(j, slots, own[:count]) for (j, slots, own), count in zip(b.keys, live)]
+    b.depths = [depth[:count] for depth, count in zip(b.depths, live)]
+    b.counts = live
+    check(out[~left], b, f"{sizes[:3]} {live[:3]} {dim}")
+
+
+VALUES = [(BF16, float("inf")), (BF16, float("nan")), (F16, float("-inf")), (F16, float("nan"))]
+ODD_SHAPES = [
+    # prefixes, trees, window, sinks, options: blocks of 32 to 256 rows, whole and in parts, one table of keys and many
+    ([100, 0], [8, 5], 43, 0, {}),
+    ([700], [200], 500, 4, dict(groups=1, kv_heads=2)),
+    ([900, 333], [150, 130], 700, 20, dict(groups=4, kv_heads=2)),
+    ([3000], [20], 2900, 8, dict(groups=4, kv_heads=2)),
+    ([60 + 5 * i for i in range(140)], [1 + i % 5 for i in range(140)], 50, 3, dict(groups=2, kv_heads=8)),
+]
+
+
+@pytest.mark.parametrize("dtype, value", VALUES)
+@pytest.mark.parametrize("dim", [64, 80, 128, 200, 256])
+@pytest.mark.parametrize("case", range(len(ODD_SHAPES)))
+def test_odd_keys_and_values_stay_with_the_rows_that_see_them(case, dim, dtype, value):
+    prefixes, sizes, window, sinks, options = ODD_SHAPES[case]
+    rng = np.random.default_rng(case)
+    parents = trees(sizes, case)
+    b, clean = (Batch(prefixes, parents, window=window, sinks=sinks, seed=case, dim=dim, dtype=dtype, **options) for _ in range(2))
+    bias, offsets = b.meta.qq_bias.cpu().numpy(), b.meta.qq_bias_offsets.tolist()
+    seen, k_pool, v_pool = [], b.k.view(-1, *b.k.shape[2:]), b.v.view(-1, *b.v.shape[2:])
+    for r, (j, slots, own) in enumerate(b.keys):
+        n, depth = sizes[r], b.depths[r]
+        at = np.concatenate([j, prefixes[r] + depth])
+        visible = np.concatenate([np.ones((n, len(j)), bool), bias[offsets[r]:offsets[r + 1]].reshape(n, n) == 0], 1)
+        mine = prefixes[r] + depth
+        visible &= (mine[:, None] - at[None] < window) | (at[None] < sinks)
+        # The first key that some row has lost, and nodes early, in the middle and last but one, where not all see them.
+        some = np.flatnonzero(~visible.all(0) & visible.any(0))
+        odd = some[:1].tolist() + [int(x) for x in rng.choice(some, size=min(3, len(some)), replace=False)] if len(some) else []
+        every = np.concatenate([slots, own])
+        for key in odd:
+            k_pool[int(every[key]), 1] = float("nan")
+            v_pool[int(every[key]), 0, dim - 3] = value
+        seen.append(visible[:, odd].any(1))
+    seen = np.concatenate(seen)
+    assert seen.any() and not seen.all()
+    want, bound = clean.expected(dtype)
+    groups = b.groups
+    for _ in range(2):
+        got = attend(b).double().cpu().numpy()
+        assert not np.isfinite(got[seen][:, :groups, dim - 3]).any()        # KV head 0: the value row
+        assert np.isnan(got[seen][:, groups:2 * groups]).all()              # KV head 1: the key row
+        off = np.abs(got - want) / bound
+        assert (off[~seen] <= 1).all() and (off[:, 2 * groups:] <= 1).all()
 
 
 def test_offsets_of_rows_at_the_ends_of_int32():
