@@ -20,23 +20,37 @@ _VALUE_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, factor: float = 1.0, original_length: int | None = None,
-                       slow: float = 1.0, fast: float = 32.0, device=None) -> torch.Tensor:
+                       slow: float = 1.0, fast: float = 32.0, ramp: str = "turns", device=None) -> torch.Tensor:
     """float64 [rotary_dim / 2] radians a position: ``base ** (-2p / rotary_dim)``, for ``factor`` times longer contexts.
 
     Without ``original_length`` all are divided by ``factor`` (positions interpolated).  With it, frequencies
     that turn more than ``fast`` times over that length stay, those below ``slow`` turns are divided, and those
-    between are blended linearly in their turns.  ``rotary_scatter`` takes a scaling's amplitude as ``gain``.
+    between are blended.  The blend is part of what a checkpoint was trained with, and the two in use differ by tens
+    of percent: ``ramp="turns"`` is linear in a frequency's turns, ``ramp="pairs"`` in its index, between the
+    index of ``fast`` turns rounded down and that of ``slow`` turns rounded up, as checkpoints with thresholds of 1 and 32
+    mostly have it.  ``rotary_scatter`` takes a scaling's amplitude as ``gain``.
     """
     if isinstance(rotary_dim, bool) or not isinstance(rotary_dim, int) or rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rotary_dim must be a positive even int")
     if not 0 < base < math.inf or not 0 < factor < math.inf:
         raise ValueError("base and factor must be positive and finite")
+    if ramp not in ("turns", "pairs"):
+        raise ValueError("ramp must be 'turns' or 'pairs'")
+    if ramp == "pairs" and (base <= 1 or slow <= 0):
+        raise ValueError("a ramp over pairs needs a base above 1 and slow above 0")
     plain = torch.tensor([base ** (-2 * p / rotary_dim) for p in range(rotary_dim // 2)], dtype=torch.float64)
     if original_length is None:
         return (plain / factor).to(device)
     if original_length <= 0 or not 0 <= slow < fast < math.inf:
         raise ValueError("original_length must be positive, and slow below fast")
-    keep = ((plain * original_length / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+    if ramp == "turns":
+        keep = ((plain * original_length / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+    else:
+        # base ** (-2p / rotary_dim) turns t times over the length at this p.
+        first, last = (rotary_dim * math.log(original_length / (2 * math.pi * t)) / (2 * math.log(base)) for t in (fast, slow))
+        first, last = max(math.floor(first), 0), min(math.ceil(last), rotary_dim - 1)
+        at = torch.arange(rotary_dim // 2, dtype=torch.float64)
+        keep = ((last - at) / max(last - first, 1e-3)).clamp(0, 1)
     return (plain * (keep + (1 - keep) / factor)).to(device)
 
 
