@@ -782,6 +782,8 @@ int tv_tree_attention_e4m3(const tv_tree_attention_e4m3_args* args, void* worksp
  * TV_STATUS_BAD_REQUEST and are left out; pages and slots outside the pool record
  * TV_STATUS_BAD_PAGE and their keys are skipped.  An infinite or NaN value row makes NaN
  * of a row that sees it, or keeps its infinities; rows that do not see it are unaffected.
+ * For output of the queries' type a probability is rounded to that type once before its
+ * product with V (bf16 2^-8 of it, f16 2^-11), for fp32 output it is kept to 2^-26 / 2^-23.
  * `workspace` is tv_window_attention_workspace_bytes() bytes (it may be 0), the call's own
  * until its work is done.
  */

@@ -605,9 +605,9 @@ logprobs_join_kernel(const LogprobParams p) {
 }
 
 // Parts of a row: three workgroups a compute unit where there are not two rows for each, since every part begins its
-// bounds anew and the join is a launch; a part is at least 4 units a thread.  700 / 1000 rows with 20 alternatives (151936
-// and 50257 words of bf16) whole 48 / 29 us, in two parts 54 / 36; 64 in 12 parts 17.5, in 16 20.2; 333 fp32 rows of 50257 in
-// 3 parts 16.2, in 2 17.2, in 4 17.9.
+// bounds anew and the join is a launch; the shortest parts have 2 to 4 units a thread.  700 / 1000 rows with 20
+// alternatives (151936 and 50257 words of bf16) whole 48 / 29 us, in two parts 54 / 36; 64 in 12 parts 17.5, in 16 20.2;
+// 333 fp32 rows of 50257 in 3 parts 16.2, in 2 17.2, in 4 17.9.
 int64_t splits_of(const tv_token_logprobs_args* a) {
     const int64_t vec = a->dtype == TV_F32 ? 4 : 8;
     const int64_t most = (a->vocab / vec + kThreads * kUnroll - 1) / (kThreads * kUnroll);

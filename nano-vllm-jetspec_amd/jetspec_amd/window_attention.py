@@ -28,7 +28,9 @@ def packed_window_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     length plus the node's depth, as the rotation takes them.  One outside [prefix, prefix + node] is taken as
     the nearer end and records TV_STATUS_BAD_POSITION.  Finite ``qq_bias`` values are added to the scores.
     The result is new, or ``out``, in q's dtype or FP32; a row that sees no key is zero, one that no request
-    counts (padding of a captured batch) is left as it was.
+    counts (padding of a captured batch) is left as it was.  For a result in q's dtype each probability is rounded to
+    it (BF16 2^-8, FP16 2^-11 of it) before it meets V; ``output_dtype=torch.float32`` keeps more (2^-26, 2^-23).
+    A row that sees a NaN or infinity in V has NaN or keeps the infinity, in that dimension or in all.
 
     Every length, page and position is read on the device, so a captured call follows the staged metadata,
     and no state is kept between calls.  Requests that reach outside the batch, the bias or their table row
