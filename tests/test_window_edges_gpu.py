@@ -137,3 +137,17 @@ def test_offsets_of_rows_at_the_ends_of_int32():
     attend(b, out=out)
     assert read_and_clear_status(DEV) == _lib.TV_STATUS_BAD_REQUEST
     assert torch.equal(out[:5], good[:5]) and torch.equal(out[10:], good[10:]) and (out[5:10] == 9.0).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("first", [True, False])
+def test_single_tokens_and_a_chunk_in_one_call(dim, first):
+    # The row blocks go by the average: a chunk among single tokens runs in blocks that are small for it.
+    prefixes, sizes = [7 * i % 311 for i in range(63)], [1] * 63
+    prefixes.insert(0 if first else 40, 900)
+    sizes.insert(0 if first else 40, 512)
+    for window, sinks in ((200, 4), (2 ** 20, 0)):
+        b = Batch(prefixes, [chain(n) for n in sizes], window=window, sinks=sinks, dim=dim, kv_heads=8, groups=2, seed=dim)
+        read_and_clear_status(DEV)
+        check(attend(b), b, f"mixed {dim} {window}")
+        assert read_and_clear_status(DEV) == 0
