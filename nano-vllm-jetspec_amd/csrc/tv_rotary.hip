@@ -14,8 +14,9 @@
 // once, an angle a lane, and deals them out through LDS while the first heads are on their way.  A pass's
 // elements are loaded while the one before it is computed.
 //
-// Memory bounds it: 4096 rows of 32 + 8 heads of 128 in bf16 with 64 dimensions turned, 101 MB, 18.0 us (5.6 TB/s);
-// 6001 fp32 rows of 10 + 5 heads of 80, 77 MB, 15.5 us (5.0).  16 rows 3.7 us: a launch and three dependent loads.
+// Memory bounds it: 4096 rows of 32 + 8 heads of 128 in bf16 with 64 dimensions turned, 101 MB, 18.0 us (5.6 TB/s) out
+// of the Infinity Cache and 26.0 (3.9) out of memory, where a copy of as many bytes takes 15.6 and 21.0; 6001 fp32 rows
+// of 10 + 5 heads of 80, 77 MB, 15.2 and 22.  16 rows 3.7 us: a launch and three dependent loads.
 #include <math.h>
 #include <stdint.h>
 
@@ -286,7 +287,9 @@ rotary_kernel(const RotaryParams) {
 }
 
 // Waves that fill the chip's 1024 SIMDs: with fewer rows than that a row's heads are spread over
-// several waves, since what counts there is the latency of one.
+// several waves, since what counts there is the latency of one.  16 / 256 / 1024 / 2048 rows of 32 + 8 heads of 128 in
+// bf16 3.7 / 4.2 / 6.3 / 9.9 us; with 2048 waves 3.7 / 4.2 / 6.5 / 10.6, with 8192 3.7 / 4.2 / 6.6 / 10.3, with a wave a
+// row 5.9 / 6.2 / 7.3 / 10.6.
 constexpr int64_t kFullWaves = 4096;
 
 template <class T, int VEC, int GS, int NP, bool INTER>
@@ -314,7 +317,8 @@ int by_lanes(RotaryParams& p, hipStream_t stream) {
 }
 
 // VEC dimensions a lane in either place: both the pairs and what is copied have to be whole pieces, and
-// every address a multiple of one.
+// every address a multiple of one.  Pieces of 16 and 8 bytes are built, and single elements for whatever else: 4096 rows
+// of 32 + 8 heads of 80 in bf16 with 16 / 40 / 20 turned dimensions (8, 20, 10 pairs) 13.6 / 15.1 / 31.1 us.
 template <class T>
 int by_size(RotaryParams& p, int64_t vec, hipStream_t stream) {
     constexpr int kVec = 16 / sizeof(typename T::storage);

@@ -31,9 +31,10 @@
 // the next tile are multiplied in turn with the values of this one, each operand read kAhead products before.
 // A row's reference is raised only when a tile's probabilities would pass 2^8, so most tiles rescale nothing.
 //
-// 32 query heads over 8 KV heads of 128, bf16: 64 trees of 64 nodes over 8192 keys each are bound by the matrix
-// units, 725 us at 0.76 PFLOP/s (keys through registers, and a reach test and a bias read for every score,
-// took 1302); 128 single tokens over 4096 keys by memory, 376 us at 5.7 TB/s (484).
+// 32 query heads over 8 KV heads of 128, bf16: 64 trees of 64 nodes over 8192 keys each take 670 to 690 us, 0.80
+// PFLOP/s, the matrix and the vector units busy 40 and 38 % of the time, hardly at once, since a tile's exponentials stand
+// before its step's products (keys through registers, and a reach test and a bias read for every score, took 1302);
+// 128 single tokens over 4096 keys are bound by memory, 376 us at 5.7 TB/s (484).
 //
 // A probability is rounded to the operands' type once where the result is of that type, since the matrix unit takes both
 // operands in one type and each further term is as many products of P . V again.  The sum is of the rounded ones, so an
@@ -661,7 +662,9 @@ window_attention_kernel(const WindowParams p) {
     };
     // Rows that do not see a key have to get zero from its V row, and zero times NaN or infinity is not.  So where some
     // node does not see all of a step, each thread, behind its own loads, makes zeros of such elements, and the key's
-    // scores NaN instead, which hidden scores never show.  It also clears what lies behind a head's end.
+    // scores NaN instead, which hidden scores never show.  It also clears what lies behind a head's end, in every step of a
+    // head size between the templates': 64 trees of 8 nodes over 4096 keys and 8 KV heads of 64 / 72 / 96 / 120 / 128 / 136 /
+    // 192 / 248 / 256 take 114 / 192 / 199 / 229 / 200 / 456 / 483 / 508 / 389 us.
     auto mend = [&](int j) {
         const bool whole = p.dim == D;
         if (hiding_tiles(j) == 0 && whole) return;

@@ -142,8 +142,10 @@ Launch launch_of(const tv_window_attention_args* a) {
     keys = keys < reach + nodes ? keys : reach + nodes;
     // Blocks have at most 128 nodes.  256 rows read their keys once for twice the rows, 128 are two workgroups a compute
     // unit, one of which fills the other's start and end: 32 query heads over 8 KV heads of 128, 4 chains of 1024 nodes,
-    // window 128 / 512 / 1024 / 4096: 128 rows 55 / 97 / 149 / 393 us, 256 rows 70 / 108 / 142 / 329; 64 trees of 64 nodes,
-    // 512 / 1024 / 4096: 85 / 142 / 408 and 93 / 141 / 358.
+    // window 128 / 512 / 1024 / 4096: 128 rows 52 / 91 / 136 / 355 us, 256 rows 67 / 102 / 138 / 328; 64 trees of 64 nodes,
+    // 512 / 1024 / 4096: 79 / 131 / 393 and 88 / 131 / 365.
+    // One chunk among single tokens runs in the blocks of the average: 63 tokens and a chunk of 512 / 2048 nodes, window
+    // 4096, 277 / 394 us, the tokens alone 205 and the chunk 73 / 199; at head size 64 155 / 285, alone 118 and 54 / 145.
     if (average > 128 && (groups == 1 || keys < kLongRun)) average = 128;
     Launch n;
     n.width = a->head_dim <= 64 ? 64 : a->head_dim <= 128 ? 128 : 256;
@@ -155,8 +157,9 @@ Launch launch_of(const tv_window_attention_args* a) {
     int64_t blocks = (rows + n.shape.rows - 1) / n.shape.rows;
     blocks = (blocks > a->num_requests ? blocks : a->num_requests) * a->num_kv_heads;
     // Few rows have small pieces, and their keys' latency is what they wait for: one request of 1 / 16 nodes over 1024 keys
-    // 12.8 / 15.7 us (with parts of 128 14.3 / 16.9), but 4 of 16 nodes over 1000 18.7 with 128 (23.2), 2 of 16 over 2820
-    // keys and 16 heads 21.3 (24.6).  Two parts of 128 do not pay for the merge: one request over 200 keys 14.1 (16.4).
+    // 13.1 / 15.7 us (with parts of 128 14.6 / 16.9), over 200 keys 12.5 (16.4), but 4 of 16 nodes over 1000 18.4 with 128
+    // (23.3).  Two parts do not pay for the merge: one token and a window of 100 11.8 in one (12.6), 32 and of 200 15.4
+    // (19.4).
     const bool few = static_cast<int64_t>(a->total_queries) * a->num_q_heads < kManyRows && keys <= kFewKeys;
     const int64_t least = few ? kLeastKeys / 2 : kLeastKeys;
     const int64_t most = (keys + least - 1) / least;
@@ -167,8 +170,9 @@ Launch launch_of(const tv_window_attention_args* a) {
     n.splits = static_cast<int32_t>(splits > 1 && most > 2 ? splits : 1);
     n.least_steps = static_cast<int32_t>(least / n.shape.step);
     // The parts are dealt out on the device, by the lengths there; a block takes one at least, and as many as its keys
-    // allow at most.  32 query heads over 8 KV heads of 128, as many parts for every block in brackets: 8 requests of 40
-    // nodes over 4096 keys 66 us (80), 4 of 8 to 60 nodes over 100 to 8192 keys 53 (61).
+    // allow at most.  32 query heads over 8 KV heads of 128, as many parts for every block in brackets: 8 requests of 1 to
+    // 64 nodes over 100 to 16384 keys 91 us (109), 16 of 1 to 16 over 10 to 8192 61 (72), 4 of 8 to 60 over 100 to 8192 51
+    // (55); where the lengths are alike it gains nothing (8 of 40 over 4096 keys 57 (57), one token 13.0 (11.7)).
     n.units = n.block_ids * n.splits;
     if (n.splits > 1 && a->num_requests <= 64) {
         n.units = n.block_ids * (most < kMostSplits ? most : kMostSplits);
@@ -306,8 +310,8 @@ extern "C" int tv_window_attention(const tv_window_attention_args* a, void* work
     p.splits = n.splits;
     p.least_steps = n.least_steps;
     // A group of lanes joins a row where there are rows for all, or few pieces; else a workgroup does.  One request of 1 /
-    // 16 nodes over 8192 keys 19 / 28 us (with groups of lanes 30 / 39), 4 of 64 69 (with workgroups 82), 8 of 40 56 (66), 32
-    // of 8 over 777 keys and one KV head 15.9 (20.2).
+    // 16 nodes over 8192 keys 18 / 27 us (with groups of lanes 28 / 36), 4 of 64 68 (with workgroups 80), 8 of 40 over 4096
+    // keys 55 (65), 32 of 8 over 777 keys and one KV head 18.3 (19.8).
     p.row_slots = n.splits <= kFewPieces || static_cast<int64_t>(a->total_queries) * a->num_q_heads >= kManyRows;
     if (n.bytes) {
         const int64_t pieces = n.units * a->num_kv_heads * n.shape.rows;

@@ -4,8 +4,11 @@
 namespace tv {
 
 // Up to 32 rows: two workgroups of two waves and one buffer a compute unit where there are as many, else larger ones.
-// 100 trees of 4 nodes over 1024 keys and 8 KV heads 190 us, 64 single tokens over 512 57 (with 64 rows 214 and 64); 32
+// 100 trees of 4 nodes over 1024 keys and 8 KV heads 190 us, 64 single tokens over 512 58 (with 64 rows 213 and 66); 32
 // trees of 8 nodes over 4096 182, 32 single tokens over 512 33 (with 32 rows 264 and 44).
+// Up to 64 rows in blocks of 64, more in blocks of 128: 4 heads a group over 4096 keys, 8 requests of 9 / 16 nodes 60 / 63
+// us, 32 of them 195 / 196 (with 128 rows 72 / 73 and 221 / 222); 8 of 24 / 64 nodes 79 / 139, 32 of 32 254 (with 64 rows 91 /
+// 154 and 320).
 WindowShape window_shape_d256(int64_t average_rows, int64_t per_cu) {
     if (average_rows <= 32 && per_cu >= 2) return {32, 128, 2, 64};
     if (average_rows <= 64) return {64, 256, 1, 64};

@@ -4,11 +4,11 @@
 namespace tv {
 
 // Up to 32 rows: four workgroups of two waves a compute unit where there are as many, else larger ones, which have more
-// keys on their way.  128 single tokens over 512 keys and 8 KV heads 32 us, 200 trees of 4 nodes over 1024 106 (with 64
-// rows 40 and 117); 64 single tokens over 512 20, 64 trees of 8 nodes over 4096 114 (with 32 rows 26 and 149).
-// Up to 64: 64 trees of 16 nodes over 4096 115 (with 128 rows 130).
-// From 129 on 256: 32 requests of 33 / 40 / 56 nodes and 4 heads a group over 4096 112 / 114 / 128 us (with 128:
-// 134 / 136 / 128).
+// keys on their way.  128 single tokens over 512 keys and 8 KV heads 31 us, 200 trees of 4 nodes over 1024 111 (with 64
+// rows 40 and 120); 64 single tokens over 512 20, 64 trees of 8 nodes over 4096 114 (with 32 rows 26 and 149).
+// Up to 64: 64 trees of 16 nodes over 4096 117 (with 128 rows 124).
+// From 129 on 256: 32 requests of 33 / 40 / 56 nodes and 4 heads a group over 4096 103 / 104 / 114 us (with 128:
+// 126 / 125 / 129).
 WindowShape window_shape_d64(int64_t average_rows, int64_t per_cu) {
     if (average_rows <= 32 && per_cu >= 4) return {32, 128, 4, 64};
     if (average_rows <= 64) return {64, 256, 2, 64};
