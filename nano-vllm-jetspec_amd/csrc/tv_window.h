@@ -290,7 +290,9 @@ __device__ __forceinline__ bool win_find(const WindowParams& p, int32_t* scratch
     block.parts = p.splits;
     block.first = id * p.splits;
     block.split = unit - (BY_PART ? block.first : unit);
-    return true;
+    // Requests that overlap by the ten thousands wrap the sums, and two threads can have found a block, one of which wrote
+    // the request and the other the number.
+    return static_cast<uint32_t>(block.b) < static_cast<uint32_t>(block.req.blocks);
 }
 
 // Position i as it is given, in 32 bits: one that they do not hold is as far outside as they say.

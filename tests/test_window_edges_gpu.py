@@ -1,12 +1,15 @@
-"""The windowed tree attention: positions that int32 does not hold, requests of fewer nodes than rows, offsets past int32's
-ends, and infinities and NaN at every launch shape (tolerances as derived in test_window_attention_gpu.py)."""
+"""The windowed tree attention: positions that int32 does not hold, requests of fewer nodes than rows, offsets at int32's ends,
+infinities and NaN at every launch shape, unlike and overlapping requests (tolerances as derived in
+test_window_attention_gpu.py)."""
 from __future__ import annotations
+
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
 import torch
 
-from jetspec_amd import _lib, read_and_clear_status
+from jetspec_amd import _lib, packed_window_attention, read_and_clear_status
 from test_window_attention_gpu import BF16, DEV, F16, F32, attend, trees
 from window_helpers import Batch, chain, check
 
@@ -151,3 +154,29 @@ def test_single_tokens_and_a_chunk_in_one_call(dim, first):
         read_and_clear_status(DEV)
         check(attend(b), b, f"mixed {dim} {window}")
         assert read_and_clear_status(DEV) == 0
+
+
+def test_requests_that_overlap_beyond_what_32_bits_count():
+    # Every second request holds all rows (each tenth of them the first one only), and the others begin where they end:
+    # 2.3 times 2^31 row blocks in all.  Which of them are computed is open, but with a window of one a row that is has its
+    # own V row.
+    requests, nodes, groups, dim = 106001, 1100, 3000, 8
+    cu = torch.zeros(requests + 1, dtype=torch.int32)
+    cu[1::2] = nodes
+    counts = torch.full((requests,), nodes, dtype=torch.int32)
+    counts[::20] = 1
+    bias = torch.full((nodes, nodes), -torch.inf).triu(1).reshape(-1)
+    gen = torch.Generator(DEV).manual_seed(1)
+    k, v = (torch.randn((5, 256, 1, dim), generator=gen, device=DEV).to(BF16) for _ in range(2))
+    q = torch.randn((nodes, groups, dim), generator=gen, device=DEV).to(BF16)
+    slots = torch.randperm(5 * 256, generator=gen, device=DEV)[:nodes]
+    meta = SimpleNamespace(cu_seqlens_q=cu.to(DEV), prefix_lens=torch.zeros(requests, dtype=torch.int32, device=DEV),
+                           node_counts=counts.to(DEV), block_tables=torch.zeros((requests, 1), dtype=torch.int32, device=DEV),
+                           tree_slots=slots, qq_bias=bias.to(DEV), block_size=256, num_requests=requests, total_queries=nodes,
+                           qq_bias_offsets=torch.zeros(requests + 1, dtype=torch.int64, device=DEV))
+    out = torch.full_like(q, 9.0)
+    read_and_clear_status(DEV)
+    packed_window_attention(q, k, v, meta, torch.arange(nodes, device=DEV), 0.3, groups, window=1, out=out)
+    assert read_and_clear_status(DEV) == _lib.TV_STATUS_BAD_REQUEST
+    own = v.view(-1, 1, dim)[slots].expand_as(out)
+    assert ((out == own) | (out == 9.0)).all()
