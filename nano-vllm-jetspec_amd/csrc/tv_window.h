@@ -31,8 +31,8 @@
 // the next tile are multiplied in turn with the values of this one, each operand read kAhead products before.
 // A row's reference is raised only when a tile's probabilities would pass 2^8, so most tiles rescale nothing.
 //
-// 32 query heads over 8 KV heads of 128, bf16: 64 trees of 64 nodes over 8192 keys each take 670 to 690 us, 0.80
-// PFLOP/s, the matrix and the vector units busy 40 and 38 % of the time, hardly at once, since a tile's exponentials stand
+// 32 query heads over 8 KV heads of 128, bf16: 64 trees of 64 nodes over 8192 keys each take 666 to 705 us by the box,
+// 0.78 to 0.82 PFLOP/s, the matrix and the vector units busy 40 and 38 % of the time, hardly at once, since a tile's exponentials stand
 // before its step's products (keys through registers, and a reach test and a bias read for every score, took 1302);
 // 128 single tokens over 4096 keys are bound by memory, 376 us at 5.7 TB/s (484).
 //
